@@ -590,10 +590,13 @@ void clear_status(int64_t device) { status_tensor(static_cast<int>(device)).zero
 }  // namespace
 
 void bind_sequence_ops(pybind11::module& m);   // bindings_seq.cpp
+void bind_tuning_ops(pybind11::module& m);     // bindings_tuning.cpp
+int* nmtg_status_word(int device) { return status_tensor(device).data_ptr<int>(); }
 extern "C" long nmtg_bounds_violations();
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   bind_sequence_ops(m);
+  bind_tuning_ops(m);
   m.def("gemm", &gemm, pybind11::arg("a"), pybind11::arg("a_mn_major"), pybind11::arg("b"), pybind11::arg("b_mn_major"), pybind11::arg("out"),
         pybind11::arg("bias"), pybind11::arg("residual"), pybind11::arg("aux"), pybind11::arg("preact"), pybind11::arg("act"),
         pybind11::arg("dropout_p"), pybind11::arg("seed"), pybind11::arg("stream_id"), pybind11::arg("alpha"), pybind11::arg("accumulate"),

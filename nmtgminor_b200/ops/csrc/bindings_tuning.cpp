@@ -1,0 +1,182 @@
+// Python bindings of the preference-tuning kernels declared in tuning_api.h.  Outputs and workspaces are allocated here, for the call
+// alone: two calls on two streams, or two captured graphs, share nothing.
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include "tuning_api.h"
+
+int* nmtg_status_word(int device);   // bindings.cpp
+
+namespace {
+
+using torch::Tensor;
+using OptTensor = c10::optional<Tensor>;
+
+cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+void ck(const char* err) {
+  if (err) throw std::runtime_error(std::string("nmtgminor_b200 kernel launch failed: ") + err);
+}
+int dtype_code(const Tensor& t, const char* name) {
+  if (t.scalar_type() == at::kFloat) return 0;
+  if (t.scalar_type() == at::kBFloat16) return 1;
+  if (t.scalar_type() == at::kHalf) return 2;
+  TORCH_CHECK(false, name, " must be float32, bfloat16 or float16");
+  return -1;
+}
+uintptr_t address(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()); }
+void need(const Tensor& t, const Tensor& like, at::ScalarType ty, int64_t n, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.is_contiguous() && t.scalar_type() == ty && t.numel() == n, name,
+              ": wrong device, layout, dtype or size");
+}
+const float* opt_f32(const OptTensor& t, const Tensor& like, int64_t n, const char* name) {
+  if (!t.has_value()) return nullptr;
+  need(*t, like, at::kFloat, n, name);
+  return t->data_ptr<float>();
+}
+
+// logits [rows, vocab] with adjacent elements in rows that do not overlap, labels [rows]
+NmtgRows rows_of(const Tensor& logits, const Tensor& labels, int64_t pad, double temperature) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.size(1) >= 1 && (logits.stride(1) == 1 || logits.size(1) == 1),
+              "logits must be rows of adjacent elements on a GPU");
+  TORCH_CHECK(logits.size(0) <= 1 || logits.stride(0) >= logits.size(1), "the rows of the logits overlap");
+  TORCH_CHECK(logits.size(0) < (1 << 30) && logits.size(1) < (1LL << 31) - 64, "logits: too many rows or words");
+  need(labels, logits, at::kLong, logits.size(0), "labels");
+  TORCH_CHECK(temperature > 0.0 && std::isfinite(1.0 / temperature), "temperature must be positive");
+  NmtgRows r = {};
+  r.logits = logits.data_ptr();
+  r.labels = labels.data_ptr<int64_t>();
+  r.rows = static_cast<int>(logits.size(0));
+  r.vocab = static_cast<int>(logits.size(1));
+  r.dtype = dtype_code(logits, "logits");
+  r.ld = logits.size(0) > 1 ? logits.stride(0) : logits.size(1);
+  r.inv_temperature = static_cast<float>(1.0 / temperature);
+  r.pad = pad;
+  r.grad_scale = 1.f;
+  r.status = nmtg_status_word(logits.get_device());
+  TORCH_CHECK(address(logits) % logits.element_size() == 0, "logits: misaligned elements");
+  return r;
+}
+
+// a gradient laid out as the logits are: the same row stride, the same address modulo 16 bytes
+Tensor grad_like(const Tensor& logits, const NmtgRows& r) {
+  const int64_t before = static_cast<int64_t>(address(logits) % 16) / logits.element_size();
+  const int64_t n = r.rows > 0 ? (r.rows - 1) * r.ld + r.vocab : 0;
+  return at::empty({before + n}, logits.options().requires_grad(false)).as_strided({r.rows, r.vocab}, {r.ld, 1}, before);
+}
+
+std::tuple<Tensor, Tensor> row_scores(const Tensor& logits, const Tensor& labels, int64_t pad, double temperature, bool keep_stat) {
+  NmtgRows r = rows_of(logits, labels, pad, temperature);
+  c10::cuda::CUDAGuard guard(logits.device());
+  const auto f32 = logits.options().dtype(at::kFloat).requires_grad(false);
+  Tensor lp = at::empty({r.rows}, f32), stat = at::empty({keep_stat ? r.rows : 0, 2}, f32);
+  r.logprobs = lp.data_ptr<float>();
+  r.stat = keep_stat ? reinterpret_cast<float2*>(stat.data_ptr<float>()) : nullptr;
+  ck(nmtg_row_scores(&r, cur_stream()));
+  return {lp, stat};
+}
+
+Tensor row_scores_grad(const Tensor& logits, const Tensor& labels, const Tensor& stat, const Tensor& weight, int64_t pad, double temperature) {
+  NmtgRows r = rows_of(logits, labels, pad, temperature);
+  c10::cuda::CUDAGuard guard(logits.device());
+  need(stat, logits, at::kFloat, 2 * static_cast<int64_t>(r.rows), "stat");
+  need(weight, logits, at::kFloat, r.rows, "weight");
+  Tensor grad = grad_like(logits, r);
+  r.grad = grad.data_ptr();
+  r.stat = reinterpret_cast<float2*>(stat.data_ptr<float>());
+  ck(nmtg_row_scores_grad(&r, weight.data_ptr<float>(), cur_stream()));
+  return grad;
+}
+
+// grad: 0 none, 1 a new tensor, 2 over the logits
+Tensor grad_of(const Tensor& logits, NmtgRows& r, int64_t grad, const OptTensor& scale_at, double scale) {
+  r.grad_scale = static_cast<float>(scale);
+  r.grad_scale_at = opt_f32(scale_at, logits, 1, "grad_scale");
+  Tensor g;
+  if (grad == 0) return g;
+  g = grad == 2 ? logits.detach() : grad_like(logits, r);
+  r.grad = g.data_ptr();
+  return g;
+}
+
+// -> loss, words clipped, KL, log-probabilities, gradient (or nothing)
+std::tuple<Tensor, Tensor, Tensor, Tensor, OptTensor> policy_loss(const Tensor& logits, const Tensor& labels, const Tensor& old_logprobs,
+                                                                  const Tensor& advantages, const OptTensor& ref_logprobs, double clip_low,
+                                                                  double clip_high, double kl_coef, int64_t pad, double temperature,
+                                                                  int64_t grad, const OptTensor& scale_at, double scale) {
+  NmtgRows r = rows_of(logits, labels, pad, temperature);
+  c10::cuda::CUDAGuard guard(logits.device());
+  NmtgPolicy p = {};
+  need(old_logprobs, logits, at::kFloat, r.rows, "old_logprobs");
+  need(advantages, logits, at::kFloat, r.rows, "advantages");
+  p.old_logprobs = old_logprobs.data_ptr<float>();
+  p.advantages = advantages.data_ptr<float>();
+  p.ref_logprobs = opt_f32(ref_logprobs, logits, r.rows, "ref_logprobs");
+  p.clip_low = static_cast<float>(1.0 - clip_low);
+  p.clip_high = static_cast<float>(1.0 + clip_high);
+  p.kl_coef = static_cast<float>(kl_coef);
+  const auto f32 = logits.options().dtype(at::kFloat).requires_grad(false);
+  Tensor lp = at::empty({r.rows}, f32), loss = at::empty({1}, f32), kl = at::empty({1}, f32), clipped = at::empty({1}, f32), rows = at::empty({3, r.rows}, f32.dtype(at::kDouble));
+  Tensor g = grad_of(logits, r, grad, scale_at, scale);
+  r.logprobs = lp.data_ptr<float>();
+  p.row_loss = rows.data_ptr<double>();
+  p.loss = loss.data_ptr<float>();
+  p.kl = kl.data_ptr<float>();
+  p.clipped = clipped.data_ptr<float>();
+  ck(nmtg_policy_loss(&r, &p, cur_stream()));
+  return {loss, clipped, kl, lp, g.defined() ? OptTensor(g) : OptTensor()};
+}
+
+// -> loss, pairs ranked as preferred, sequences' log-probabilities, gradient (or nothing)
+std::tuple<Tensor, Tensor, Tensor, OptTensor> preference_loss(const Tensor& logits, const Tensor& labels, const Tensor& cu, const OptTensor& ref,
+                                                              int64_t kind, double beta, double smoothing, double margin, double nll_weight,
+                                                              bool average, int64_t pad, double temperature, int64_t grad,
+                                                              const OptTensor& scale_at, double scale) {
+  NmtgRows r = rows_of(logits, labels, pad, temperature);
+  c10::cuda::CUDAGuard guard(logits.device());
+  TORCH_CHECK(cu.numel() % 2 == 1 && cu.numel() < (1 << 28), "cu must hold 2 * pairs + 1 offsets");
+  need(cu, logits, at::kInt, cu.numel(), "cu");
+  NmtgPairs p = {};
+  p.pairs = static_cast<int>(cu.numel() / 2);
+  p.cu = cu.data_ptr<int>();
+  p.ref = opt_f32(ref, logits, 2 * static_cast<int64_t>(p.pairs), "ref_logprobs");
+  p.kind = static_cast<int>(kind);
+  p.average = average;
+  p.beta = static_cast<float>(beta);
+  p.smoothing = static_cast<float>(smoothing);
+  p.margin = static_cast<float>(margin);
+  p.nll_weight = static_cast<float>(nll_weight);
+  const auto f32 = logits.options().dtype(at::kFloat).requires_grad(false);
+  Tensor seq = at::empty({2 * static_cast<int64_t>(p.pairs)}, f32), loss = at::empty({1}, f32), ranked = at::empty({1}, f32),
+         work = at::empty({nmtg_pairs_workspace(r.rows, p.pairs)}, f32.dtype(at::kByte));
+  Tensor g = grad_of(logits, r, grad, scale_at, scale);
+  p.seq_logprobs = seq.data_ptr<float>();
+  p.loss = loss.data_ptr<float>();
+  p.ranked = ranked.data_ptr<float>();
+  p.workspace = work.data_ptr();
+  ck(nmtg_preference_loss(&r, &p, cur_stream()));
+  return {loss, ranked, seq, g.defined() ? OptTensor(g) : OptTensor()};
+}
+
+// grad [rows, vocab] of one of the losses times the one element of `factor`
+void scale_rows(Tensor& grad, const Tensor& factor) {
+  TORCH_CHECK(grad.is_cuda() && grad.dim() == 2 && (grad.stride(1) == 1 || grad.size(1) == 1), "grad must be rows of adjacent elements on a GPU");
+  need(factor, grad, at::kFloat, 1, "factor");
+  c10::cuda::CUDAGuard guard(grad.device());
+  NmtgRows r = {};
+  r.grad = grad.data_ptr();
+  r.rows = static_cast<int>(grad.size(0));
+  r.vocab = static_cast<int>(grad.size(1));
+  r.dtype = dtype_code(grad, "grad");
+  r.ld = grad.size(0) > 1 ? grad.stride(0) : grad.size(1);
+  ck(nmtg_scale_rows(&r, factor.data_ptr<float>(), cur_stream()));
+}
+
+}  // namespace
+
+void bind_tuning_ops(pybind11::module& m) {
+  m.def("row_scores", &row_scores);
+  m.def("row_scores_grad", &row_scores_grad);
+  m.def("policy_loss", &policy_loss);
+  m.def("preference_loss", &preference_loss);
+  m.def("scale_rows", &scale_rows);
+}

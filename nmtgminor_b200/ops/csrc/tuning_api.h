@@ -1,0 +1,59 @@
+// C launch API of preference tuning: log-probabilities of target words, paired and clipped policy losses (preference.cu), the embedding
+// gradient by sorted tokens (embed_sorted.cu) and activations kept in 8 bits (kept8.cu).
+// Every launcher returns nullptr on success or a static error string; nothing allocates.
+#pragma once
+#include <cuda_runtime.h>
+#include <cstdint>
+
+extern "C" {
+
+// ---- rows of logits (preference.cu) ----------------------------------------------------------------------------------
+// dtype of logits and gradient: 0 = fp32, 1 = bf16, 2 = fp16.  Rows are `ld` elements apart, elements of a row adjacent; the gradient has
+// the same `ld` and the same address modulo 16 bytes (it may be the logits themselves).  Rows whose label is `pad` or no word count as padding:
+// log-probability, loss and gradient 0.
+struct NmtgRows {
+  const void* logits;
+  void* grad;               // null: no gradient
+  const int64_t* labels;    // [rows]
+  int rows, vocab, dtype;
+  long ld;
+  float inv_temperature;
+  long pad;
+  float grad_scale;         // factor of the gradient of the two losses, times *grad_scale_at where that is not null
+  const float* grad_scale_at;
+  float* logprobs;          // [rows] out
+  float2* stat;             // [rows] (largest logit, sum of exp((x - largest) / T)): out of the scores, in of their gradient
+  int* status;
+};
+// log-probability of every label, and `stat` where it is not null
+const char* nmtg_row_scores(const NmtgRows* r, cudaStream_t stream);
+// grad = weight[row] * d logprob / d logits, from `stat`
+const char* nmtg_row_scores_grad(const NmtgRows* r, const float* weight, cudaStream_t stream);
+
+struct NmtgPolicy {
+  const float* old_logprobs;   // [rows]
+  const float* advantages;     // [rows]
+  const float* ref_logprobs;   // [rows] or null
+  float clip_low, clip_high, kl_coef;
+  double* row_loss;            // [3, rows] scratch: loss, KL, 1 where the ratio was clipped
+  float *loss, *kl, *clipped;  // [1] each, out: sums of losses and KL terms, number of clipped words
+};
+const char* nmtg_policy_loss(const NmtgRows* r, const NmtgPolicy* p, cudaStream_t stream);
+
+// Sequences 2i (preferred) and 2i + 1 (rejected) of `cu` are pair i.
+struct NmtgPairs {
+  const int* cu;               // [2 pairs + 1]
+  const float* ref;            // [2 pairs] or null
+  int pairs;
+  int kind;                    // 0 sigmoid, 1 hinge, 2 squared distance to 1 / (2 beta)
+  int average;
+  float beta, smoothing, margin, nll_weight;
+  float* seq_logprobs;         // [2 pairs] out
+  float *loss, *ranked;        // [1] each, out: sum of losses, number of pairs ranked as preferred
+  void* workspace;             // nmtg_pairs_workspace bytes, 16-byte aligned
+};
+long nmtg_pairs_workspace(int rows, int pairs);
+const char* nmtg_preference_loss(const NmtgRows* r, const NmtgPairs* p, cudaStream_t stream);
+// r->grad *= *factor, unless it is 1
+const char* nmtg_scale_rows(const NmtgRows* r, const float* factor, cudaStream_t stream);
+}
