@@ -219,16 +219,18 @@ def _keep_scale(p: float) -> float:
 
 
 class _LinearFn(torch.autograd.Function):
-    """y = [residual +] dropout(act(x W^T + b)); weight/bias gradients go to the main_grad buffers."""
+    """y = [residual +] dropout(act(x W^T + b)); weight/bias gradients go to the main_grad buffers.  ``keep8``: x and the
+    pre-activation wait for the backward pass in 8 bits (csrc/kept8.cu)."""
 
     @staticmethod
-    def forward(ctx, x, w, bias, residual, gw, gb, act, dropout_p, seed, stream_id, need_input_grad, gather=None):
+    def forward(ctx, x, w, bias, residual, gw, gb, act, dropout_p, seed, stream_id, need_input_grad, gather=None, keep8=False):
         M, N = x.shape[0], w.shape[0]
         y = empty_rows(M, N, x.device)
         z = empty_rows(M, N, x.device) if act != 0 else None  # pre-activation, needed by act'
         gemm(x, w, y, bias=bias, residual=residual, preact=z, act=act, dropout_p=dropout_p, seed=seed,
              stream_id=stream_id, gather=gather)
-        ctx.save_for_backward(x, w, z)
+        ctx.keep8 = (_keep8(x) if gw is not None else None, _keep8(z) if act != 0 else None, x.shape[1]) if keep8 else None
+        ctx.save_for_backward(None if keep8 else x, w, None if keep8 else z)
         ctx.cfg = (act, dropout_p, seed, stream_id, residual is not None, bias is not None, need_input_grad)
         ctx.gw, ctx.gb = gw, gb
         ctx.gather = gather
@@ -246,8 +248,16 @@ class _LinearFn(torch.autograd.Function):
             dy = dy.contiguous()
         want_gb = has_bias and ctx.gb is not None
         fused_gb = want_gb and act == 0 and p > 0.0 and _colsum_fusable(dy)
+        kept_x, kept_z, K = ctx.keep8 if ctx.keep8 is not None else (None, None, x.shape[1])
         if fused_gb:
             dz = ext().dropout_colsum(dy, p, seed, sid, ctx.gb)  # regenerated mask and bias gradient in one pass
+        elif kept_z is not None:
+            LAUNCHES[0] += 1
+            dz = ext().kept_backward(dy, kept_z.codes, kept_z.scales, act, p, seed, sid)
+            if dz.shape[1] % 8:
+                padded = empty_rows(dz.shape[0], dz.shape[1], dz.device)
+                padded.copy_(dz)
+                dz = padded
         elif act != 0 and dy.numel() % 8 == 0:
             dz = ext().act_backward(dy, z, act, p, seed, sid)    # regenerated mask times act'(z) in one pass
         else:
@@ -255,14 +265,25 @@ class _LinearFn(torch.autograd.Function):
             if act != 0:
                 dz = _act_backward(dz, z, act)
         if ctx.gw is not None:
-            gemm(dz, x, ctx.gw, a_mn_major=True, b_mn_major=True, accumulate=True, allow_split_k=True)
+            gemm(dz, x if kept_x is None else _restore8(kept_x), ctx.gw, a_mn_major=True, b_mn_major=True, accumulate=True,
+                 allow_split_k=True)
         if want_gb and not fused_gb:
             ext().colsum(dz, ctx.gb)
         dx = None
         if need_dx:
-            dx = torch.empty((dy.shape[0], x.shape[1]), dtype=torch.bfloat16, device=dy.device)
+            dx = torch.empty((dy.shape[0], K), dtype=torch.bfloat16, device=dy.device)
             gemm(dz, w, dx, b_mn_major=True, gather=ctx.gather)
-        return dx, None, None, (dy if has_res else None), None, None, None, None, None, None, None, None
+        return dx, None, None, (dy if has_res else None), None, None, None, None, None, None, None, None, None
+
+
+def _keep8(x):
+    from .kept import quantise
+    return quantise(x)
+
+
+def _restore8(kept):
+    from .kept import restore
+    return restore(kept)
 
 
 def _colsum_fusable(dy):
@@ -285,10 +306,14 @@ def _act_backward(dh, z, act):
     return (dh.float() * g).to(torch.bfloat16)
 
 
-def linear(x, weight, bias=None, act="none", dropout_p=0.0, residual=None, training=True):
-    """Fused Linear: ``[residual +] dropout(act(x @ weight.T + bias))`` on 2-D ``x``."""
+def linear(x, weight, bias=None, act="none", dropout_p=0.0, residual=None, training=True, keep8=False):
+    """Fused Linear: ``[residual +] dropout(act(x @ weight.T + bias))`` on 2-D ``x``.  ``keep8``: ``x`` (for the weight's gradient) and the
+    pre-activation (for the slope of ``act``) wait for the backward pass in 8 bits (``ops.kept``), half of what they take otherwise; the forward pass
+    and, without ``act``, the gradient with respect to ``x`` are the same."""
     act_id = ACT_IDS[act] if not isinstance(act, int) else act
     p = float(dropout_p) if training else 0.0
+    if keep8 and act_id != 0 and p > 0.0 and weight.shape[0] % 4:
+        raise ValueError("linear: keep8 with an activation and dropout takes a multiple of 4 outputs (the mask is drawn for 4 elements at a time)")
     if fused_param(weight) and x.is_cuda:
         b = bias.work if bias is not None else None
         gw = getattr(weight, "main_grad", None) if weight.requires_grad else None
@@ -305,7 +330,9 @@ def linear(x, weight, bias=None, act="none", dropout_p=0.0, residual=None, train
             return gemm(xin, weight.work, y, bias=b, residual=residual, act=act_id, dropout_p=p, seed=_Rng.seed,
                         stream_id=sid, allow_split_k=step_sums.depth > 0, gather=_gather_of(weight))
         return _LinearFn.apply(_track(xin), weight.work, b, residual, gw, gb, act_id, p, _Rng.seed, sid, need_dx,
-                               _gather_of(weight))
+                               _gather_of(weight), bool(keep8))
+    if keep8 and torch.is_grad_enabled():
+        return ref.linear_kept(x, weight, bias, act_id, p, residual)
     return ref.linear(x, weight, bias, act_id, p, residual)
 
 
@@ -334,10 +361,13 @@ class _MlpFn(torch.autograd.Function):
     Every element-wise step rides in a GEMM epilogue: bias + activation + dropout (fc1), bias + dropout +
     residual (fc2), and in backward the activation gradient (and, for GELU/SiLU, the regenerated fc1
     dropout mask) is the epilogue of the fc2 data-gradient product.
+
+    ``keep8``: x and one matrix of the hidden layer wait for the backward pass in 8 bits, instead of x and h (and z).  With
+    ReLU that is h, whose sign bits are kept as they are; with GELU and SiLU it is z, from which h is computed again.
     """
 
     @staticmethod
-    def forward(ctx, x, w1, b1, w2, b2, residual, g, act, p1, p2, seed, sid1, sid2, gather1=None, gather2=None):
+    def forward(ctx, x, w1, b1, w2, b2, residual, g, act, p1, p2, seed, sid1, sid2, gather1=None, gather2=None, keep8=False):
         M = x.shape[0]
         h = torch.empty((M, w1.shape[0]), dtype=torch.bfloat16, device=x.device)
         z = torch.empty_like(h) if act != 1 else None
@@ -347,7 +377,12 @@ class _MlpFn(torch.autograd.Function):
         gemm(x, w1, h, bias=b1, preact=z, act=act, dropout_p=p1, seed=seed, stream_id=sid1, mask=bits, gather=gather1)
         y = torch.empty((M, w2.shape[0]), dtype=torch.bfloat16, device=x.device)
         gemm(h, w2, y, bias=b2, residual=residual, dropout_p=p2, seed=seed, stream_id=sid2, gather=gather2)
-        ctx.save_for_backward(x, w1, w2, h, z if z is not None else bits)
+        if keep8:
+            ctx.save_for_backward(None, w1, w2, None, bits)
+            ctx.keep8 = (_keep8(x) if g[0] is not None else None, _keep8(h if act == 1 else z))
+        else:
+            ctx.save_for_backward(x, w1, w2, h, z if z is not None else bits)
+            ctx.keep8 = None
         ctx.cfg = (act, p1, p2, seed, sid1, sid2, residual is not None)
         ctx.g = g
         ctx.gathers = (gather1, gather2)
@@ -359,6 +394,13 @@ class _MlpFn(torch.autograd.Function):
         act, p1, p2, seed, sid1, sid2, has_res = ctx.cfg
         gw1, gb1, gw2, gb2 = ctx.g
         dy = dy.contiguous()
+        if ctx.keep8 is not None:
+            from .kept import restore_activated
+            x = _restore8(ctx.keep8[0]) if gw1 is not None else None
+            if act == 1:
+                h = _restore8(ctx.keep8[1])
+            else:
+                z, h = restore_activated(ctx.keep8[1], act, p1, seed, sid1, True)
         fused_gb2 = gb2 is not None and p2 > 0.0 and _colsum_fusable(dy)
         if fused_gb2:
             dz2 = ext().dropout_colsum(dy, p2, seed, sid2, gb2)
@@ -382,13 +424,14 @@ class _MlpFn(torch.autograd.Function):
             gemm(dz1, x, gw1, a_mn_major=True, b_mn_major=True, accumulate=True, allow_split_k=True)
         if gb1 is not None and not fused_gb1:
             ext().colsum(dz1, gb1)
-        dx = torch.empty_like(x)
+        dx = torch.empty((dz1.shape[0], w1.shape[1]), dtype=torch.bfloat16, device=dz1.device)
         gemm(dz1, w1, dx, b_mn_major=True, gather=ctx.gathers[0])
-        return (dx, None, None, None, None, (dy if has_res else None)) + (None,) * 9
+        return (dx, None, None, None, None, (dy if has_res else None)) + (None,) * 10
 
 
-def mlp(x, w1, b1, w2, b2, act="relu", dropout_p=0.0, out_dropout_p=0.0, residual=None, training=True):
-    """Position-wise feed-forward block: ``[residual +] D(D(act(x W1^T + b1)) W2^T + b2)``."""
+def mlp(x, w1, b1, w2, b2, act="relu", dropout_p=0.0, out_dropout_p=0.0, residual=None, training=True, keep8=False):
+    """Position-wise feed-forward block: ``[residual +] D(D(act(x W1^T + b1)) W2^T + b2)``.  ``keep8``: what the backward pass needs of ``x`` and of the
+    hidden layer waits in 8 bits (``ops.kept``); the forward pass is the same."""
     act_id = ACT_IDS[act] if not isinstance(act, int) else act
     p1 = float(dropout_p) if training else 0.0
     p2 = float(out_dropout_p) if training else 0.0
@@ -401,13 +444,15 @@ def mlp(x, w1, b1, w2, b2, act="relu", dropout_p=0.0, out_dropout_p=0.0, residua
                       for t in (w1, b1, w2, b2))
             return _MlpFn.apply(_track(xin), w1.work, b1.work if b1 is not None else None, w2.work,
                                 b2.work if b2 is not None else None, residual, g, act_id, p1, p2, _Rng.seed, sid1, sid2,
-                                _gather_of(w1), _gather_of(w2))
+                                _gather_of(w1), _gather_of(w2), bool(keep8))
         if step_sums.depth > 0:
             return linear(linear(xin, w1, b1, act_id, 0.0, None, False), w2, b2, 0, 0.0, residual, False)
         h = torch.empty((x.shape[0], w1.shape[0]), dtype=torch.bfloat16, device=x.device)
         gemm(xin, w1.work, h, bias=b1.work if b1 is not None else None, act=act_id, gather=_gather_of(w1))
         y = torch.empty((x.shape[0], w2.shape[0]), dtype=torch.bfloat16, device=x.device)
         return gemm(h, w2.work, y, bias=b2.work if b2 is not None else None, residual=residual, gather=_gather_of(w2))
+    if keep8 and torch.is_grad_enabled():
+        return ref.mlp_kept(x, w1, b1, w2, b2, act_id, p1, p2, residual)
     h = ref.linear(x, w1, b1, act_id, p1, None)
     return ref.linear(h, w2, b2, 0, p2, residual)
 
@@ -653,20 +698,47 @@ def attention(q, k, v, cu_q, cu_k, heads, max_q, max_k, causal=False, dropout_p=
 # ---------------------------------------------------------------------------------------------------
 class _EmbedFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, dummy, tokens, positions, table, pos_table, gtable, gpos, scale, p, seed, sid, pad_idx):
+    def forward(ctx, dummy, tokens, positions, table, pos_table, gtable, gpos, scale, p, seed, sid, pad_idx, sorted_grad=False):
         out = ext().embed_fwd(tokens, positions, table, pos_table, scale, p, seed, sid)
         ctx.save_for_backward(tokens, positions)
-        ctx.cfg = (scale, p, seed, sid, pad_idx)
+        ctx.cfg = (scale, p, seed, sid, pad_idx, table.shape[0], sorted_grad)
         ctx.gtable, ctx.gpos = gtable, gpos
         return out
 
     @staticmethod
     def backward(ctx, dy):
         tokens, positions = ctx.saved_tensors
-        scale, p, seed, sid, pad_idx = ctx.cfg
-        if ctx.gtable is not None:
+        scale, p, seed, sid, pad_idx, vocab, sorted_grad = ctx.cfg
+        if sorted_grad:
+            dy = dy.contiguous()
+            if ctx.gtable is not None:
+                LAUNCHES[0] += 3
+                ext().embed_grad(tokens, None, dy, ctx.gtable, vocab, vocab, scale, p, seed, sid, pad_idx)
+            if ctx.gpos is not None:
+                LAUNCHES[0] += 3
+                pos = torch.zeros_like(tokens) if positions is None else positions
+                ext().embed_grad(tokens, pos, dy, ctx.gpos, vocab, ctx.gpos.shape[0], 1.0, p, seed, sid, pad_idx)
+        elif ctx.gtable is not None:
             ext().embed_bwd(tokens, positions, dy.contiguous(), ctx.gtable, ctx.gpos, scale, p, seed, sid, pad_idx)
-        return (None,) * 12
+        return (None,) * 13
+
+
+class _EmbedSortedFn(torch.autograd.Function):
+    """``table[tokens] * scale`` of an ordinary CUDA tensor; its gradient is written whole, in the table's type."""
+
+    @staticmethod
+    def forward(ctx, table, tokens, scale, pad_idx):
+        ctx.save_for_backward(tokens)
+        ctx.cfg = (scale, pad_idx, table.shape)
+        LAUNCHES[0] += 1
+        return ext().embed_rows(tokens, table, scale)
+
+    @staticmethod
+    def backward(ctx, dy):
+        (tokens,) = ctx.saved_tensors
+        scale, pad_idx, shape = ctx.cfg
+        LAUNCHES[0] += 3
+        return ext().embed_grad(tokens, None, dy.contiguous(), None, shape[0], shape[0], scale, 0.0, 0, 0, pad_idx), None, None, None
 
 
 _dummy = {}
@@ -681,9 +753,15 @@ def _grad_anchor(device):
 
 
 def embedding(tokens, table, positions=None, pos_table=None, scale=1.0, dropout_p=0.0, training=True, pad_idx=0,
-              pos_trainable=False):
-    """out = dropout(table[tokens] * scale + pos_table[positions]) for 1-D packed ``tokens``."""
+              pos_trainable=False, sorted_grad=None):
+    """out = dropout(table[tokens] * scale + pos_table[positions]) for 1-D packed ``tokens``.
+
+    ``sorted_grad``: every row of the table's gradient (and of a trainable position table's) is summed in the order of the tokens, without atomic
+    additions, so that it repeats to the last bit (csrc/embed_sorted.cu); None: where ``torch.use_deterministic_algorithms`` asks for it.  It
+    then serves ordinary CUDA tables (bf16, fp16, fp32, any width) as well as those of the flat store.  Rows of padding give no gradient."""
     p = float(dropout_p) if training else 0.0
+    if sorted_grad is None:
+        sorted_grad = torch.are_deterministic_algorithms_enabled()
     if fused_param(table) and tokens.is_cuda and table.shape[1] % 16 == 0:
         sid = next_stream() if p > 0 else 0
         pt = None
@@ -697,9 +775,30 @@ def embedding(tokens, table, positions=None, pos_table=None, scale=1.0, dropout_
         gtable = table.main_grad if table.requires_grad else None
         if torch.is_grad_enabled() and (gtable is not None or gpos is not None):
             return _EmbedFn.apply(_grad_anchor(tokens.device), tokens, positions, table.work, pt, gtable, gpos, scale, p,
-                                  _Rng.seed, sid, pad_idx)
+                                  _Rng.seed, sid, pad_idx, bool(sorted_grad))
         return ext().embed_fwd(tokens, positions, table.work, pt, scale, p, _Rng.seed, sid)
+    if sorted_grad:
+        return _embedding_sorted(tokens, table, positions, pos_table, float(scale), p, int(pad_idx))
     return ref.embedding(tokens, table, positions, pos_table, scale, p, pad_idx)
+
+
+def _embedding_sorted(tokens, table, positions, pos_table, scale, p, pad_idx):
+    """Sorted gradients of tables outside the flat store; on the CPU they are sums in order as they are."""
+    if tokens.dim() != 1 or tokens.dtype != torch.int64 or table.dim() != 2 or table.shape[0] < 1:
+        raise ValueError("embedding: int64 tokens [rows] and a table [words, width], got %s and %s" % (tuple(tokens.shape), tuple(table.shape)))
+    if tokens.device != table.device:
+        raise ValueError("embedding: tokens are on %s, the table on %s" % (tokens.device, table.device))
+    on_gpu = table.is_cuda and table.dtype in (torch.bfloat16, torch.float16, torch.float32)
+    if on_gpu:
+        out = _EmbedSortedFn.apply(table.contiguous(), tokens.contiguous(), scale, pad_idx)
+    else:
+        out = F.embedding(tokens, table, padding_idx=pad_idx if 0 <= pad_idx < table.shape[0] else None) * scale
+    if pos_table is not None:
+        pos = (positions if positions is not None else torch.zeros_like(tokens)).clamp(0, pos_table.shape[0] - 1)
+        on_gpu = pos_table.is_cuda and pos_table.dtype in (torch.bfloat16, torch.float16, torch.float32)
+        rows = _EmbedSortedFn.apply(pos_table.contiguous(), pos.contiguous(), 1.0, -1) if on_gpu else F.embedding(pos, pos_table)
+        out = out + rows.to(out.dtype)
+    return F.dropout(out, p, True) if p > 0 else out
 
 
 # ---------------------------------------------------------------------------------------------------

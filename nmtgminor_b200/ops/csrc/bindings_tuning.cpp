@@ -5,7 +5,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include "tuning_api.h"
 
-int* nmtg_status_word(int device);   // bindings.cpp
+int* nmtg_status_word(int device);                          // bindings.cpp
+const unsigned long long* nmtg_seed_word(int device);
 
 namespace {
 
@@ -36,7 +37,7 @@ const float* opt_f32(const OptTensor& t, const Tensor& like, int64_t n, const ch
 
 // logits [rows, vocab] with adjacent elements in rows that do not overlap, labels [rows]
 NmtgRows rows_of(const Tensor& logits, const Tensor& labels, int64_t pad, double temperature) {
-  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.size(1) >= 1 && (logits.stride(1) == 1 || logits.size(1) == 1),
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.size(1) >= 1 && (logits.stride(1) == 1 || logits.size(1) == 1 || logits.numel() == 0),
               "logits must be rows of adjacent elements on a GPU");
   TORCH_CHECK(logits.size(0) <= 1 || logits.stride(0) >= logits.size(1), "the rows of the logits overlap");
   TORCH_CHECK(logits.size(0) < (1 << 30) && logits.size(1) < (1LL << 31) - 64, "logits: too many rows or words");
@@ -171,6 +172,164 @@ void scale_rows(Tensor& grad, const Tensor& factor) {
   ck(nmtg_scale_rows(&r, factor.data_ptr<float>(), cur_stream()));
 }
 
+// ---- embedding -----------------------------------------------------------------------------------------------------------
+void need_dense(const Tensor& t, const Tensor& like, int64_t rows, int64_t width, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.is_contiguous() && t.dim() == 2 && t.size(0) == rows && t.size(1) == width,
+              name, ": wrong device, layout or size");
+}
+
+Tensor embed_rows(const Tensor& tokens, const Tensor& table, double scale) {
+  TORCH_CHECK(table.is_cuda() && table.dim() == 2 && table.is_contiguous(), "table must be a dense matrix on a GPU");
+  need(tokens, table, at::kLong, tokens.numel(), "tokens");
+  TORCH_CHECK(tokens.numel() < (1 << 30) && table.size(0) < (1LL << 31) && table.size(1) < (1 << 30), "embedding: too large");
+  c10::cuda::CUDAGuard guard(table.device());
+  Tensor out = at::empty({tokens.numel(), table.size(1)}, table.options().requires_grad(false));
+  ck(nmtg_embed_rows(tokens.data_ptr<int64_t>(), table.data_ptr(), out.data_ptr(), static_cast<int>(tokens.numel()),
+                     static_cast<int>(table.size(0)), static_cast<int>(table.size(1)), dtype_code(table, "table"), static_cast<float>(scale),
+                     cur_stream()));
+  return out;
+}
+
+// Into `grad` (fp32 [keys, width], added to), or a new [keys, width] matrix of dy's type
+Tensor embed_grad(const Tensor& tokens, const OptTensor& positions, const Tensor& dy, const OptTensor& grad, int64_t vocab, int64_t keys,
+                  double scale, double p, int64_t seed, int64_t stream_id, int64_t pad) {
+  TORCH_CHECK(dy.is_cuda() && dy.dim() == 2, "dy must be a matrix on a GPU");
+  const int64_t rows = tokens.numel(), width = dy.size(1);
+  need(tokens, dy, at::kLong, rows, "tokens");
+  need_dense(dy, dy, rows, width, "dy");
+  if (positions.has_value()) need(*positions, dy, at::kLong, rows, "positions");
+  TORCH_CHECK(rows < (1 << 30) && vocab >= 0 && vocab < (1LL << 31) && keys >= 0 && keys < (1 << 30) && width < (1 << 30), "embedding: too large");
+  TORCH_CHECK(p >= 0.0 && p < 1.0, "embedding: dropout must be in [0, 1)");
+  c10::cuda::CUDAGuard guard(dy.device());
+  NmtgEmbedGrad e = {};
+  Tensor out;
+  if (grad.has_value()) {
+    out = *grad;
+    need_dense(out, dy, keys, width, "grad");
+    TORCH_CHECK(out.scalar_type() == at::kFloat, "grad must be float32");
+  } else {
+    out = at::empty({keys, width}, dy.options().requires_grad(false));
+  }
+  e.tokens = tokens.data_ptr<int64_t>();
+  e.positions = positions.has_value() ? positions->data_ptr<int64_t>() : nullptr;
+  e.dy = dy.data_ptr();
+  e.grad = out.data_ptr();
+  e.rows = static_cast<int>(rows);
+  e.vocab = static_cast<int>(vocab);
+  e.keys = static_cast<int>(keys);
+  e.width = static_cast<int>(width);
+  e.dtype = dtype_code(dy, "dy");
+  e.accumulate = grad.has_value();
+  e.pad = pad;
+  e.scale = static_cast<float>(scale);
+  e.p = static_cast<float>(p);
+  e.seed = static_cast<unsigned long long>(seed);
+  e.stream_id = static_cast<unsigned long long>(stream_id);
+  e.seed_dev = nmtg_seed_word(dy.get_device());
+  Tensor work = at::empty({nmtg_embed_grad_workspace(e.rows, e.keys, e.width)}, dy.options().dtype(at::kByte).requires_grad(false));
+  e.workspace = work.data_ptr();
+  e.stream = cur_stream();
+  ck(nmtg_embed_grad(&e));
+  return out;
+}
+
+// ---- activations kept in 8 bits ------------------------------------------------------------------------------------------
+NmtgKept kept_of(const Tensor& like, int64_t rows, int64_t width, int64_t act, double p, int64_t seed, int64_t stream_id) {
+  TORCH_CHECK(p >= 0.0 && p < 1.0, "kept: dropout must be in [0, 1)");
+  NmtgKept k = {};
+  k.rows = rows;
+  k.width = k.ld_in = width;
+  k.act = static_cast<int>(act);
+  k.p = static_cast<float>(p);
+  k.seed = static_cast<unsigned long long>(seed);
+  k.stream_id = static_cast<unsigned long long>(stream_id);
+  k.seed_dev = nmtg_seed_word(like.get_device());
+  k.stream = cur_stream();
+  return k;
+}
+void codes_of(NmtgKept& k, const Tensor& codes, const Tensor& scales) {
+  const int64_t blocks = (k.width + 31) / 32;
+  TORCH_CHECK(codes.is_cuda() && codes.is_contiguous() && codes.scalar_type() == at::kByte && codes.numel() == k.rows * blocks * 32 &&
+              address(codes) % 8 == 0, "codes: wrong device, layout, dtype or size");
+  need(scales, codes, at::kByte, k.rows * blocks, "scales");
+  k.codes = codes.data_ptr<uint8_t>();
+  k.scales = scales.data_ptr<uint8_t>();
+}
+void matrix(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 2 && (t.numel() == 0 || ((t.stride(1) == 1 || t.size(1) == 1) && (t.size(0) == 1 || t.stride(0) >= t.size(1)))), name,
+              " must be rows of adjacent elements on a GPU");
+}
+std::tuple<Tensor, Tensor> new_codes(const Tensor& x) {
+  const int64_t blocks = (x.size(1) + 31) / 32;
+  const auto o = x.options().dtype(at::kByte).requires_grad(false);
+  return {at::empty({x.size(0), blocks * 32}, o), at::empty({x.size(0), blocks}, o)};
+}
+
+// x [rows, width] -> codes [rows, 32 * blocks], scales [rows, blocks]
+std::tuple<Tensor, Tensor> kept_quantise(const Tensor& x) {
+  matrix(x, "x");
+  c10::cuda::CUDAGuard guard(x.device());
+  NmtgKept k = kept_of(x, x.size(0), x.size(1), 0, 0.0, 0, 0);
+  auto [codes, scales] = new_codes(x);
+  codes_of(k, codes, scales);
+  k.in = x.data_ptr();
+  k.ld_in = x.size(0) > 1 ? x.stride(0) : x.size(1);
+  k.dtype = dtype_code(x, "x");
+  ck(nmtg_kept_quantise(&k));
+  return {codes, scales};
+}
+
+// -> x' (where `plain`), dropout(act(x')) (where act is not negative)
+std::tuple<OptTensor, OptTensor> kept_restore(const Tensor& codes, const Tensor& scales, int64_t width, at::ScalarType dtype, bool plain, int64_t act,
+                                              double p, int64_t seed, int64_t stream_id) {
+  TORCH_CHECK(codes.is_cuda() && codes.dim() == 2, "codes must be a matrix on a GPU");
+  c10::cuda::CUDAGuard guard(codes.device());
+  NmtgKept k = kept_of(codes, codes.size(0), width, act < 0 ? 0 : act, act < 0 ? 0.0 : p, seed, stream_id);
+  codes_of(k, codes, scales);
+  const auto o = codes.options().dtype(dtype);
+  OptTensor x, h;
+  if (plain) { x = at::empty({k.rows, width}, o); k.out = x->data_ptr(); k.dtype = dtype_code(*x, "x"); }
+  if (act >= 0) { h = at::empty({k.rows, width}, o); k.out2 = h->data_ptr(); k.dtype = dtype_code(*h, "h"); }
+  if (plain || act >= 0) ck(nmtg_kept_restore(&k));
+  return {x, h};
+}
+
+// -> dropout(act(z)), codes and scales where `keep`
+std::tuple<Tensor, OptTensor, OptTensor> kept_forward(const Tensor& z, int64_t act, bool keep, double p, int64_t seed, int64_t stream_id) {
+  matrix(z, "z");
+  c10::cuda::CUDAGuard guard(z.device());
+  NmtgKept k = kept_of(z, z.size(0), z.size(1), act, p, seed, stream_id);
+  Tensor y = at::empty({z.size(0), z.size(1)}, z.options().requires_grad(false));
+  OptTensor codes, scales;
+  if (keep) {
+    auto [c, s] = new_codes(z);
+    codes_of(k, c, s);
+    codes = c;
+    scales = s;
+  }
+  k.in = z.data_ptr();
+  k.ld_in = z.size(0) > 1 ? z.stride(0) : z.size(1);
+  k.out = y.data_ptr();
+  k.dtype = dtype_code(z, "z");
+  ck(nmtg_kept_forward(&k));
+  return {y, codes, scales};
+}
+
+Tensor kept_backward(const Tensor& dy, const Tensor& codes, const Tensor& scales, int64_t act, double p, int64_t seed, int64_t stream_id) {
+  matrix(dy, "dy");
+  TORCH_CHECK(codes.device() == dy.device(), "codes and dy are on different devices");
+  c10::cuda::CUDAGuard guard(dy.device());
+  NmtgKept k = kept_of(dy, dy.size(0), dy.size(1), act, p, seed, stream_id);
+  codes_of(k, codes, scales);
+  Tensor dz = at::empty({dy.size(0), dy.size(1)}, dy.options().requires_grad(false));
+  k.in = dy.data_ptr();
+  k.ld_in = dy.size(0) > 1 ? dy.stride(0) : dy.size(1);
+  k.out = dz.data_ptr();
+  k.dtype = dtype_code(dy, "dy");
+  ck(nmtg_kept_backward(&k));
+  return dz;
+}
+
 }  // namespace
 
 void bind_tuning_ops(pybind11::module& m) {
@@ -179,4 +338,13 @@ void bind_tuning_ops(pybind11::module& m) {
   m.def("policy_loss", &policy_loss);
   m.def("preference_loss", &preference_loss);
   m.def("scale_rows", &scale_rows);
+  m.def("embed_rows", &embed_rows);
+  m.def("embed_grad", &embed_grad);
+  m.def("kept_quantise", &kept_quantise);
+  m.def("kept_restore", [](const Tensor& codes, const Tensor& scales, int64_t width, pybind11::object dtype, bool plain, int64_t act, double p,
+                           int64_t seed, int64_t stream_id) {
+    return kept_restore(codes, scales, width, torch::python::detail::py_object_to_dtype(dtype), plain, act, p, seed, stream_id);
+  });
+  m.def("kept_forward", &kept_forward);
+  m.def("kept_backward", &kept_backward);
 }

@@ -498,12 +498,13 @@ extern "C" long nmtg_bounds_xentropy();
 extern "C" long nmtg_bounds_decode();
 extern "C" long nmtg_bounds_sequence();
 extern "C" long nmtg_bounds_attention_short();
+extern "C" long nmtg_bounds_embed_sorted();
 
 // Number of out-of-range indices corrected by the kernels of this library since load; -1 when the checks are compiled out.
 extern "C" long nmtg_bounds_violations() {
   long total = 0;
   const long parts[] = {nmtg_bounds_elementwise(), nmtg_bounds_xentropy(), nmtg_bounds_decode(), nmtg_bounds_sequence(),
-                        nmtg_bounds_attention_short()};
+                        nmtg_bounds_attention_short(), nmtg_bounds_embed_sorted()};
   for (long v : parts) {
     if (v < 0) return v;
     total += v;

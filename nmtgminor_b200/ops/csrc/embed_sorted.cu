@@ -1,0 +1,507 @@
+// Gradient of an embedding lookup, each row's sum taken in the order of the tokens: no atomic additions, the same bits every time.
+//   1. order:  the rows sorted by key (stable).  Up to kRankRows rows one kernel counts, for every row, the rows before it in the order
+//      (keys and row numbers packed into 32 bits, N^2 comparisons in registers); more rows take stable radix passes of up to 10 bits
+//      (count, scan, scatter).
+//   2. reduce: the sorted rows in chunks of 8 to 32, a group of threads each, whatever the words' frequencies are; a sum that begins and
+//      ends in a chunk goes to its row of the gradient, one that crosses an end leaves its part in the workspace.
+//   3. join:   the parts of a sum, in order.
+// Where the gradient is written whole, its rows are cleared by further blocks of the sorting kernels: these wait on latency, the clearing on memory.
+// Bound by the bytes of dy and of the gradient's rows.  Sums in 32 bits, one rounding at the end.
+#include <cuda_runtime.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+#include "b200_ptx.cuh"
+#include "bounds_check.cuh"
+#include "tuning_api.h"
+
+namespace b200 {
+
+int num_sms();
+
+namespace {
+
+constexpr int kRankBits = 13, kRankRows = 1 << kRankBits;      // rows that the counting kernel takes
+constexpr int kRankTile = 64;                                  // rows of one of its blocks
+constexpr int kTile = 2048;                                    // rows of a block of a radix pass
+constexpr int kDigitBits = 10;                                 // at most
+
+struct Keys {
+  const int64_t* tokens;
+  const int64_t* positions;
+  int rows, vocab, keys;
+  long pad;
+  __device__ __forceinline__ int of(int r) const {            // `keys`: the row has none
+    const int64_t t = tokens[r];
+    if (t == pad || t < 0 || t >= vocab) return keys;
+    if (!positions) return static_cast<int>(t);
+    const int64_t p = positions[r];
+    return p < 0 ? 0 : p >= keys ? keys - 1 : static_cast<int>(p);
+  }
+};
+
+// part `at` of `of` of the memory to clear, by the blocks from `first` on
+struct Clear {
+  uint4* p;
+  long n;
+  int first, at, of;
+  __device__ __forceinline__ bool mine() const { return static_cast<int>(blockIdx.x) >= first; }
+  __device__ __forceinline__ void run() const {
+    const long begin = n * at / of, end = n * (at + 1) / of;
+    const long step = static_cast<long>(gridDim.x - first) * blockDim.x;
+    for (long i = begin + (blockIdx.x - first) * static_cast<long>(blockDim.x) + threadIdx.x; i < end; i += step) p[i] = make_uint4(0, 0, 0, 0);
+  }
+};
+
+// order[rank] = row, sorted[rank] = key.  A thread counts for 4 rows over every 16th group of 4 rows.
+__global__ void __launch_bounds__(256) rank_kernel(const Keys k, int* __restrict__ order, int* __restrict__ sorted, const Clear clear) {
+  if (clear.mine()) { clear.run(); return; }
+  extern __shared__ __align__(16) uint32_t all[];
+  const int padded = (k.rows + 63) & ~63;
+  for (int i = threadIdx.x; i < padded; i += 256) all[i] = i < k.rows ? static_cast<uint32_t>(k.of(i)) << kRankBits | i : 0xFFFFFFFFu;
+  __syncthreads();
+  const int lane16 = threadIdx.x & 15, first = blockIdx.x * kRankTile + (threadIdx.x >> 4) * 4;
+  uint32_t mine[4];
+  int count[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) mine[j] = first + j < padded ? all[first + j] : 0xFFFFFFFFu;
+  for (int i = lane16; i < padded / 4; i += 16) {
+    const uint4 u = reinterpret_cast<const uint4*>(all)[i];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) count[j] += (u.x < mine[j]) + (u.y < mine[j]) + (u.z < mine[j]) + (u.w < mine[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) count[j] += __shfl_xor_sync(0xffffffffu, count[j], o);
+    if (lane16 == 0 && first + j < k.rows) {
+      order[count[j]] = first + j;
+      sorted[count[j]] = static_cast<int>(mine[j] >> kRankBits);
+    }
+  }
+}
+
+// ---- radix passes ----------------------------------------------------------------------------------------------------------
+struct Pass {
+  const int* key;           // null: the first pass, keys from the tokens
+  const int* row;
+  int* key_out;
+  int* row_out;
+  int* counts;              // [bins][tiles]
+  int shift, bins, tiles;
+};
+
+__device__ __forceinline__ int key_at(const Keys& k, const Pass& p, int i) { return p.key ? p.key[i] : k.of(i); }
+
+__global__ void __launch_bounds__(256) radix_count_kernel(const Keys k, const Pass p, const Clear clear) {
+  if (clear.mine()) { clear.run(); return; }
+  __shared__ int bins[1 << kDigitBits];
+  for (int b = threadIdx.x; b < p.bins; b += 256) bins[b] = 0;
+  __syncthreads();
+  for (int i = blockIdx.x * kTile + threadIdx.x; i < min(k.rows, (static_cast<int>(blockIdx.x) + 1) * kTile); i += 256)
+    atomicAdd(&bins[(key_at(k, p, i) >> p.shift) & (p.bins - 1)], 1);
+  __syncthreads();
+  for (int b = threadIdx.x; b < p.bins; b += 256) p.counts[static_cast<long>(b) * p.tiles + blockIdx.x] = bins[b];
+}
+
+// counts -> their exclusive sums, one block
+__global__ void __launch_bounds__(1024) radix_scan_kernel(int* __restrict__ counts, int n, const Clear clear) {
+  if (clear.mine()) { clear.run(); return; }
+  __shared__ int warps[32];
+  __shared__ int carry;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  if (t == 0) carry = 0;
+  __syncthreads();
+  constexpr int kEach = 8;
+  for (int base = 0; base < n; base += 1024 * kEach) {
+    int v[kEach], sum = 0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int i = base + t * kEach + j;
+      v[j] = i < n ? counts[i] : 0;
+      sum += v[j];
+    }
+    int before = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += u; }
+    if (lane == 31) warps[warp] = before;
+    __syncthreads();
+    if (warp == 0) {
+      int w = warps[lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, w, o); if (lane >= o) w += u; }
+      warps[lane] = w;
+    }
+    __syncthreads();
+    int at = carry + before - sum + (warp ? warps[warp - 1] : 0);
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int i = base + t * kEach + j;
+      if (i < n) counts[i] = at;
+      at += v[j];
+    }
+    __syncthreads();
+    if (t == 1023) carry = at;
+    __syncthreads();
+  }
+}
+
+// A warp has kTile / 8 rows one after another: it counts its digits, the warps' counts are summed in order, then rows go to their places.
+__global__ void __launch_bounds__(256) radix_scatter_kernel(const Keys k, const Pass p, const Clear clear) {
+  if (clear.mine()) { clear.run(); return; }
+  extern __shared__ int at[];                                   // [8][bins]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int b = threadIdx.x; b < 8 * p.bins; b += 256) at[b] = 0;
+  __syncthreads();
+  const int begin = blockIdx.x * kTile + warp * (kTile / 8), end = min(k.rows, begin + kTile / 8);
+  int* const mine = at + warp * p.bins;
+  const uint32_t below = (1u << lane) - 1;
+  for (int i0 = begin; i0 < end; i0 += 32) {
+    const int i = i0 + lane, d = i < end ? (key_at(k, p, i) >> p.shift) & (p.bins - 1) : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, d);
+    if (d >= 0 && (same & below) == 0) mine[d] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < p.bins; b += 256) {
+    int sum = p.counts[static_cast<long>(b) * p.tiles + blockIdx.x];
+#pragma unroll
+    for (int w = 0; w < 8; ++w) { const int n = at[w * p.bins + b]; at[w * p.bins + b] = sum; sum += n; }
+  }
+  __syncthreads();
+  for (int i0 = begin; i0 < end; i0 += 32) {
+    const int i = i0 + lane, key = i < end ? key_at(k, p, i) : 0, d = i < end ? (key >> p.shift) & (p.bins - 1) : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, d);
+    const int place = d >= 0 ? mine[d] + __popc(same & below) : 0;
+    __syncwarp();
+    if (d >= 0) {
+      p.key_out[place] = key;
+      p.row_out[place] = p.row ? p.row[i] : i;
+      if ((same & below) == 0) mine[d] += __popc(same);
+    }
+    __syncwarp();
+  }
+}
+
+// ---- sums ------------------------------------------------------------------------------------------------------------------
+template <typename T> __device__ __forceinline__ float to_f(T v);
+template <> __device__ __forceinline__ float to_f(float v) { return v; }
+template <> __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
+template <typename T, int kN> struct alignas(sizeof(T) * kN) Pack { T v[kN]; };
+
+struct Sum {
+  const int* order;
+  const int* sorted;
+  const void* dy;
+  void* grad;
+  float* parts;             // [chunks][2][width]: of a sum that began before the chunk, of one that goes on behind it
+  int rows, keys, width, chunk, chunks;
+  float scale, p;
+  unsigned long long seed, stream_id;
+  const unsigned long long* seed_dev;
+};
+
+template <typename T, int kN, bool kAdd>
+__device__ __forceinline__ void to_grad(const Sum& s, int key, int col, const float (&acc)[kN]) {
+  const long at = static_cast<long>(key) * s.width + col;
+  if constexpr (kAdd) {
+    float* g = static_cast<float*>(s.grad) + at;
+    if constexpr (kN % 4 == 0) {
+#pragma unroll
+      for (int j = 0; j < kN; j += 4) {
+        float4 v = *reinterpret_cast<float4*>(g + j);
+        v.x = fmaf(acc[j], s.scale, v.x); v.y = fmaf(acc[j + 1], s.scale, v.y);
+        v.z = fmaf(acc[j + 2], s.scale, v.z); v.w = fmaf(acc[j + 3], s.scale, v.w);
+        *reinterpret_cast<float4*>(g + j) = v;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kN; ++j) g[j] = fmaf(acc[j], s.scale, g[j]);
+    }
+  } else {
+    Pack<T, kN> o;
+#pragma unroll
+    for (int j = 0; j < kN; ++j) o.v[j] = from_f<T>(acc[j] * s.scale);
+    *reinterpret_cast<Pack<T, kN>*>(static_cast<T*>(s.grad) + at) = o;
+  }
+}
+
+// blockDim = (column vectors, chunks of this block)
+template <typename T, int kN, bool kDrop, bool kAdd>
+__global__ void __launch_bounds__(256) reduce_kernel(const Sum s) {
+  constexpr int kAhead = 8;
+  const int c = blockIdx.x * blockDim.y + threadIdx.y;
+  if (c >= s.chunks) return;
+  const int begin = c * s.chunk, end = min(s.rows, begin + s.chunk);
+  const DropRng rng(s.seed + ((kDrop && s.seed_dev) ? *s.seed_dev : 0ull), s.stream_id, s.p);
+  const int before = begin > 0 ? s.sorted[begin - 1] : -1;
+  const int after = end < s.rows ? s.sorted[end] : -1;
+  if (s.sorted[begin] >= s.keys) return;                        // rows without a key come last
+  for (int col = (blockIdx.y * blockDim.x + threadIdx.x) * kN; col < s.width; col += gridDim.y * blockDim.x * kN) {
+    float acc[kN];
+#pragma unroll
+    for (int j = 0; j < kN; ++j) acc[j] = 0.f;
+    const auto flush = [&](int key, bool began_before, bool goes_on) {
+      if (began_before || goes_on) {
+        float* part = s.parts + (static_cast<long>(c) * 2 + (began_before ? 0 : 1)) * s.width + col;
+        if constexpr (kN % 4 == 0) {
+#pragma unroll
+          for (int j = 0; j < kN; j += 4) *reinterpret_cast<float4*>(part + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kN; ++j) part[j] = acc[j];
+        }
+      } else {
+        to_grad<T, kN, kAdd>(s, key, col, acc);
+      }
+    };
+    int key = s.sorted[begin];
+    bool began_before = key == before;
+    for (int i0 = begin; i0 < end; i0 += kAhead) {
+      Pack<T, kN> v[kAhead];
+      int keys[kAhead], rows[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        keys[j] = i0 + j < end ? s.sorted[i0 + j] : s.keys;
+        rows[j] = i0 + j < end ? s.order[i0 + j] : 0;
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (keys[j] < s.keys) v[j] = *reinterpret_cast<const Pack<T, kN>*>(static_cast<const T*>(s.dy) + static_cast<long>(rows[j]) * s.width + col);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        if (i0 + j >= end) break;
+        if (keys[j] != key) {
+          if (key < s.keys) flush(key, began_before, false);
+          key = keys[j];
+          began_before = false;
+#pragma unroll
+          for (int q = 0; q < kN; ++q) acc[q] = 0.f;
+        }
+        if (key >= s.keys) break;
+#pragma unroll
+        for (int q = 0; q < kN; ++q) {
+          float f = to_f<T>(v[j].v[q]);
+          if constexpr (kDrop) {
+            const unsigned long long at = static_cast<unsigned long long>(rows[j]) * s.width + col;
+            bool keep;
+            if constexpr (kN % 4 == 0) keep = rng.keep(rng.word((at >> 2) + q / 4), q % 4);
+            else keep = rng.keep(rng.word((at + q) >> 2), static_cast<int>((at + q) & 3));
+            f = keep ? f * rng.scale : 0.f;
+          }
+          acc[q] += f;
+        }
+      }
+      if (key >= s.keys) break;
+    }
+    if (key < s.keys) flush(key, began_before, key == after);
+  }
+}
+
+// A block to each chunk in which a sum begins that goes on behind it: its parts, in 8 runs one after another, the runs in order.
+template <typename T, int kN, bool kAdd>
+__global__ void __launch_bounds__(256) join_kernel(const Sum s) {
+  constexpr int kRuns = 8, kCols = 32;
+  __shared__ float runs[kRuns][kCols * kN];
+  const int c = blockIdx.x, begin = c * s.chunk, end = begin + s.chunk;
+  if (end >= s.rows) return;
+  const int key = s.sorted[end - 1];
+  if (key >= s.keys || s.sorted[end] != key) return;
+  if (s.sorted[begin] == key && begin > 0 && s.sorted[begin - 1] == key) return;       // began earlier
+  int lo = end, hi = s.rows;                                    // first place behind the sum's last
+  while (lo < hi) { const int mid = lo + (hi - lo) / 2; if (s.sorted[mid] > key) hi = mid; else lo = mid + 1; }
+  const int n = (lo - 1) / s.chunk - c;                         // parts in the chunks behind this one
+  const int x = threadIdx.x & 31, run = threadIdx.x >> 5;
+  const int from = static_cast<int>(static_cast<long>(n + 1) * run / kRuns), to = static_cast<int>(static_cast<long>(n + 1) * (run + 1) / kRuns);
+  for (int base = blockIdx.y * kCols * kN; base < s.width; base += gridDim.y * kCols * kN) {
+    const int col = base + x * kN;
+    float acc[kN];
+#pragma unroll
+    for (int j = 0; j < kN; ++j) acc[j] = 0.f;
+    if (col < s.width) {
+#pragma unroll 4
+      for (int i = from; i < to; ++i) {
+        const float* part = s.parts + (static_cast<long>(c + i) * 2 + (i == 0 ? 1 : 0)) * s.width + col;
+        if constexpr (kN % 4 == 0) {
+#pragma unroll
+          for (int j = 0; j < kN; j += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(part + j);
+            acc[j] += v.x; acc[j + 1] += v.y; acc[j + 2] += v.z; acc[j + 3] += v.w;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < kN; ++j) acc[j] += part[j];
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kN; ++j) runs[run][x * kN + j] = acc[j];
+    __syncthreads();
+    if (run == 0 && col < s.width) {
+#pragma unroll
+      for (int j = 0; j < kN; ++j) {
+        acc[j] = 0.f;
+#pragma unroll
+        for (int r = 0; r < kRuns; ++r) acc[j] += runs[r][x * kN + j];
+      }
+      to_grad<T, kN, kAdd>(s, key, col, acc);
+    }
+    __syncthreads();
+  }
+}
+
+// out[r] = table[token] * scale
+template <typename T, int kN>
+__global__ void __launch_bounds__(256) rows_kernel(const int64_t* __restrict__ tokens, const T* __restrict__ table, T* __restrict__ out, int rows,
+                                                   int vocab, int width, float scale) {
+  for (int r = blockIdx.x * blockDim.y + threadIdx.y; r < rows; r += gridDim.x * blockDim.y) {
+    int64_t t = tokens[r];
+    if (t < 0 || t >= vocab) { NMTG_BOUNDS_HIT(); t = 0; }
+    for (int col = threadIdx.x * kN; col < width; col += blockDim.x * kN) {
+      Pack<T, kN> v = *reinterpret_cast<const Pack<T, kN>*>(table + t * width + col);
+#pragma unroll
+      for (int j = 0; j < kN; ++j) v.v[j] = from_f<T>(to_f<T>(v.v[j]) * scale);
+      *reinterpret_cast<Pack<T, kN>*>(out + static_cast<long>(r) * width + col) = v;
+    }
+  }
+}
+
+const char* problem(cudaError_t e) { return e == cudaSuccess ? nullptr : cudaGetErrorString(e); }
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+long up16(long n) { return (n + 15) & ~15L; }
+
+// Rows of a chunk: enough chunks for every SM where there are few rows, fewer parts to join where there are many
+int chunk_of(int rows) { return rows < 4096 ? 8 : rows < 32768 ? 16 : 32; }
+int key_bits(int keys) {           // of numbers up to `keys`
+  int b = 1;
+  while (b < 31 && (1L << b) <= keys) ++b;
+  return b;
+}
+
+// dim3(threads over the columns, rows or chunks of a block)
+dim3 shape(int width, int n) {
+  int x = 32;
+  while (x < 256 && x * n < width) x *= 2;
+  return dim3(x, 256 / x);
+}
+
+template <typename T, int kN, bool kDrop, bool kAdd>
+const char* sums(const Sum& s, cudaStream_t stream) {
+  const dim3 block = shape(s.width, kN);
+  reduce_kernel<T, kN, kDrop, kAdd><<<dim3((s.chunks + block.y - 1) / block.y), block, 0, stream>>>(s);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || s.chunks < 2) return problem(e);
+  const int cols = (s.width + 32 * kN - 1) / (32 * kN);
+  join_kernel<T, kN, kAdd><<<dim3(s.chunks, cols < 8 ? cols : 8), 256, 0, stream>>>(s);
+  return problem(cudaGetLastError());
+}
+
+template <typename T, int kN, bool kAdd>
+const char* sums_drop(const Sum& s, cudaStream_t stream) {
+  return s.p > 0.f ? sums<T, kN, true, kAdd>(s, stream) : sums<T, kN, false, kAdd>(s, stream);
+}
+
+template <typename T>
+const char* sums_type(const Sum& s, bool add, cudaStream_t stream) {
+  constexpr int kN = 16 / sizeof(T);
+  const bool vectors = s.width % kN == 0 && aligned(s.dy) && aligned(s.grad);
+  if (add) return vectors ? sums_drop<T, kN, true>(s, stream) : sums_drop<T, 1, true>(s, stream);
+  return vectors ? sums_drop<T, kN, false>(s, stream) : sums_drop<T, 1, false>(s, stream);
+}
+
+template <typename T>
+const char* gather(const int64_t* tokens, const void* table, void* out, int rows, int vocab, int width, float scale, cudaStream_t stream) {
+  constexpr int kN = 16 / sizeof(T);
+  const bool vectors = width % kN == 0 && aligned(table) && aligned(out);
+  const dim3 block = shape(width, vectors ? kN : 1);
+  const int blocks = (rows + static_cast<int>(block.y) - 1) / static_cast<int>(block.y), most = 32 * num_sms();
+  const int grid = blocks < most ? blocks : most;
+  if (vectors) rows_kernel<T, kN><<<grid, block, 0, stream>>>(tokens, static_cast<const T*>(table), static_cast<T*>(out), rows, vocab, width, scale);
+  else rows_kernel<T, 1><<<grid, block, 0, stream>>>(tokens, static_cast<const T*>(table), static_cast<T*>(out), rows, vocab, width, scale);
+  return problem(cudaGetLastError());
+}
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+long nmtg_embed_grad_workspace(int rows, int keys, int width) {
+  const long n = rows, chunks = (n + chunk_of(rows) - 1) / chunk_of(rows), tiles = (n + kTile - 1) / kTile;
+  return 4 * up16(4 * n) + up16(4 * tiles << kDigitBits) + up16(8 * chunks * width);
+}
+
+const char* nmtg_embed_grad(const NmtgEmbedGrad* d) {
+  cudaStream_t stream = d->stream;
+  const int size = d->dtype == 0 ? 4 : 2;
+  const long bytes = d->accumulate ? 0 : static_cast<long>(d->keys) * d->width * size;
+  if (bytes > 0 && !aligned(d->grad)) return "embedding gradient: not on a 16-byte boundary";
+  if (d->rows <= 0 || d->keys <= 0 || d->width <= 0) return bytes > 0 ? problem(cudaMemsetAsync(d->grad, 0, bytes, stream)) : nullptr;
+  const int n = d->rows, bits = key_bits(d->keys);
+  Keys k = {d->tokens, d->positions, n, d->vocab, d->keys, d->pad};
+  char* at = static_cast<char*>(d->workspace);
+  const auto take = [&](long b) { char* here = at; at += up16(b); return reinterpret_cast<int*>(here); };
+  int *key[2], *row[2];
+  for (int i = 0; i < 2; ++i) { key[i] = take(4L * n); row[i] = take(4L * n); }
+  const int tiles = (n + kTile - 1) / kTile;
+  int* counts = take(4L * tiles << kDigitBits);
+  // whole vectors are cleared beside the sort, the last bytes by themselves
+  Clear clear = {static_cast<uint4*>(d->accumulate ? nullptr : d->grad), bytes / 16, 0, 0, 1};
+  if (bytes % 16) {
+    const cudaError_t e = cudaMemsetAsync(static_cast<char*>(d->grad) + bytes / 16 * 16, 0, bytes % 16, stream);
+    if (e != cudaSuccess) return cudaGetErrorString(e);
+  }
+  const long want = (clear.n + 1023) / 1024, most = 4L * num_sms();
+  const int extra = static_cast<int>(want < most ? want : most);
+  int last = 0;
+  cudaError_t e;
+  if (n <= kRankRows && bits + kRankBits <= 32) {
+    clear.first = (n + kRankTile - 1) / kRankTile;
+    rank_kernel<<<clear.first + extra, 256, ((n + 63) & ~63) * 4, stream>>>(k, row[0], key[0], clear);
+    if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
+  } else {
+    const int passes = (bits + kDigitBits - 1) / kDigitBits, digit = (bits + passes - 1) / passes;
+    const size_t smem = 8 * sizeof(int) << digit;
+    clear.of = 3 * passes;
+    for (int i = 0; i < passes; ++i) {
+      Pass p = {i ? key[(i - 1) & 1] : nullptr, i ? row[(i - 1) & 1] : nullptr, key[i & 1], row[i & 1], counts, i * digit, 1 << digit, tiles};
+      clear.first = tiles;
+      radix_count_kernel<<<tiles + extra, 256, 0, stream>>>(k, p, clear);
+      if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
+      ++clear.at;
+      clear.first = 1;
+      radix_scan_kernel<<<1 + (extra + 3) / 4, 1024, 0, stream>>>(counts, tiles << digit, clear);
+      if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
+      ++clear.at;
+      clear.first = tiles;
+      radix_scatter_kernel<<<tiles + extra, 256, smem, stream>>>(k, p, clear);
+      if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
+      ++clear.at;
+      last = i & 1;
+    }
+  }
+  Sum s = {row[last], key[last], d->dy, d->grad, nullptr, n, d->keys, d->width, chunk_of(n), 0, d->scale, d->p, d->seed, d->stream_id, d->seed_dev};
+  s.chunks = (n + s.chunk - 1) / s.chunk;
+  s.parts = reinterpret_cast<float*>(take(8L * s.chunks * d->width));
+  if (d->dtype == 0) return sums_type<float>(s, d->accumulate, stream);
+  if (d->dtype == 1) return sums_type<__nv_bfloat16>(s, d->accumulate, stream);
+  if (d->dtype == 2) return sums_type<__half>(s, d->accumulate, stream);
+  return "embedding gradient: the type must be fp32, bf16 or fp16";
+}
+
+const char* nmtg_embed_rows(const int64_t* tokens, const void* table, void* out, int rows, int vocab, int width, int dtype, float scale,
+                            cudaStream_t stream) {
+  if (rows <= 0 || width <= 0) return nullptr;
+  if (vocab <= 0) return "embedding: the table is empty";
+  if (dtype == 0) return gather<float>(tokens, table, out, rows, vocab, width, scale, stream);
+  if (dtype == 1) return gather<__nv_bfloat16>(tokens, table, out, rows, vocab, width, scale, stream);
+  if (dtype == 2) return gather<__half>(tokens, table, out, rows, vocab, width, scale, stream);
+  return "embedding: the type must be fp32, bf16 or fp16";
+}
+
+NMTG_BOUNDS_READER(nmtg_bounds_embed_sorted)

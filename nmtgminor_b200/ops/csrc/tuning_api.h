@@ -56,4 +56,48 @@ long nmtg_pairs_workspace(int rows, int pairs);
 const char* nmtg_preference_loss(const NmtgRows* r, const NmtgPairs* p, cudaStream_t stream);
 // r->grad *= *factor, unless it is 1
 const char* nmtg_scale_rows(const NmtgRows* r, const float* factor, cudaStream_t stream);
+
+// ---- activations kept in 8 bits (kept8.cu) -----------------------------------------------------------------------------
+// dtype as above.  codes: [rows, 32 * blocks] bytes, 8-byte aligned; scales: [rows, blocks]; blocks = ceil(width / 32).  Tensors other than `in` are
+// dense [rows, width].
+struct NmtgKept {
+  const void* in;           // x (quantise), z (forward) or dy (backward), rows ld_in elements apart
+  void* out;                // restore: x' or null; forward: dropout(act(z)); backward: dropout-mask(dy) act'(z')
+  void* out2;               // restore: dropout(act(x')) or null
+  uint8_t* codes;           // forward: null where nothing is to be kept
+  uint8_t* scales;
+  long rows, width, ld_in;
+  int dtype, act;           // act: 0 none, 1 ReLU, 2 GELU (erf), 3 SiLU
+  float p;                  // dropout of the activation: the mask of dropout_add for the same seed and stream
+  unsigned long long seed, stream_id;
+  const unsigned long long* seed_dev;
+  cudaStream_t stream;
+};
+const char* nmtg_kept_quantise(const NmtgKept* k);
+const char* nmtg_kept_restore(const NmtgKept* k);
+const char* nmtg_kept_forward(const NmtgKept* k);
+const char* nmtg_kept_backward(const NmtgKept* k);
+
+// ---- embedding gradient by sorted tokens (embed_sorted.cu) ----------------------------------------------------------------
+// grad[k] (+)= scale * sum over the rows r with key k, in the order of r, of dropout-mask(dy)[r].  Key of a row: its token, or with `positions` its
+// position brought into [0, keys); none where the token is `pad` or outside [0, vocab).
+struct NmtgEmbedGrad {
+  const int64_t* tokens;    // [rows]
+  const int64_t* positions; // [rows] or null
+  const void* dy;           // dense [rows, width]
+  void* grad;               // dense [keys, width]: fp32 added to (accumulate), or of dy's type and written whole
+  int rows, vocab, keys, width;
+  int dtype, accumulate;
+  long pad;
+  float scale, p;
+  unsigned long long seed, stream_id;
+  const unsigned long long* seed_dev;
+  void* workspace;          // nmtg_embed_grad_workspace bytes, 16-byte aligned
+  cudaStream_t stream;
+};
+long nmtg_embed_grad_workspace(int rows, int keys, int width);
+const char* nmtg_embed_grad(const NmtgEmbedGrad* e);
+// out[r] = table[tokens[r]] * scale, dense [rows, width] of the table's type; tokens outside the table read its first row
+const char* nmtg_embed_rows(const int64_t* tokens, const void* table, void* out, int rows, int vocab, int width, int dtype, float scale,
+                            cudaStream_t stream);
 }

@@ -33,6 +33,38 @@ def linear(x, weight, bias, act_id, dropout_p, residual):
     return y
 
 
+def linear_kept(x, weight, bias, act_id, dropout_p, residual):
+    """``linear`` whose input and pre-activation wait for the backward pass in 8 bits."""
+    from . import kept
+    y = kept.act_reference(kept.linear_reference(x, weight.to(x.dtype), bias.to(x.dtype) if bias is not None else None), act_id)
+    if dropout_p > 0:
+        y = F.dropout(y, dropout_p, True)
+    return y if residual is None else y + residual
+
+
+def mlp_kept(x, w1, b1, w2, b2, act_id, p1, p2, residual):
+    """The feed-forward block whose input and hidden layer wait for the backward pass in 8 bits: with ReLU (act 1) the activated hidden layer
+    (its signs exact), otherwise the pre-activation, from which the activated one is computed again."""
+    from . import kept
+    z = kept.linear_reference(x, w1.to(x.dtype), b1.to(x.dtype) if b1 is not None else None)
+    h = _act(z, act_id) if act_id == 1 else kept.act_reference(z, act_id)
+    mask = F.dropout(torch.ones_like(h), p1, True) if p1 > 0 else None
+    h = h if mask is None else h * mask
+    w, b = w2.to(h.dtype), b2.to(h.dtype) if b2 is not None else None
+    y = F.linear(h, w.detach(), b)
+    if w2.requires_grad:
+        if act_id == 1:
+            again = kept.restore_reference(kept.quantise_reference(h)).to(h.dtype)
+        else:
+            again = _act(kept.restore_reference(kept.quantise_reference(z)).to(z.dtype), act_id)
+            again = again if mask is None else again * mask
+        term = F.linear(again, w)
+        y = y + (term - term.detach())
+    if p2 > 0:
+        y = F.dropout(y, p2, True)
+    return y if residual is None else y + residual
+
+
 def layer_norm(x, weight, bias, eps):
     return F.layer_norm(x, (x.shape[-1],), weight.to(x.dtype), bias.to(x.dtype), eps)
 
