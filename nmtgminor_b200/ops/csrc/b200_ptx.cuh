@@ -28,7 +28,6 @@ enum Status : int {
   kTimeoutTmemEmpty = 4,  // MMA warp waited for an accumulator that was never drained
   kTimeoutPeerFlag = 5,   // a peer GPU never raised its flag
   kTimeoutGather = 7,     // the in-kernel gather of a sharded operand never completed a segment
-  kTimeoutPair = 8,       // a gradient of a paired loss waited in vain for the sums of its pair
   kBadArgument = 6,
 };
 

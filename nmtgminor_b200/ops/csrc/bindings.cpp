@@ -591,7 +591,6 @@ void clear_status(int64_t device) { status_tensor(static_cast<int>(device)).zero
 
 void bind_sequence_ops(pybind11::module& m);   // bindings_seq.cpp
 void bind_tuning_ops(pybind11::module& m);     // bindings_tuning.cpp
-int* nmtg_status_word(int device) { return status_tensor(device).data_ptr<int>(); }
 const unsigned long long* nmtg_seed_word(int device) { return reinterpret_cast<const unsigned long long*>(seed_tensor(device).data_ptr<int64_t>()); }
 extern "C" long nmtg_bounds_violations();
 

@@ -5,8 +5,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include "tuning_api.h"
 
-int* nmtg_status_word(int device);                          // bindings.cpp
-const unsigned long long* nmtg_seed_word(int device);
+const unsigned long long* nmtg_seed_word(int device);       // bindings.cpp
 
 namespace {
 
@@ -53,7 +52,6 @@ NmtgRows rows_of(const Tensor& logits, const Tensor& labels, int64_t pad, double
   r.inv_temperature = static_cast<float>(1.0 / temperature);
   r.pad = pad;
   r.grad_scale = 1.f;
-  r.status = nmtg_status_word(logits.get_device());
   TORCH_CHECK(address(logits) % logits.element_size() == 0, "logits: misaligned elements");
   return r;
 }
@@ -65,6 +63,12 @@ Tensor grad_like(const Tensor& logits, const NmtgRows& r) {
   return at::empty({before + n}, logits.options().requires_grad(false)).as_strided({r.rows, r.vocab}, {r.ld, 1}, before);
 }
 
+Tensor workspace(const Tensor& logits, NmtgRows& r, int pairs) {
+  Tensor t = at::empty({nmtg_rows_workspace(r.rows, r.vocab, r.dtype, pairs)}, logits.options().dtype(at::kByte).requires_grad(false));
+  r.workspace = t.data_ptr();
+  return t;
+}
+
 std::tuple<Tensor, Tensor> row_scores(const Tensor& logits, const Tensor& labels, int64_t pad, double temperature, bool keep_stat) {
   NmtgRows r = rows_of(logits, labels, pad, temperature);
   c10::cuda::CUDAGuard guard(logits.device());
@@ -72,6 +76,7 @@ std::tuple<Tensor, Tensor> row_scores(const Tensor& logits, const Tensor& labels
   Tensor lp = at::empty({r.rows}, f32), stat = at::empty({keep_stat ? r.rows : 0, 2}, f32);
   r.logprobs = lp.data_ptr<float>();
   r.stat = keep_stat ? reinterpret_cast<float2*>(stat.data_ptr<float>()) : nullptr;
+  const Tensor work = workspace(logits, r, 0);
   ck(nmtg_row_scores(&r, cur_stream()));
   return {lp, stat};
 }
@@ -84,6 +89,7 @@ Tensor row_scores_grad(const Tensor& logits, const Tensor& labels, const Tensor&
   Tensor grad = grad_like(logits, r);
   r.grad = grad.data_ptr();
   r.stat = reinterpret_cast<float2*>(stat.data_ptr<float>());
+  const Tensor work = workspace(logits, r, 0);
   ck(nmtg_row_scores_grad(&r, weight.data_ptr<float>(), cur_stream()));
   return grad;
 }
@@ -116,10 +122,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, OptTensor> policy_loss(const Tensor& 
   p.clip_high = static_cast<float>(1.0 + clip_high);
   p.kl_coef = static_cast<float>(kl_coef);
   const auto f32 = logits.options().dtype(at::kFloat).requires_grad(false);
-  Tensor lp = at::empty({r.rows}, f32), loss = at::empty({1}, f32), kl = at::empty({1}, f32), clipped = at::empty({1}, f32), rows = at::empty({3, r.rows}, f32.dtype(at::kDouble));
+  Tensor lp = at::empty({r.rows}, f32), loss = at::empty({1}, f32), kl = at::empty({1}, f32), clipped = at::empty({1}, f32);
+  const Tensor work = workspace(logits, r, 0);
   Tensor g = grad_of(logits, r, grad, scale_at, scale);
   r.logprobs = lp.data_ptr<float>();
-  p.row_loss = rows.data_ptr<double>();
   p.loss = loss.data_ptr<float>();
   p.kl = kl.data_ptr<float>();
   p.clipped = clipped.data_ptr<float>();
@@ -147,13 +153,12 @@ std::tuple<Tensor, Tensor, Tensor, OptTensor> preference_loss(const Tensor& logi
   p.margin = static_cast<float>(margin);
   p.nll_weight = static_cast<float>(nll_weight);
   const auto f32 = logits.options().dtype(at::kFloat).requires_grad(false);
-  Tensor seq = at::empty({2 * static_cast<int64_t>(p.pairs)}, f32), loss = at::empty({1}, f32), ranked = at::empty({1}, f32),
-         work = at::empty({nmtg_pairs_workspace(r.rows, p.pairs)}, f32.dtype(at::kByte));
+  Tensor seq = at::empty({2 * static_cast<int64_t>(p.pairs)}, f32), loss = at::empty({1}, f32), ranked = at::empty({1}, f32);
+  const Tensor work = workspace(logits, r, p.pairs);
   Tensor g = grad_of(logits, r, grad, scale_at, scale);
   p.seq_logprobs = seq.data_ptr<float>();
   p.loss = loss.data_ptr<float>();
   p.ranked = ranked.data_ptr<float>();
-  p.workspace = work.data_ptr();
   ck(nmtg_preference_loss(&r, &p, cur_stream()));
   return {loss, ranked, seq, g.defined() ? OptTensor(g) : OptTensor()};
 }

@@ -3,18 +3,12 @@
 //     lp = (x[y] - M) / T - log s          d lp / d x = (onehot(y) - exp((x - M) / T) / s) / T
 // Each loss is a function of the lp of its rows, so a row's gradient is one coefficient times d lp / d x.
 //
-// One kernel serves all of them (rows_kernel): a block, or a cluster of up to 8 blocks for a long row, takes a whole row, 32 elements of
-// 16 bits (16 of 32 bits) a thread, so a row is read from memory once.  Every thread copies the vectors that it will itself use
-// (cp.async, two rows ahead of the one in work), which needs no barrier but the one of the row's sum.  Blocks have as few threads as hold a
-// row, 1024 threads to an SM in all: 64 KB of rows in work and 128 KB on their way.
-//   * the policy loss knows its coefficient once the row is summed: exp((x - max of the thread) / T) stays in registers, and the gradient is
-//     one multiplication; each logit is read once, its gradient written once, and one exponential taken (of 16 a cycle and SM, the sum
-//     and the gradient together would take three quarters of the time that the row's bytes do).
-//   * the paired loss knows it once every row of the pair is summed.  Work is handed out in one order, the sum of row i + lag before the
-//     gradient of row i, lag = the longest pair and what is in work elsewhere; the gradient's read then comes from L2 where a
-//     pair is small against it.  A gradient waits for its pair only (bounded), and whatever it waits for was handed out before it to a
-//     block that runs: no order of blocks can lock.
-// A row that no cluster holds is read twice (kLong).
+// rows_kernel takes a piece of a row at a time: its sums, or its gradient, or for the policy loss of rows that a block holds both, the logits
+// read once.  The scores, the paired loss and the policy loss of longer rows are two passes, sums and then gradients, with a small kernel between
+// that makes rows of the pieces and coefficients of the rows.  (Both passes at once, the gradients some rows behind the sums so
+// that they would find the logits in L2, were built and measured: 353 us against 272 for 8200 rows of 32000 in bf16.  The coefficient of a pair
+// comes so late that most blocks wait for it.)
+// Bound by memory in 32 bits and in every gradient pass; the sums of 16-bit logits are bound by exponentials, 16 a cycle and SM.
 //
 // All sums over rows are taken in one order in 64 bits: results do not depend on which block was first.
 // This file is compiled without fast math: expf and logf below are the accurate ones, ex2 where it is asked for.
@@ -31,29 +25,26 @@ int num_sms();
 
 namespace {
 
-constexpr int kVecs = 4;              // 16-byte vectors of a row that a thread holds
-constexpr int kAhead = 2;             // rows on their way to shared memory
-constexpr int kSlots = kAhead + 1;
-constexpr int kMaxCluster = 8;
-constexpr int kRing = 8;              // numbers of work items known ahead (kAhead + 3 needed)
+constexpr int kVecs = 8;              // 16-byte vectors of an item that a thread holds
+constexpr int kSlots = 3;             // items in shared memory or on their way there
+constexpr int kRing = 8;              // entries of work known: one behind, kSlots + 3 ahead, and that in hand
+constexpr int kBlock = 256, kWide = 512;      // threads of a block for the elements; two or three blocks to an SM, and one
 
-enum Mode { kScores = 0, kGrad = 1, kPolicy = 2, kPairs = 3 };
+// kScores: sums of pieces.  kGrad: gradients from `stat` or `part` and a coefficient.  kLocal: the policy loss of rows that one block holds.
+enum Mode { kScores = 0, kGrad = 1, kLocal = 2 };
 
-struct PairState {          // the head of the workspace
-  int ticket, longest, pairs_done, pairs_expected, failed;
-};
-struct PairWork {
-  PairState* state;
+struct State { int ticket, pairs_done; };
+struct Work {
+  State* state;
+  float2* part;             // [rows][pieces] largest logit, sum of exponentials
+  float2* stat;             // [rows] the same of a row
+  float* coef;              // [2 pairs] or [rows]: d loss / d lp
   int* cu;                  // [2 pairs + 1] offsets, put in order and into range
   int* seq;                 // [rows] sequence of a row, -1: none
   int* label;               // [rows] label of a row, -1: padding
-  int* arrived;             // [pairs] rows summed so far
-  int* ready;               // [pairs] 1 once `coef` holds
-  float* coef;              // [2 pairs] d loss / d lp of the rows of a sequence
   double* lp;               // [rows]
   double* loss;             // [pairs]
   int* ranked;              // [pairs]
-  float2* stat;             // [rows]
 };
 
 struct Args {
@@ -62,17 +53,18 @@ struct Args {
   const int64_t* labels;
   long ld, pad;
   int rows, vocab;
+  int pieces, each;         // of a row; vectors of a piece
+  int slot;                 // vectors of a slot
+  int aligned;              // every row starts on a 16-byte boundary
   float k, inv_t;           // log2(e) / T, 1 / T
   float* logprobs;
   float2* stat;
-  const float* weight;
+  const float* weight;      // kGrad: of rows or, where `w.seq` is there, of sequences
   const float* scale_at;    // the gradient's factor on the device, or null
   float scale;
   NmtgPolicy policy;
   NmtgPairs pairs;
-  PairWork w;
-  int slack;                // rows between a pair's end and the gradients taken up, beyond the longest pair
-  int* status;
+  Work w;
 };
 
 template <typename T> struct Num;
@@ -81,11 +73,12 @@ template <> struct Num<float> {
   static constexpr uint32_t kLow = 0xFF800000u;                   // -inf
   static __device__ __forceinline__ float get(float v) { return v; }
   static __device__ __forceinline__ float put(float v) { return v; }
-  static __device__ __forceinline__ void unpack(const uint4& u, float (&f)[4]) {
-    f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+  static __device__ __forceinline__ void unpack(const uint4& u, float2 (&f)[2]) {
+    f[0] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+    f[1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
   }
-  static __device__ __forceinline__ uint4 pack(const float (&f)[4]) {
-    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  static __device__ __forceinline__ uint4 pack(const float2 (&f)[2]) {
+    return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
   }
   static __device__ __forceinline__ float largest(const uint4& u) {
     return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
@@ -96,16 +89,16 @@ template <> struct Num<__nv_bfloat16> {
   static constexpr uint32_t kLow = 0xFF80FF80u;
   static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
-  static __device__ __forceinline__ void unpack(const uint4& u, float (&f)[8]) {
+  static __device__ __forceinline__ void unpack(const uint4& u, float2 (&f)[4]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) { f[2 * j] = __uint_as_float(w[j] << 16); f[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u); }
+    for (int j = 0; j < 4; ++j) f[j] = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
   }
-  static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
+  static __device__ __forceinline__ uint4 pack(const float2 (&f)[4]) {
     uint4 o;
     __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&o);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) h[j] = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
+    for (int j = 0; j < 4; ++j) h[j] = __floats2bfloat162_rn(f[j].x, f[j].y);
     return o;
   }
   static __device__ __forceinline__ float largest(const uint4& u) {
@@ -119,16 +112,16 @@ template <> struct Num<__half> {
   static constexpr uint32_t kLow = 0xFC00FC00u;
   static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
   static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
-  static __device__ __forceinline__ void unpack(const uint4& u, float (&f)[8]) {
+  static __device__ __forceinline__ void unpack(const uint4& u, float2 (&f)[4]) {
     const __half2* h = reinterpret_cast<const __half2*>(&u);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) { const float2 t = __half22float2(h[j]); f[2 * j] = t.x; f[2 * j + 1] = t.y; }
+    for (int j = 0; j < 4; ++j) f[j] = __half22float2(h[j]);
   }
-  static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
+  static __device__ __forceinline__ uint4 pack(const float2 (&f)[4]) {
     uint4 o;
     __half2* h = reinterpret_cast<__half2*>(&o);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+    for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(f[j].x, f[j].y);
     return o;
   }
   static __device__ __forceinline__ float largest(const uint4& u) {
@@ -138,32 +131,41 @@ template <> struct Num<__half> {
   }
 };
 
+// 2^v; below 2^-126 zero: 2^-126 of a sum that is at least 1
 __device__ __forceinline__ float ex2(float v) {
   float r;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// two 32-bit operations in one instruction
+__device__ __forceinline__ uint64_t both(float2 v) { return *reinterpret_cast<const uint64_t*>(&v); }
+__device__ __forceinline__ float2 each(uint64_t v) { return *reinterpret_cast<const float2*>(&v); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(both(a)), "l"(both(b)));
+  return each(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(both(a)), "l"(both(b)));
+  return each(r);
+}
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
 __device__ __forceinline__ void copy16(uint4* to, const uint4* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
 }
+__device__ __forceinline__ void copy4(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy8(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kLeft> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
-__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
-  uint32_t r;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
-  return r;
-}
-template <bool kCluster> __device__ __forceinline__ void meet() {
-  if constexpr (kCluster) {
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  } else {
-    __syncthreads();
-  }
-}
-
 // sum of exponentials relative to a reference; a reference of -inf stands for no elements (or only -inf ones) and a sum of 0
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2, float k) {
   const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top;
@@ -171,45 +173,62 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2, flo
   m = top;
 }
 __device__ __forceinline__ void join_lanes(float& m, float& s, float k) {
+  const float top = warp_max(m), base = top == -INFINITY ? 0.f : top;
+  s *= ex2((m - base) * k);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) join(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o), k);
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  m = top;
+}
+// exponentials of a vector relative to a reference: 2^((x - base) k)
+template <typename T>
+__device__ __forceinline__ void exps(const uint4& u, float minus_base, float k, float2 (&e)[Num<T>::kE / 2]) {
+  Num<T>::unpack(u, e);
+#pragma unroll
+  for (int q = 0; q < Num<T>::kE / 2; ++q) {
+    const float2 v = mul2(add2(e[q], make_float2(minus_base, minus_base)), make_float2(k, k));
+    e[q] = make_float2(ex2(v.x), ex2(v.y));
+  }
 }
 
-// (x[y] - M) / T - log s in 64 bits; log s as exponent * log 2 + log of a mantissa near 1, whose 32-bit rounding is below 2^-25
-__device__ __forceinline__ double log_probability(float xy, float m, float s, float inv_t) {
+// A log-probability (x[y] - M) / T - log s as a sum of two floats: log s is an exponent times log 2, whose upper part has 15 bits so that the product is
+// exact, and the log of a mantissa near 1, whose rounding is below 2^-26; the rounding of the sum of the large terms is kept.
+struct LogProb {
+  float hi, lo;
+  __device__ __forceinline__ double wide() const { return static_cast<double>(hi) + lo; }
+  __device__ __forceinline__ float minus(float v) const { return (hi - v) + lo; }
+};
+__device__ __forceinline__ LogProb log_probability(float xy, float m, float s, float inv_t) {
+  const float t = (xy - m) * inv_t;
+  if (!(s > 0.f && s < 3e38f)) return LogProb{t - logf(s), 0.f};           // nothing but -inf, or NaN
   const uint32_t bits = __float_as_uint(s);
-  if (!(s > 0.f) || bits >= 0x7F800000u || bits < 0x00800000u) return (static_cast<double>(xy) - m) * inv_t - log(static_cast<double>(s));
   int e = static_cast<int>(bits >> 23) - 127;
   float f = __uint_as_float((bits & 0x007FFFFFu) | 0x3F800000u);
   if (f > 1.41421356f) { f *= 0.5f; ++e; }
-  return (static_cast<double>(xy) - m) * inv_t - (e * 0.693147180559945309417 + static_cast<double>(logf(f)));
+  const float n = static_cast<float>(-e), big = n * 0.693145751953125f;     // log 2 = 0.693145751953125 + 1.42860682030941723e-6
+  const float hi = t + big, back = hi - t, lost = (t - (hi - back)) + (big - back);
+  const float lo = lost + fmaf(n, 1.42860682e-6f, -logf(f)), sum = hi + lo;
+  return fabsf(hi) < INFINITY ? LogProb{sum, lo - (sum - hi)} : LogProb{hi, 0.f};
 }
 
-// a row as this block's part of it: vectors [v0, v1) after `head` single elements, `tail` single ones at the end
-template <typename T> struct Span {
-  const T* x;
-  T* g;
-  int head, tail, nvec, v0, v1;
-  __device__ __forceinline__ Span(const Args& a, int row, uint32_t rank, uint32_t parts) {
-    x = static_cast<const T*>(a.x) + static_cast<long>(row) * a.ld;
-    g = a.g ? static_cast<T*>(a.g) + static_cast<long>(row) * a.ld : nullptr;
-    head = min(static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / static_cast<int>(sizeof(T)), a.vocab);
-    nvec = (a.vocab - head) / Num<T>::kE;
-    tail = a.vocab - head - nvec * Num<T>::kE;
-    const int each = (nvec + static_cast<int>(parts) - 1) / static_cast<int>(parts);
-    v0 = min(nvec, static_cast<int>(rank) * each);
-    v1 = min(nvec, v0 + each);
-  }
-  __device__ __forceinline__ const uint4* xv() const { return reinterpret_cast<const uint4*>(x + head); }
-  __device__ __forceinline__ uint4* gv() const { return reinterpret_cast<uint4*>(g + head); }
-  // the single element of this thread, -1: none.  Threads 0..7 of the first block have the head, 8..15 of the last the tail.
-  __device__ __forceinline__ int single(uint32_t rank, uint32_t parts) const {
-    const int t = threadIdx.x;
-    if (rank == 0 && t < head) return t;
-    if (rank == parts - 1 && t >= 8 && t - 8 < tail) return head + nvec * Num<T>::kE + t - 8;
-    return -1;
-  }
-};
+// A piece of a row: vectors [v0, v1) behind `head` single elements; `tail` single ones follow the row's last vector.
+struct Shape { int head, tail, nvec, v0, v1; };
+template <typename T>
+__device__ __forceinline__ Shape shape_of(const Args& a, const T* x, int piece) {
+  Shape s;
+  s.head = a.aligned ? 0 : min(static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / static_cast<int>(sizeof(T)), a.vocab);
+  s.nvec = (a.vocab - s.head) / Num<T>::kE;
+  s.tail = a.vocab - s.head - s.nvec * Num<T>::kE;
+  s.v0 = min(s.nvec, piece * a.each);
+  s.v1 = min(s.nvec, s.v0 + a.each);
+  return s;
+}
+// The single element of this thread, -1: none.  Threads 0..7 have the head with the first piece, 8..15 the tail with the last.
+template <typename T>
+__device__ __forceinline__ int single_at(const Shape& s, int thread, int piece, int pieces) {
+  if (piece == 0 && thread < s.head) return thread;
+  if (piece == pieces - 1 && thread >= 8 && thread - 8 < s.tail) return s.head + s.nvec * Num<T>::kE + thread - 8;
+  return -1;
+}
 
 // loss of pair p from the sums of its two sequences: one lane
 __device__ __noinline__ void pair_loss(const Args& a, int p, double sw, double sl, int nw, int nl) {
@@ -239,346 +258,359 @@ __device__ __noinline__ void pair_loss(const Args& a, int p, double sw, double s
     }
   }
   if (q.nll_weight != 0.f) loss -= q.nll_weight * cw * sw;
-  a.w.coef[2 * p] = static_cast<float>(cw * (slope - q.nll_weight));
-  a.w.coef[2 * p + 1] = static_cast<float>(-cl * slope);
   a.w.loss[p] = loss;
   a.w.ranked[p] = h > 0.0;
+  a.w.coef[2 * p] = static_cast<float>(cw * (slope - q.nll_weight));
+  a.w.coef[2 * p + 1] = static_cast<float>(-cl * slope);
 }
 
-// all lanes of a warp, after the last pair
-__device__ __noinline__ void total_loss(const Args& a) {
-  __syncwarp();
-  __threadfence();
-  double loss = 0.0;
-  int ranked = 0;
-  for (int p = threadIdx.x & 31; p < a.pairs.pairs; p += 32) { loss += __ldcg(a.w.loss + p); ranked += __ldcg(a.w.ranked + p); }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    loss += __shfl_xor_sync(0xffffffffu, loss, o);
-    ranked += __shfl_xor_sync(0xffffffffu, ranked, o);
-  }
-  if ((threadIdx.x & 31) == 0) { *a.pairs.loss = static_cast<float>(loss); *a.pairs.ranked = static_cast<float>(ranked); }
+// An item of work, a piece of a row.  row -1: no more; label -1: padding.
+struct __align__(16) Entry { int row, piece, label, unused; };
+// What the last warp needs of an entry
+struct __align__(16) Mail {
+  union { int64_t label; int label32; };
+  float2 stat;
+  uint32_t word, upper;     // the label's logit, of 16 bits the upper half where `upper`
+  int seq;
+  float old, adv, ref;      // kGrad: `old` is the weight
+};
+
+// d loss / d lp of a row under the policy loss
+__device__ __forceinline__ float policy_coef(const Args& a, LogProb lp, float old, float adv, float ref) {
+  const float ratio = expf(lp.minus(old)), held = fminf(fmaxf(ratio, a.policy.clip_low), a.policy.clip_high);
+  const bool free = !(ratio * adv > held * adv);           // NaN counts as free, so that it shows
+  const float up = a.policy.ref_logprobs ? expm1f(-lp.minus(ref)) : 0.f;
+  return (free ? -ratio * adv : 0.f) - a.policy.kl_coef * up;
 }
 
-// all lanes of a warp, after the last row of pair p: sums in one order, coefficients, and at the last pair the loss
-__device__ __noinline__ void finish_pair(const Args& a, int p) {
-  __syncwarp();
-  __threadfence();               // behind lane 0, which has counted the last arrival: the other blocks' rows
-  const int lane = threadIdx.x & 31;
-  double sum[2];
-  int count[2];
-  for (int h = 0; h < 2; ++h) {
-    double s = 0.0;
-    int n = 0;
-    for (int r = a.w.cu[2 * p + h] + lane; r < a.w.cu[2 * p + h + 1]; r += 32) {
-      s += __ldcg(a.w.lp + r);
-      n += a.w.label[r] >= 0;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) { s += __shfl_xor_sync(0xffffffffu, s, o); n += __shfl_xor_sync(0xffffffffu, n, o); }
-    sum[h] = s;
-    count[h] = n;
-  }
-  int last = 0;
-  if (lane == 0) {
-    pair_loss(a, p, sum[0], sum[1], count[0], count[1]);
-    __threadfence();
-    atomicExch(a.w.ready + p, 1);
-    last = atomicAdd(&a.w.state->pairs_done, 1) + 1 == a.w.state->pairs_expected;
-    __threadfence();
-  }
-  if (__shfl_sync(0xffffffffu, last, 0)) total_loss(a);
-}
-
-// Work item: row and whether it is the gradient's turn; row -1: no more
-struct Item { int row; bool grad; };
-__device__ __forceinline__ Item pair_item(int t, int rows, int lag, bool grads) {
-  if (!grads) return {t < rows ? t : -1, false};
-  if (t < lag) return {t, false};
-  if (t < 2 * rows - lag) { const int u = t - lag; return (u & 1) ? Item{u >> 1, true} : Item{lag + (u >> 1), false}; }
-  return {t < 2 * rows ? t - rows : -1, true};
-}
-
-template <typename T, int kThreads, int kMode, bool kCluster, bool kLong>
-__global__ void __launch_bounds__(kThreads, 1024 / kThreads) rows_kernel(const __grid_constant__ Args a) {
-  constexpr int kE = Num<T>::kE, kWarps = kThreads / 32, kParts = kCluster ? kMaxCluster : 1;
-  extern __shared__ __align__(16) uint4 slots[];            // [kSlots][kVecs][kThreads]
-  __shared__ float2 part[2][kParts * kWarps];
+// kCompute threads do the elements' work; one more warp fetches the entries, joins the partial sums and brings the coefficients.  Step i of the
+// block: the sums of entry i, the barrier, the gradient of entry i - 1 (its logits still in their slot).  Between barriers i - 1 and i the last warp
+// joins the sums of entry i - 1 and brings its coefficient, and publishes entry i + kLead + 1.
+template <typename T, int kCompute, int kMode>
+__global__ void __launch_bounds__(kCompute + 32, kCompute == kBlock ? 3 : 1) rows_kernel(const __grid_constant__ Args a) {
+  constexpr int kE = Num<T>::kE, kWarps = kCompute / 32;
+  constexpr bool kSums = kMode != kGrad, kGrads = kMode != kScores;
+  constexpr int kLead = kMode == kScores ? kSlots : kSlots - 1;             // entries whose logits are under way
+  extern __shared__ __align__(16) uint4 slots[];            // [kSlots][a.slot]
+  __shared__ float2 part[2][kWarps];
   __shared__ float4 bc[2];                                  // largest logit, factor of the exponentials, coefficient / T
-  __shared__ int ring[kRing];
-  const uint32_t rank = kCluster ? cluster_rank() : 0, parts = kCluster ? cluster_size() : 1;
+  __shared__ Entry ring[kRing];
+  __shared__ Mail mail[kRing];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const int groups = static_cast<int>(gridDim.x / parts), group = static_cast<int>(blockIdx.x / parts);
-  const float scale = a.scale_at ? *a.scale_at * a.scale : a.scale;
-  const int lag = kMode == kPairs ? min(a.rows, a.w.state->longest + a.slack) : 0;
+  const T* const x0 = static_cast<const T*>(a.x);
+  T* const g0 = static_cast<T*>(a.g);
 
-  const auto item = [&](int i) -> Item {
-    if constexpr (kMode == kPairs) {
-      return pair_item(ring[i & (kRing - 1)], a.rows, lag, a.g != nullptr);
-    } else {
-      const long r = group + static_cast<long>(i) * groups;
-      return {r < a.rows ? static_cast<int>(r) : -1, kMode == kGrad};
-    }
-  };
-  const auto label_of = [&](int row) -> int {
-    if (row < 0) return -1;
-    if constexpr (kMode == kPairs) {
-      return a.w.label[row];
-    } else {
-      const int64_t y = a.labels[row];
-      return y == a.pad || y < 0 || y >= a.vocab ? -1 : static_cast<int>(y);
-    }
-  };
-  const auto issue = [&](int i, int row, int label) {
-    if constexpr (!kLong) {
-      if (label >= 0) {
-        const Span<T> s(a, row, rank, parts);
-        uint4* to = slots + (i % kSlots) * (kVecs * kThreads) + t;
+  if (warp == kWarps) {
+    // ------------------------------------------------------------------------------------------------ the last warp
+    const float scale = a.scale_at ? *a.scale_at * a.scale : a.scale;
+    // What an entry needs comes by asynchronous copies, so that this warp never waits for memory: at step i the label of entry i + kLead + 3, at step
+    // i + 2, when its label is there and the entry is published, its logit and the numbers of its row.
+    // Items are handed out one by one, asked for a step ahead: SMs do not get at memory equally fast, and equal shares would wait for the slowest
+    // (sums of 8200 rows of 32000: most blocks done after 87 us, the last after 111).
+    const auto next_number = [&](int i) -> int {              // of entry i
+      if (a.w.state) return atomicAdd(&a.w.state->ticket, 1);
+      return i == 0 ? static_cast<int>(blockIdx.x) : a.rows * a.pieces;      // an item to each block
+    };
+    const auto ask = [&](int i, int number) {                 // lane 0
+      const int q = a.pieces == 1 ? number : number / a.pieces;
+      const Entry e = {q < a.rows ? q : -1, number - q * a.pieces, -1, 0};
+      Mail& m = mail[i & (kRing - 1)];
+      if (e.row < 0) m.label = -1;
+      else if (a.w.label) copy4(&m.label32, a.w.label + e.row);
+      else copy8(&m.label, a.labels + e.row);
+      if (kMode == kGrad && e.row >= 0 && a.w.seq) copy4(&m.seq, a.w.seq + e.row);
+      ring[i & (kRing - 1)] = e;
+    };
+    const auto publish = [&](int i) {                         // lane 0
+      Mail& m = mail[i & (kRing - 1)];
+      Entry e = ring[i & (kRing - 1)];
+      if (e.row >= 0) {
+        if (a.w.label) e.label = m.label32;
+        else e.label = m.label == a.pad || m.label < 0 || m.label >= a.vocab ? -1 : static_cast<int>(m.label);
+      }
+      ring[i & (kRing - 1)] = e;
+      if (e.label >= 0) {
+        if constexpr (kMode == kLocal) {
+          const uintptr_t at = reinterpret_cast<uintptr_t>(x0 + static_cast<long>(e.row) * a.ld + e.label);
+          m.upper = at & 2;
+          copy4(&m.word, reinterpret_cast<const void*>(at & ~static_cast<uintptr_t>(3)));
+          copy4(&m.old, a.policy.old_logprobs + e.row);
+          copy4(&m.adv, a.policy.advantages + e.row);
+          if (a.policy.ref_logprobs) copy4(&m.ref, a.policy.ref_logprobs + e.row);
+        }
+        if constexpr (kMode == kGrad) {
+          copy8(&m.stat, a.stat + e.row);
+          copy4(&m.old, a.weight + (a.w.seq ? m.seq : e.row));
+        }
+      }
+    };
+    const auto logit_of = [&](const Mail& m) -> float {
+      if constexpr (sizeof(T) == 4) return __uint_as_float(m.word);
+      else return Num<T>::get(reinterpret_cast<const T*>(&m.word)[m.upper ? 1 : 0]);
+    };
+    int fresh = 0;                                           // the number of entry i + kLead + 3
+    if (lane == 0) {
+      int first[kLead + 3];
 #pragma unroll
-        for (int j = 0; j < kVecs; ++j)
-          if (s.v0 + t + j * kThreads < s.v1) copy16(to + j * kThreads, s.xv() + s.v0 + t + j * kThreads);
+      for (int i = 0; i < kLead + 3; ++i) first[i] = next_number(i);
+      fresh = next_number(kLead + 3);
+#pragma unroll
+      for (int i = 0; i < kLead + 3; ++i) ask(i, first[i]);
+      copies_end();
+      copies_wait<0>();
+      for (int i = 0; i < kLead + 1; ++i) publish(i);
+    }
+    copies_end();
+    __syncthreads();
+    Entry before = Entry{-1, 0, -1, 0};                      // entry i - 1
+    for (int i = 0;; ++i) {
+      const Entry now = ring[i & (kRing - 1)];
+      copies_wait<1>();
+      if (lane == 0) {
+        publish(i + kLead + 1);
+        ask(i + kLead + 3, fresh);
+        fresh = next_number(i + kLead + 4);
       }
       copies_end();
-    }
-  };
-  const auto single_of = [&](int row) -> float {
-    if (row < 0) return -INFINITY;
-    const Span<T> s(a, row, rank, parts);
-    const int e = s.single(rank, parts);
-    return e >= 0 ? Num<T>::get(s.x[e]) : -INFINITY;
-  };
-
-  if constexpr (kCluster) meet<true>();     // every block of the cluster runs before the first store to its shared memory
-  if constexpr (kMode == kPairs) {
-    if (rank == 0 && t == 0) {
-      const int first = atomicAdd(&a.w.state->ticket, kAhead + 2);
-      for (int i = 0; i < kAhead + 2; ++i) {
-        ring[i] = first + i;
-        if constexpr (kCluster)
-          for (uint32_t c = 1; c < parts; ++c) asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(at_rank(ring + i, c)), "r"(first + i) : "memory");
-      }
-    }
-  }
-  if constexpr (kMode == kPairs) meet<kCluster>();
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) { const int r = item(i).row; issue(i, r, label_of(r)); }
-  int label = label_of(item(0).row), label_ahead = label_of(item(kAhead).row);
-  float one = single_of(item(0).row);
-
-  for (int i = 0;; ++i) {
-    const Item now = item(i);
-    if (now.row < 0) break;
-    const int row = now.row;
-    int ticket = 0;
-    if constexpr (kMode == kPairs)
-      if (rank == 0 && t == 0) ticket = atomicAdd(&a.w.state->ticket, 1);
-    issue(i + kAhead, item(i + kAhead).row, label_ahead);
-    label_ahead = label_of(item(i + kAhead + 1).row);
-    const int next = item(i + 1).row, next_label = label_of(next);
-    const float next_one = single_of(next);
-
-    const Span<T> s(a, row, rank, parts);
-    const bool real = label >= 0;
-    const bool grads = kMode == kPolicy || now.grad;
-    const bool sums = kMode != kGrad && !now.grad;
-    const float xy = real ? Num<T>::get(s.x[label]) : 0.f;
-    uint4 raw[kLong ? 1 : kVecs];
-    float e[kMode == kPolicy && !kLong ? kVecs * kE : 1];
-    float m = -INFINITY, sum = 0.f;
-    if constexpr (!kLong) {
-      copies_wait<kAhead>();
-      if (real) {
-        const uint4* from = slots + (i % kSlots) * (kVecs * kThreads) + t;
-#pragma unroll
-        for (int j = 0; j < kVecs; ++j)
-          raw[j] = s.v0 + t + j * kThreads < s.v1 ? from[j * kThreads] : make_uint4(Num<T>::kLow, Num<T>::kLow, Num<T>::kLow, Num<T>::kLow);
-      }
-    }
-    if (real && sums) {
-      if constexpr (kLong) {
-        for (int v = s.v0 + t; v < s.v1; v += kThreads) {
-          const uint4 u = s.xv()[v];
-          float f[kE], add = 0.f;
-          Num<T>::unpack(u, f);
-          const float top = fmaxf(m, Num<T>::largest(u)), base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-          for (int q = 0; q < kE; ++q) add += ex2((f[q] - base) * a.k);
-          sum = sum * ex2((m - base) * a.k) + add;
-          m = top;
-        }
-        join(m, sum, one, one == -INFINITY ? 0.f : ex2((one - one) * a.k), a.k);
-      } else {
-        m = one;
-#pragma unroll
-        for (int j = 0; j < kVecs; ++j) m = fmaxf(m, Num<T>::largest(raw[j]));
-        const float base = m == -INFINITY ? 0.f : m;
-        sum = ex2((one - base) * a.k);
-#pragma unroll
-        for (int j = 0; j < kVecs; ++j) {
-          float f[kE], add = 0.f;
-          Num<T>::unpack(raw[j], f);
-#pragma unroll
-          for (int q = 0; q < kE; ++q) {
-            const float v = ex2((f[q] - base) * a.k);
-            if constexpr (kMode == kPolicy) e[j * kE + q] = v;
-            add += v;
-          }
-          sum += add;
-        }
-      }
-    }
-    const float mine = m;              // reference of this thread's exponentials
-    float2* const meeting = part[i & 1];
-    if constexpr (kMode != kGrad) {
-      if (sums) {
-        join_lanes(m, sum, a.k);
-        if (lane == 0) {
-          const int at = static_cast<int>(rank) * kWarps + warp;
-          if constexpr (kCluster) {
-            for (uint32_t c = 0; c < parts; ++c)
-              asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at_rank(meeting + at, c)), "f"(m), "f"(sum) : "memory");
-          } else {
-            meeting[at] = make_float2(m, sum);
-          }
-        }
-      }
-      if constexpr (kMode == kPairs) {
-        if (t == 0 && now.grad && real) {
-          const int q = a.w.seq[row], p = q >> 1;
-          bool ok = false;
-#pragma unroll 1
-          for (uint32_t polls = 0; polls < B200_WAIT_POLLS; ++polls) {
-            if (ld_acquire_gpu(a.w.ready + p)) { ok = true; break; }
-            if ((polls & 63) == 63 && ld_acquire_gpu(&a.w.state->failed)) break;        // one wait in vain is enough
-            __nanosleep(polls > 4096 ? 256 : 32);
-          }
-          if (!ok) { atomicExch(&a.w.state->failed, 1); atomicCAS(a.status, 0, static_cast<int>(kTimeoutPair)); }
-          const float2 st = __ldcg(a.w.stat + row);
-          const float c = __ldcg(a.w.coef + q) * a.inv_t * scale;
-          bc[i & 1] = make_float4(st.x, c / st.y, c, 0.f);
-        }
-        if (rank == 0 && t == 0) {
-          ring[(i + kAhead + 2) & (kRing - 1)] = ticket;
-          if constexpr (kCluster)
-            for (uint32_t c = 1; c < parts; ++c)
-              asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(at_rank(ring + ((i + kAhead + 2) & (kRing - 1)), c)), "r"(ticket) : "memory");
-        }
-      }
-      meet<kCluster>();
-      if (sums && warp == 0 && (kMode == kPolicy || rank == 0)) {
-        m = -INFINITY;
-        sum = 0.f;
-        for (int j = lane; j < static_cast<int>(parts) * kWarps; j += 32) join(m, sum, meeting[j].x, meeting[j].y, a.k);
-        join_lanes(m, sum, a.k);
-        const double lp = real ? log_probability(xy, m, sum, a.inv_t) : 0.0;
-        if constexpr (kMode == kScores) {
+      if (before.row >= 0) {
+        const int row = before.row;
+        const bool real = before.label >= 0;
+        const Mail& letter = mail[(i - 1) & (kRing - 1)];
+        if constexpr (kMode == kGrad) {
           if (lane == 0) {
-            a.logprobs[row] = static_cast<float>(lp);
-            if (a.stat) a.stat[row] = real ? make_float2(m, sum) : make_float2(0.f, 1.f);
+            const float2 st = letter.stat;
+            const float c = real ? letter.old * a.inv_t * scale : 0.f;
+            bc[(i - 1) & 1] = make_float4(st.x, __fdividef(c, st.y), c, 0.f);
           }
-        } else if constexpr (kMode == kPairs) {
-          const int q = a.w.seq[row];
-          int last = 0;
-          if (lane == 0) {
-            a.w.lp[row] = lp;
-            a.w.stat[row] = make_float2(m, sum);
-            __threadfence();
-            if (q >= 0) last = atomicAdd(a.w.arrived + (q >> 1), 1) + 1 == a.w.cu[(q | 1) + 1] - a.w.cu[q & ~1];
-            __threadfence();
-          }
-          if (__shfl_sync(0xffffffffu, last, 0)) finish_pair(a, q >> 1);
-        } else if (lane == 0) {
-          double loss = 0.0, kl = 0.0, clipped = 0.0;
-          float coef = 0.f;
+        } else {
+          float m = -INFINITY, sum = 0.f;
           if (real) {
-            const float adv = a.policy.advantages[row];
-            const float ratio = expf(static_cast<float>(lp - a.policy.old_logprobs[row]));
-            const float held = fminf(fmaxf(ratio, a.policy.clip_low), a.policy.clip_high);
-            const bool free = !(ratio * adv > held * adv);         // NaN counts as free, so that it shows
-            coef = free ? -ratio * adv : 0.f;
-            loss = -static_cast<double>(free ? ratio : held) * adv;
-            clipped = free ? 0.0 : 1.0;
-            if (a.policy.ref_logprobs) {
-              const double d = a.policy.ref_logprobs[row] - lp;
-              const float up = expm1f(static_cast<float>(d));
-              kl = static_cast<double>(up) - d;
-              loss += a.policy.kl_coef * kl;
-              coef -= a.policy.kl_coef * up;
+            if (lane < kWarps) { m = part[(i - 1) & 1][lane].x; sum = part[(i - 1) & 1][lane].y; }
+            join_lanes(m, sum, a.k);
+          }
+          if (lane == 0) {
+            if constexpr (kMode == kScores) {
+              a.w.part[static_cast<long>(row) * a.pieces + before.piece] = make_float2(m, sum);
+            } else {
+              LogProb lp = {0.f, 0.f};
+              float c = 0.f;
+              if (real) {
+                lp = log_probability(logit_of(letter), m, sum, a.inv_t);
+                c = policy_coef(a, lp, letter.old, letter.adv, letter.ref) * a.inv_t * scale;
+              }
+              bc[(i - 1) & 1] = make_float4(m, __fdividef(c, sum), c, 0.f);
+              a.logprobs[row] = lp.hi;
+              a.w.lp[row] = lp.wide();
             }
           }
-          const float c = coef * a.inv_t * scale;
-          bc[i & 1] = make_float4(m, c / sum, c, 0.f);
-          if (rank == 0) {
-            a.logprobs[row] = static_cast<float>(lp);
-            a.policy.row_loss[row] = loss;
-            a.policy.row_loss[a.rows + static_cast<long>(row)] = kl;
-            a.policy.row_loss[2 * static_cast<long>(a.rows) + row] = clipped;
-          }
         }
       }
-      if constexpr (kMode == kPolicy) __syncthreads();
+      __syncthreads();
+      if (now.row == -1) break;
+      before = now;
     }
-    if (grads && s.g) {
-      float4 c = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (real) {
-        if constexpr (kMode == kGrad) {
-          const float2 st = a.stat[row];
-          const float w = a.weight[row] * a.inv_t;
-          c = make_float4(st.x, w / st.y, w, 0.f);
-        } else {
-          c = bc[i & 1];
-        }
-      }
-      uint4* const out = s.gv();
-      if (!real) {
-        for (int v = s.v0 + t; v < s.v1; v += kThreads) __stcs(out + v, make_uint4(0, 0, 0, 0));
-      } else if constexpr (kLong) {
-        for (int v = s.v0 + t; v < s.v1; v += kThreads) {
-          float f[kE];
-          Num<T>::unpack(s.xv()[v], f);
+    copies_wait<0>();
+    return;
+  }
+
+  // -------------------------------------------------------------------------------------------------- the elements' warps
+  const bool singles = !a.aligned || a.vocab % kE != 0;
+  const auto issue = [&](int i) {
+    const Entry n = ring[i & (kRing - 1)];
+    if (n.label >= 0) {
+      const T* x = x0 + static_cast<long>(n.row) * a.ld;
+      const Shape s = shape_of(a, x, n.piece);
+      const uint4* from = reinterpret_cast<const uint4*>(x + s.head) + s.v0 + t;
+      uint4* to = slots + (i % kSlots) * a.slot + t;
+      const int left = s.v1 - s.v0 - t;
 #pragma unroll
-          for (int q = 0; q < kE; ++q) f[q] = -c.y * ex2((f[q] - c.x) * a.k);
-          __stcs(out + v, Num<T>::pack(f));
-        }
+      for (int j = 0; j < kVecs; ++j)
+        if (j * kCompute < left) copy16(to + j * kCompute, from + j * kCompute);
+    }
+    copies_end();
+  };
+  const auto single_of = [&](int i) -> float {
+    if (!singles || warp > 0) return -INFINITY;
+    const Entry n = ring[i & (kRing - 1)];
+    if (n.label < 0) return -INFINITY;
+    const T* x = x0 + static_cast<long>(n.row) * a.ld;
+    const int e = single_at<T>(shape_of(a, x, n.piece), t, n.piece, a.pieces);
+    return e >= 0 ? Num<T>::get(x[e]) : -INFINITY;
+  };
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kLead; ++i) issue(i);
+  float one = single_of(0), one_before = -INFINITY;
+  Entry before = Entry{-1, 0, -1, 0};
+  for (int i = 0;; ++i) {
+    const Entry now = ring[i & (kRing - 1)];
+    copies_wait<kLead - 1>();
+    if (kSums && now.label >= 0) {
+      const T* const x = x0 + static_cast<long>(now.row) * a.ld;
+      const Shape s = shape_of(a, x, now.piece);
+      const int left = s.v1 - s.v0 - t;                          // vectors of this thread: j with j * kCompute < left
+      const uint4* const from = slots + (i % kSlots) * a.slot + t;
+      uint4 raw[kVecs];
+#pragma unroll
+      for (int j = 0; j < kVecs; ++j)
+        raw[j] = j * kCompute < left ? from[j * kCompute] : make_uint4(Num<T>::kLow, Num<T>::kLow, Num<T>::kLow, Num<T>::kLow);
+      float m = one;
+#pragma unroll
+      for (int j = 0; j < kVecs; ++j) m = fmaxf(m, Num<T>::largest(raw[j]));
+      m = warp_max(m);
+      const float base = m == -INFINITY ? 0.f : m;
+      float2 total[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int j = 0; j < kVecs; ++j) {
+        if (j > 0 && j * kCompute >= left) break;
+        float2 e[kE / 2];
+        exps<T>(raw[j], -base, a.k, e);
+#pragma unroll
+        for (int q = 0; q < kE / 2; ++q) total[q & 1] = add2(total[q & 1], e[q]);
+      }
+      total[0] = add2(total[0], total[1]);
+      float sum = total[0].x + total[0].y;
+      if (singles) sum += ex2((one - base) * a.k);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) part[i & 1][warp] = make_float2(m, sum);
+    }
+    __syncthreads();
+    const float next_one = single_of(i + 1);
+    if constexpr (kMode == kScores) issue(i + kLead);           // the slot's values are read
+    if (kGrads && before.row >= 0 && a.g) {
+      T* const g = g0 + static_cast<long>(before.row) * a.ld;
+      const T* const x = x0 + static_cast<long>(before.row) * a.ld;
+      const Shape s = shape_of(a, x, before.piece);
+      const int left = s.v1 - s.v0 - t;
+      uint4* const out = reinterpret_cast<uint4*>(g + s.head) + s.v0 + t;
+      const int label = before.label;
+      const bool real = label >= 0;
+      if (!real) {
+        for (int v = 0; v < left; v += kCompute) __stcs(out + v, make_uint4(0, 0, 0, 0));
+        const int e1 = single_at<T>(s, t, before.piece, a.pieces);
+        if (e1 >= 0) g[e1] = Num<T>::put(0.f);
       } else {
-        const float own = kMode == kPolicy ? -c.y * ex2((mine - c.x) * a.k) : -c.y;
+        const float4 c = bc[(i - 1) & 1];
+        const uint4* const from = slots + ((i - 1) % kSlots) * a.slot + t;
 #pragma unroll
         for (int j = 0; j < kVecs; ++j) {
-          float f[kE];
-          if constexpr (kMode == kPolicy) {
+          if (j * kCompute >= left) break;
+          float2 e[kE / 2];
+          exps<T>(from[j * kCompute], -c.x, a.k, e);
 #pragma unroll
-            for (int q = 0; q < kE; ++q) f[q] = own * e[j * kE + q];
-          } else {
-            Num<T>::unpack(raw[j], f);
-#pragma unroll
-            for (int q = 0; q < kE; ++q) f[q] = own * ex2((f[q] - c.x) * a.k);
-          }
-          if (s.v0 + t + j * kThreads < s.v1) __stcs(out + s.v0 + t + j * kThreads, Num<T>::pack(f));
+          for (int q = 0; q < kE / 2; ++q) e[q] = mul2(e[q], make_float2(-c.y, -c.y));
+          __stcs(out + j * kCompute, Num<T>::pack(e));
+        }
+        if (singles && warp == 0) {
+          const int e1 = single_at<T>(s, t, before.piece, a.pieces);
+          if (e1 >= 0) g[e1] = Num<T>::put((e1 == label ? c.z : 0.f) - c.y * ex2((one_before - c.x) * a.k));
+        }
+        const int v = (label - s.head) / kE;                    // the label's element again, by the thread that has just written its vector
+        if (label >= s.head && v >= s.v0 && v < s.v1 && (v - s.v0) % kCompute == t) {
+          const T* const held = reinterpret_cast<const T*>(slots + ((i - 1) % kSlots) * a.slot + v - s.v0);
+          g[label] = Num<T>::put(c.z - c.y * ex2((Num<T>::get(held[(label - s.head) % kE]) - c.x) * a.k));
         }
       }
-      const int e1 = s.single(rank, parts);
-      if (e1 >= 0) s.g[e1] = Num<T>::put(real ? (e1 == label ? c.z : 0.f) - c.y * ex2((one - c.x) * a.k) : 0.f);
-      if (real) {                       // the label's element again, by the thread that has just written its vector
-        const int v = label >= s.head ? (label - s.head) / kE : s.nvec;
-        if (v >= s.v0 && v < s.v1 && (v - s.v0) % kThreads == t) s.g[label] = Num<T>::put(c.z - c.y * ex2((xy - c.x) * a.k));
-      }
     }
-    label = next_label;
+    if (now.row == -1) break;
+    if constexpr (kMode != kScores) issue(i + kLead);           // into the slot of entry i - 1
+    before = now;
+    one_before = one;
     one = next_one;
   }
-  if constexpr (!kLong) copies_wait<0>();
-  if constexpr (kCluster) meet<true>();     // no block leaves while another may still write to it
+  copies_wait<0>();
 }
 
-// Offsets put in order, rows' sequences and labels, the longest pair; pairs without rows get their loss here.  One block: 8 bytes a row
-// against the kilobytes that the row has.
+// Rows that a warp holds (up to 8 vectors a lane): a warp to a row, everything in registers.  kScores, kGrad, kLocal.
+template <typename T, int kMode>
+__global__ void __launch_bounds__(256) short_rows_kernel(const __grid_constant__ Args a) {
+  constexpr int kE = Num<T>::kE;
+  const int lane = threadIdx.x & 31, row = static_cast<int>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= a.rows) return;
+  const T* const x = static_cast<const T*>(a.x) + static_cast<long>(row) * a.ld;
+  T* const g = static_cast<T*>(a.g) + static_cast<long>(row) * a.ld;
+  const Shape s = shape_of(a, x, 0);
+  const int left = s.nvec - lane, e1 = single_at<T>(s, lane, 0, 1);
+  uint4 raw[kVecs];
+#pragma unroll
+  for (int j = 0; j < kVecs; ++j)
+    raw[j] = j * 32 < left ? reinterpret_cast<const uint4*>(x + s.head)[lane + j * 32] : make_uint4(Num<T>::kLow, Num<T>::kLow, Num<T>::kLow, Num<T>::kLow);
+  const float one = e1 >= 0 ? Num<T>::get(x[e1]) : -INFINITY;
+  const int64_t y = a.w.label ? a.w.label[row] : a.labels[row];
+  const bool real = y >= 0 && y < a.vocab && (a.w.label || y != a.pad);
+  const int label = real ? static_cast<int>(y) : -1;
+  const float scale = a.scale_at ? *a.scale_at * a.scale : a.scale;
+  float old = 0.f, adv = 0.f, ref = 0.f;
+  if (kMode == kLocal && real) {
+    old = a.policy.old_logprobs[row];
+    adv = a.policy.advantages[row];
+    if (a.policy.ref_logprobs) ref = a.policy.ref_logprobs[row];
+  }
+  const float xy = real ? Num<T>::get(x[label]) : 0.f;
+  float m, sum, c = 0.f;
+  if constexpr (kMode == kGrad) {
+    const float2 st = a.stat[row];
+    m = st.x;
+    sum = st.y;
+    if (real) c = a.weight[a.w.seq ? a.w.seq[row] : row] * scale * a.inv_t;
+  } else {
+    m = one;
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) m = fmaxf(m, Num<T>::largest(raw[j]));
+    m = warp_max(m);
+    const float base = m == -INFINITY ? 0.f : m;
+    float2 total = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) {
+      if (j > 0 && j * 32 >= s.nvec) break;
+      float2 e[kE / 2];
+      exps<T>(raw[j], -base, a.k, e);
+#pragma unroll
+      for (int q = 0; q < kE / 2; ++q) total = add2(total, e[q]);
+    }
+    sum = total.x + total.y + ex2((one - base) * a.k);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    LogProb lp = {0.f, 0.f};
+    if (real) lp = log_probability(xy, m, sum, a.inv_t);
+    if constexpr (kMode == kLocal) {
+      if (real) c = policy_coef(a, lp, old, adv, ref) * a.inv_t * scale;
+      if (lane == 0) { a.logprobs[row] = lp.hi; a.w.lp[row] = lp.wide(); }
+    } else if (lane == 0) {
+      if (a.logprobs) a.logprobs[row] = lp.hi;
+      if (a.stat) a.stat[row] = real ? make_float2(m, sum) : make_float2(0.f, 1.f);
+    }
+  }
+  if (kMode == kScores || !a.g) return;
+  const float f = real ? -c / sum : 0.f;
+  uint4* const out = reinterpret_cast<uint4*>(g + s.head) + lane;
+#pragma unroll
+  for (int j = 0; j < kVecs; ++j) {
+    if (j * 32 >= left) break;
+    float2 e[kE / 2];
+    exps<T>(raw[j], -m, a.k, e);
+#pragma unroll
+    for (int q = 0; q < kE / 2; ++q) e[q] = real ? mul2(e[q], make_float2(f, f)) : make_float2(0.f, 0.f);
+    out[j * 32] = Num<T>::pack(e);
+  }
+  if (e1 >= 0) g[e1] = Num<T>::put(real ? f * ex2((one - m) * a.k) : 0.f);
+  __syncwarp();
+  if (lane == 0 && real) g[label] = Num<T>::put(c + f * ex2((xy - m) * a.k));
+}
+
+// Offsets put in order (running maximum, within the rows), rows' sequences and labels.  Every block goes through the offsets; its share of the
+// sequences it writes.
 __global__ void __launch_bounds__(1024) pairs_setup_kernel(const __grid_constant__ Args a) {
+  __shared__ int bounds[1025];
   __shared__ int warp_top[32];
-  __shared__ int carry, longest, empty;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, n = 2 * a.pairs.pairs + 1;
-  if (t == 0) { carry = 0; longest = 0; empty = 0; }
-  __syncthreads();
-  for (int base = 0; base < n; base += 1024) {                 // running maximum of the offsets
+  const auto none = [&](int begin, int end) {                // rows outside every sequence
+    for (int r = begin + static_cast<int>(blockIdx.x) * 1024 + t; r < end; r += static_cast<int>(gridDim.x) * 1024) { a.w.seq[r] = -1; a.w.label[r] = -1; }
+  };
+  if (blockIdx.x == 0 && t == 0) *a.w.state = State{0, 0};
+  int carry = 0;
+  for (int base = 0; base < n; base += 1024) {
     int v = base + t < n ? min(max(a.pairs.cu[base + t], 0), a.rows) : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) v = max(v, u); }
@@ -586,40 +618,145 @@ __global__ void __launch_bounds__(1024) pairs_setup_kernel(const __grid_constant
     __syncthreads();
     v = max(v, carry);
     for (int w = 0; w < warp; ++w) v = max(v, warp_top[w]);
-    if (base + t < n) a.w.cu[base + t] = v;
+    bounds[t + 1] = v;
+    if (t == 0) bounds[0] = carry;
+    if (blockIdx.x == 0 && base + t < n) a.w.cu[base + t] = v;
     __syncthreads();
-    if (t == 1023) carry = v;
-    __syncthreads();
-  }
-  const int first = a.w.cu[0], end = a.w.cu[n - 1];
-  for (int r = t; r < a.rows; r += 1024)
-    if (r < first || r >= end) { a.w.seq[r] = -1; a.w.label[r] = -1; }
-  for (int q = warp; q < n - 1; q += 32)
-    for (int r = a.w.cu[q] + lane; r < a.w.cu[q + 1]; r += 32) {
-      const int64_t y = a.labels[r];
-      a.w.seq[r] = q;
-      a.w.label[r] = y == a.pad || y < 0 || y >= a.vocab ? -1 : static_cast<int>(y);
+    if (base == 0) none(0, bounds[1]);
+    for (int j = warp + 32 * static_cast<int>(blockIdx.x); j < 1024; j += 32 * static_cast<int>(gridDim.x)) {
+      const int q = base + j - 1;                             // between bounds[j] and bounds[j + 1]
+      if (q < 0 || q >= n - 1) continue;
+      for (int r = bounds[j] + lane; r < bounds[j + 1]; r += 32) {
+        const int64_t y = a.labels[r];
+        a.w.seq[r] = q;
+        a.w.label[r] = y == a.pad || y < 0 || y >= a.vocab ? -1 : static_cast<int>(y);
+      }
     }
-  for (int p = t; p < a.pairs.pairs; p += 1024) {
-    const int rows = a.w.cu[2 * p + 2] - a.w.cu[2 * p];
-    a.w.arrived[p] = 0;
-    a.w.ready[p] = 0;
-    if (rows == 0) { pair_loss(a, p, 0.0, 0.0, 0, 0); atomicAdd(&empty, 1); }
-    atomicMax(&longest, rows);
+    carry = bounds[1024];
+    __syncthreads();
   }
-  __syncthreads();
-  if (t == 0) *a.w.state = PairState{0, longest, empty, a.pairs.pairs, 0};
-  if (empty == a.pairs.pairs && warp == 0) {
-    __threadfence();
-    total_loss(a);
-  }
+  none(carry, a.rows);
 }
 
-// a block for each of the sums of v[0 .. 3, 0 .. n), in one order
-__global__ void __launch_bounds__(1024) sum_rows_kernel(const double* __restrict__ v, int n, float* out0, float* out1, float* out2) {
+// A block to a pair: its rows' sums from their pieces, their log-probabilities, its loss and coefficients; the last block adds up the losses.
+template <typename T>
+__global__ void __launch_bounds__(128) pairs_kernel(const __grid_constant__ Args a) {
+  __shared__ double sums[2][4];
+  __shared__ int counts[2][4];
+  __shared__ int last;
+  const int p = static_cast<int>(blockIdx.x), t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int begin = a.w.cu[2 * p], middle = a.w.cu[2 * p + 1], end = a.w.cu[2 * p + 2];
+  double sum[2] = {0.0, 0.0};
+  int count[2] = {0, 0};
+  for (int r = begin + t; r < end; r += 128) {
+    const int label = a.w.label[r];
+    if (label < 0) continue;
+    const float xy = Num<T>::get(static_cast<const T*>(a.x)[static_cast<long>(r) * a.ld + label]);
+    float m = -INFINITY, s = 0.f;
+    if (a.pieces == 1 && a.stat) {
+      m = a.stat[r].x;
+      s = a.stat[r].y;
+    } else {
+      for (int q = 0; q < a.pieces; ++q) {
+        const float2 v = a.w.part[static_cast<long>(r) * a.pieces + q];
+        join(m, s, v.x, v.y, a.k);
+      }
+      a.w.stat[r] = make_float2(m, s);
+    }
+    const double lp = log_probability(xy, m, s, a.inv_t).wide();
+    const int which = r >= middle;
+    if (which) { sum[1] += lp; ++count[1]; } else { sum[0] += lp; ++count[0]; }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], o);
+      count[h] += __shfl_xor_sync(0xffffffffu, count[h], o);
+    }
+    if (lane == 0) { sums[h][warp] = sum[h]; counts[h][warp] = count[h]; }
+  }
+  __syncthreads();
+  if (t == 0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      sum[h] = sums[h][0] + sums[h][1] + sums[h][2] + sums[h][3];
+      count[h] = counts[h][0] + counts[h][1] + counts[h][2] + counts[h][3];
+    }
+    pair_loss(a, p, sum[0], sum[1], count[0], count[1]);
+    __threadfence();
+    last = atomicAdd(&a.w.state->pairs_done, 1) + 1 == a.pairs.pairs;
+    __threadfence();
+  }
+  __syncthreads();
+  if (!last || warp > 0) return;
+  double loss = 0.0;
+  int ranked = 0;
+  for (int i = lane; i < a.pairs.pairs; i += 32) { loss += __ldcg(a.w.loss + i); ranked += __ldcg(a.w.ranked + i); }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    loss += __shfl_xor_sync(0xffffffffu, loss, o);
+    ranked += __shfl_xor_sync(0xffffffffu, ranked, o);
+  }
+  if (lane == 0) { *a.pairs.loss = static_cast<float>(loss); *a.pairs.ranked = static_cast<float>(ranked); }
+}
+
+// After the sums of rows' pieces: log-probabilities, `stat`, and under the policy loss the coefficient; a thread to a row
+template <typename T>
+__global__ void __launch_bounds__(128) whole_rows_kernel(const __grid_constant__ Args a) {
+  const int row = static_cast<int>(blockIdx.x * 128 + threadIdx.x);
+  if (row >= a.rows) return;
+  const int64_t y = a.labels[row];
+  const bool real = y != a.pad && y >= 0 && y < a.vocab;
+  float m = -INFINITY, s = 0.f;
+  LogProb lp = {0.f, 0.f};
+  if (real) {
+    const float xy = Num<T>::get(static_cast<const T*>(a.x)[static_cast<long>(row) * a.ld + y]);
+    for (int p = 0; p < a.pieces; ++p) {
+      const float2 v = a.w.part[static_cast<long>(row) * a.pieces + p];
+      join(m, s, v.x, v.y, a.k);
+    }
+    lp = log_probability(xy, m, s, a.inv_t);
+  }
+  if (a.logprobs) a.logprobs[row] = lp.hi;
+  if (a.w.lp) a.w.lp[row] = lp.wide();
+  if (a.stat) a.stat[row] = real ? make_float2(m, s) : make_float2(0.f, 1.f);
+  if (a.policy.old_logprobs)
+    a.w.coef[row] = real ? policy_coef(a, lp, a.policy.old_logprobs[row], a.policy.advantages[row],
+                                       a.policy.ref_logprobs ? a.policy.ref_logprobs[row] : 0.f) : 0.f;
+}
+
+// The sums of the policy loss from the rows' log-probabilities, in one order: a block for the loss, the KL terms, the clipped words
+__global__ void __launch_bounds__(1024) policy_sums_kernel(const __grid_constant__ Args a) {
   __shared__ double warps[32];
   double s = 0.0;
-  for (int i = threadIdx.x; i < n; i += 1024) s += v[static_cast<long>(blockIdx.x) * n + i];
+  for (int r0 = threadIdx.x; r0 < a.rows; r0 += 8 * 1024) {
+    int64_t y[8];
+    double lp[8];
+    float adv[8], old[8], ref[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {                              // several rows' numbers are asked for at a time
+      const int r = r0 + j * 1024;
+      const bool in = r < a.rows;
+      y[j] = in ? a.labels[r] : -1;
+      lp[j] = in ? a.w.lp[r] : 0.0;
+      adv[j] = in ? a.policy.advantages[r] : 0.f;
+      old[j] = in ? a.policy.old_logprobs[r] : 0.f;
+      ref[j] = in && a.policy.ref_logprobs ? a.policy.ref_logprobs[r] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (y[j] == a.pad || y[j] < 0 || y[j] >= a.vocab) continue;
+      const float ratio = expf(static_cast<float>(lp[j] - old[j])), held = fminf(fmaxf(ratio, a.policy.clip_low), a.policy.clip_high);
+      const bool free = !(ratio * adv[j] > held * adv[j]);
+      double kl = 0.0;
+      if (blockIdx.x < 2 && a.policy.ref_logprobs) {
+        const double d = ref[j] - lp[j];
+        kl = static_cast<double>(expm1f(static_cast<float>(d))) - d;
+      }
+      s += blockIdx.x == 0 ? a.policy.kl_coef * kl - static_cast<double>(free ? ratio : held) * adv[j] : blockIdx.x == 1 ? kl : free ? 0.0 : 1.0;
+    }
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = s;
@@ -628,7 +765,7 @@ __global__ void __launch_bounds__(1024) sum_rows_kernel(const double* __restrict
     s = warps[threadIdx.x];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (threadIdx.x == 0) *(blockIdx.x == 0 ? out0 : blockIdx.x == 1 ? out1 : out2) = static_cast<float>(s);
+    if (threadIdx.x == 0) *(blockIdx.x == 0 ? a.policy.loss : blockIdx.x == 1 ? a.policy.kl : a.policy.clipped) = static_cast<float>(s);
   }
 }
 
@@ -638,80 +775,105 @@ __global__ void __launch_bounds__(256) scale_rows_kernel(const Args a, const flo
   const float f = *factor;
   if (f == 1.f) return;
   for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    const Span<T> s(a, r, 0, 1);
+    T* const row = static_cast<T*>(a.g) + static_cast<long>(r) * a.ld;
+    const Shape s = shape_of(a, row, 0);
+    uint4* const vectors = reinterpret_cast<uint4*>(row + s.head);
     for (int v = threadIdx.x; v < s.nvec; v += 256) {
-      float g[kE];
-      Num<T>::unpack(s.gv()[v], g);
+      float2 g[kE / 2];
+      Num<T>::unpack(vectors[v], g);
 #pragma unroll
-      for (int q = 0; q < kE; ++q) g[q] *= f;
-      s.gv()[v] = Num<T>::pack(g);
+      for (int q = 0; q < kE / 2; ++q) g[q] = mul2(g[q], make_float2(f, f));
+      vectors[v] = Num<T>::pack(g);
     }
-    const int one = s.single(0, 1);
-    if (one >= 0) s.g[one] = Num<T>::put(Num<T>::get(s.g[one]) * f);
+    const int one = single_at<T>(s, threadIdx.x, 0, 1);
+    if (one >= 0) row[one] = Num<T>::put(Num<T>::get(row[one]) * f);
   }
 }
 
 const char* problem(cudaError_t e) { return e == cudaSuccess ? nullptr : cudaGetErrorString(e); }
 
-template <typename T, int kThreads, int kMode, bool kCluster, bool kLong>
-const char* launch_rows(Args a, int parts, long items, cudaStream_t stream) {
-  auto kernel = rows_kernel<T, kThreads, kMode, kCluster, kLong>;
-  const size_t smem = kLong ? 0 : static_cast<size_t>(kSlots) * kVecs * kThreads * 16;
-  // how many groups of blocks the GPU holds; all GPUs of a machine are alike
-  static int groups[kMaxCluster + 1] = {};
-  cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(parts);
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = kCluster ? 1 : 0;
+template <typename T, int kCompute, int kMode>
+const char* launch_rows(const Args& from, cudaStream_t stream) {
+  Args a = from;
+  auto kernel = rows_kernel<T, kCompute, kMode>;
+  // slots as long as a piece: shorter rows leave room for a third block
+  const int across = (a.each < kVecs * kCompute ? (a.each + kCompute - 1) / kCompute * kCompute : kVecs * kCompute);
+  const int smem = kSlots * across * 16;
+  a.slot = across;
   // the attribute belongs to a device's context: set at every call, which costs less than keeping account of the devices
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSlots * kVecs * kCompute * 16);
   if (e != cudaSuccess) return cudaGetErrorString(e);
-  int held = groups[parts];
+  static int blocks[kVecs + 1] = {};    // that an SM holds; all GPUs of a machine are alike
+  int& held = blocks[across / kCompute];
   if (held == 0) {
-    if (kCluster) {
-      cfg.gridDim = dim3(parts);
-      e = cudaOccupancyMaxActiveClusters(&held, kernel, &cfg);
-    } else {
-      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kernel, kThreads, smem);
-      held *= num_sms();
-    }
+    int n = 0;
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kCompute + 32, smem);
     if (e != cudaSuccess) return cudaGetErrorString(e);
-    if (held < 1) return "preference: no block of this shape fits the GPU";
-    groups[parts] = held;
+    if (n < 1) return "preference: no block fits an SM";
+    held = n;
   }
-  const long g = items < held ? items : held;
-  a.slack = 2 * held;
-  cfg.gridDim = dim3(static_cast<unsigned>(g * parts));
-  e = cudaLaunchKernelEx(&cfg, kernel, a);
-  return problem(e);
+  const long items = static_cast<long>(a.rows) * a.pieces, most = static_cast<long>(held) * num_sms();
+  if (4 * items + (1L << 20) >= 1L << 31) return "preference: too many rows";
+  const int grid = static_cast<int>(items < most ? items : most);
+  if (items <= most) {
+    a.w.state = nullptr;
+  } else {
+    e = cudaMemsetAsync(a.w.state, 0, sizeof(State), stream);
+    if (e != cudaSuccess) return cudaGetErrorString(e);
+  }
+  kernel<<<grid, kCompute + 32, smem, stream>>>(a);
+  return problem(cudaGetLastError());
+}
+
+template <typename T> constexpr int warp_row() { return 32 * kVecs * Num<T>::kE; }       // elements that a warp holds
+
+// Pieces of a row: as many as hold it; for few rows more, of 4 KB at least, until every block that the GPU holds has one.
+#ifndef NMTG_PIECE
+#define NMTG_PIECE 8
+#endif
+int pieces_of(int rows, int vocab, int dtype) {
+  const int vectors = vocab / (dtype == 0 ? 4 : 8);
+  int n = (vectors + kBlock * NMTG_PIECE - 1) / (kBlock * NMTG_PIECE);
+  if (n < 1) n = 1;
+  while (2L * n * rows <= 2 * num_sms() && vectors >= 512 * n) n *= 2;
+  return n;
 }
 
 template <typename T, int kMode>
-const char* launch_mode(const Args& a, long items, cudaStream_t stream) {
-  constexpr int kEach = kVecs * Num<T>::kE;                 // elements of a thread
-  if (a.vocab <= 32 * kEach) return launch_rows<T, 32, kMode, false, false>(a, 1, items, stream);
-  if (a.vocab <= 128 * kEach) return launch_rows<T, 128, kMode, false, false>(a, 1, items, stream);
-  if (a.vocab <= 256 * kEach) return launch_rows<T, 256, kMode, false, false>(a, 1, items, stream);
-  if (a.vocab <= 512 * kEach) return launch_rows<T, 512, kMode, false, false>(a, 1, items, stream);
-  if (a.vocab <= 1024 * kEach) return launch_rows<T, 1024, kMode, false, false>(a, 1, items, stream);
-  for (int parts = 2; parts <= kMaxCluster; parts *= 2)
-    if (a.vocab <= parts * 1024 * kEach) return launch_rows<T, 1024, kMode, true, false>(a, parts, items, stream);
-  return launch_rows<T, 1024, kMode, true, true>(a, kMaxCluster, items, stream);
+const char* launch_short(const Args& a, cudaStream_t stream) {
+  short_rows_kernel<T, kMode><<<(a.rows + 7) / 8, 256, 0, stream>>>(a);
+  return problem(cudaGetLastError());
 }
 
+// kMode: kScores or kGrad
 template <int kMode>
-const char* launch_type(const Args& a, int dtype, long items, cudaStream_t stream) {
+const char* launch_pass(Args a, int dtype, cudaStream_t stream) {
   if (a.rows <= 0) return nullptr;
-  if (dtype == 0) return launch_mode<float, kMode>(a, items, stream);
-  if (dtype == 1) return launch_mode<__nv_bfloat16, kMode>(a, items, stream);
-  if (dtype == 2) return launch_mode<__half, kMode>(a, items, stream);
-  return "preference: logits must be fp32, bf16 or fp16";
+  const int size = dtype == 0 ? 4 : 2;
+  if (a.vocab <= (dtype == 0 ? warp_row<float>() : warp_row<__half>())) {
+    a.pieces = 1;
+    a.each = a.vocab / (16 / size);
+    return dtype == 0 ? launch_short<float, kMode>(a, stream) : dtype == 1 ? launch_short<__nv_bfloat16, kMode>(a, stream) : launch_short<__half, kMode>(a, stream);
+  }
+  a.pieces = pieces_of(a.rows, a.vocab, dtype);
+  a.each = (a.vocab / (16 / size) + a.pieces - 1) / a.pieces;
+  const char* err = dtype == 0 ? launch_rows<float, kBlock, kMode>(a, stream) : dtype == 1 ? launch_rows<__nv_bfloat16, kBlock, kMode>(a, stream)
+                                                                                          : launch_rows<__half, kBlock, kMode>(a, stream);
+  if (kMode != kScores || err || a.pairs.pairs > 0) return err;
+  const int blocks = (a.rows + 127) / 128;
+  if (dtype == 0) whole_rows_kernel<float><<<blocks, 128, 0, stream>>>(a);
+  else if (dtype == 1) whole_rows_kernel<__nv_bfloat16><<<blocks, 128, 0, stream>>>(a);
+  else whole_rows_kernel<__half><<<blocks, 128, 0, stream>>>(a);
+  return problem(cudaGetLastError());
+}
+
+template <typename T>
+const char* launch_local(Args a, cudaStream_t stream) {
+  a.pieces = 1;
+  a.each = a.vocab / Num<T>::kE;
+  if (a.vocab <= warp_row<T>()) return launch_short<T, kLocal>(a, stream);
+  if (a.vocab <= kBlock * kVecs * Num<T>::kE) return launch_rows<T, kBlock, kLocal>(a, stream);
+  return launch_rows<T, kWide, kLocal>(a, stream);
 }
 
 Args row_args(const NmtgRows* r) {
@@ -719,68 +881,136 @@ Args row_args(const NmtgRows* r) {
   a.x = r->logits; a.g = r->grad; a.labels = r->labels; a.ld = r->ld; a.pad = r->pad; a.rows = r->rows; a.vocab = r->vocab;
   a.inv_t = r->inv_temperature; a.k = static_cast<float>(1.4426950408889634074 * r->inv_temperature);
   a.scale_at = r->grad_scale_at; a.scale = r->grad_scale;
-  a.logprobs = r->logprobs; a.stat = r->stat; a.status = r->status;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(r->logits ? r->logits : r->grad);
+  a.aligned = at % 16 == 0 && (r->rows <= 1 || r->ld * (r->dtype == 0 ? 4 : 2) % 16 == 0);
+  a.logprobs = r->logprobs; a.stat = r->stat;
+  a.pieces = 1;
+  a.each = a.vocab;
   return a;
 }
 
 long up16(long n) { return (n + 15) & ~15L; }
+const char* bad_type = "preference: logits must be fp32, bf16 or fp16";
+
+// The workspace of a call; null pointers where it is not asked for
+Work workspace(char* at, long rows, long pairs, long pieces, long* bytes) {
+  char* const begin = at;
+  const auto take = [&](long n) { char* here = at; at += up16(n); return static_cast<void*>(here); };
+  Work w = {};
+  w.state = static_cast<State*>(take(sizeof(State)));
+  w.part = static_cast<float2*>(take(8 * rows * pieces));
+  w.stat = static_cast<float2*>(take(8 * rows));
+  w.coef = static_cast<float*>(take(4 * (2 * pairs > rows ? 2 * pairs : rows)));
+  w.cu = static_cast<int*>(take(4 * (2 * pairs + 1)));
+  w.seq = static_cast<int*>(take(4 * rows));
+  w.label = static_cast<int*>(take(4 * rows));
+  w.lp = static_cast<double*>(take(8 * rows));
+  w.loss = static_cast<double*>(take(8 * pairs));
+  w.ranked = static_cast<int*>(take(4 * pairs));
+  *bytes = at - begin;
+  return w;
+}
 
 }  // namespace
 }  // namespace b200
 
 using namespace b200;
 
+long nmtg_rows_workspace(int rows, int vocab, int dtype, int pairs) {
+  long bytes = 0;
+  workspace(nullptr, rows, pairs, pieces_of(rows, vocab, dtype), &bytes);
+  return bytes;
+}
+
 const char* nmtg_row_scores(const NmtgRows* r, cudaStream_t stream) {
-  return launch_type<kScores>(row_args(r), r->dtype, r->rows, stream);
+  if (r->dtype < 0 || r->dtype > 2) return bad_type;
+  Args a = row_args(r);
+  long bytes;
+  const Work w = workspace(static_cast<char*>(r->workspace), r->rows, 0, pieces_of(r->rows, r->vocab, r->dtype), &bytes);
+  a.w.state = w.state;
+  a.w.part = w.part;
+  return launch_pass<kScores>(a, r->dtype, stream);
 }
 
 const char* nmtg_row_scores_grad(const NmtgRows* r, const float* weight, cudaStream_t stream) {
+  if (r->dtype < 0 || r->dtype > 2) return bad_type;
   Args a = row_args(r);
   a.weight = weight;
-  return launch_type<kGrad>(a, r->dtype, r->rows, stream);
+  a.scale = 1.f;
+  long bytes;
+  a.w.state = workspace(static_cast<char*>(r->workspace), r->rows, 0, 1, &bytes).state;
+  return launch_pass<kGrad>(a, r->dtype, stream);
 }
 
 const char* nmtg_policy_loss(const NmtgRows* r, const NmtgPolicy* p, cudaStream_t stream) {
+  if (r->dtype < 0 || r->dtype > 2) return bad_type;
   Args a = row_args(r);
   a.policy = *p;
-  const char* err = launch_type<kPolicy>(a, r->dtype, r->rows, stream);
+  const int size = r->dtype == 0 ? 4 : 2;
+  const char* err = nullptr;
+  long bytes;
+  const Work w = workspace(static_cast<char*>(r->workspace), r->rows, 0, pieces_of(r->rows, r->vocab, r->dtype), &bytes);
+  a.w.lp = w.lp;
+  a.w.state = w.state;
+  if (r->rows <= 0) {
+  } else if (r->vocab <= kWide * kVecs * (16 / size)) {
+    err = r->dtype == 0 ? launch_local<float>(a, stream) : r->dtype == 1 ? launch_local<__nv_bfloat16>(a, stream) : launch_local<__half>(a, stream);
+  } else {
+    a.w.part = w.part;
+    a.w.coef = w.coef;
+    a.weight = w.coef;
+    a.stat = w.stat;
+    err = launch_pass<kScores>(a, r->dtype, stream);
+    if (!err && a.g) err = launch_pass<kGrad>(a, r->dtype, stream);
+  }
   if (err) return err;
-  sum_rows_kernel<<<3, 1024, 0, stream>>>(p->row_loss, r->rows, p->loss, p->kl, p->clipped);
+  policy_sums_kernel<<<3, 1024, 0, stream>>>(a);
   return problem(cudaGetLastError());
 }
 
-long nmtg_pairs_workspace(int rows, int pairs) {
-  const long r = rows, p = pairs;
-  return up16(sizeof(PairState)) + up16(4 * (2 * p + 1)) + 2 * up16(4 * r) + 3 * up16(4 * p) + up16(8 * p) + up16(8 * r) + up16(8 * p) + up16(8 * r);
-}
-
 const char* nmtg_preference_loss(const NmtgRows* r, const NmtgPairs* p, cudaStream_t stream) {
+  if (r->dtype < 0 || r->dtype > 2) return bad_type;
   Args a = row_args(r);
   a.pairs = *p;
-  char* at = static_cast<char*>(p->workspace);
-  const auto take = [&](long bytes) { char* here = at; at += up16(bytes); return static_cast<void*>(here); };
-  const long rows = r->rows, pairs = p->pairs;
-  a.w.state = static_cast<PairState*>(take(sizeof(PairState)));
-  a.w.cu = static_cast<int*>(take(4 * (2 * pairs + 1)));
-  a.w.seq = static_cast<int*>(take(4 * rows));
-  a.w.label = static_cast<int*>(take(4 * rows));
-  a.w.arrived = static_cast<int*>(take(4 * pairs));
-  a.w.ready = static_cast<int*>(take(4 * pairs));
-  a.w.ranked = static_cast<int*>(take(4 * pairs));
-  a.w.coef = static_cast<float*>(take(8 * pairs));
-  a.w.lp = static_cast<double*>(take(8 * rows));
-  a.w.loss = static_cast<double*>(take(8 * pairs));
-  a.w.stat = static_cast<float2*>(take(8 * rows));
-  pairs_setup_kernel<<<1, 1024, 0, stream>>>(a);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return cudaGetErrorString(e);
-  return launch_type<kPairs>(a, r->dtype, (r->grad ? 2L : 1L) * rows, stream);
+  long bytes;
+  const int pieces = pieces_of(r->rows, r->vocab, r->dtype);
+  const Work w = workspace(static_cast<char*>(r->workspace), r->rows, p->pairs, pieces, &bytes);
+  if (p->pairs == 0) {                    // no loss; every row is outside
+    cudaError_t e = cudaMemsetAsync(p->loss, 0, sizeof(float), stream);
+    if (e == cudaSuccess) e = cudaMemsetAsync(p->ranked, 0, sizeof(float), stream);
+    if (e != cudaSuccess) return cudaGetErrorString(e);
+  }
+  a.w = w;
+  const int share = 1 + (p->pairs >= 8) * (p->pairs < 256 ? p->pairs / 8 : 32);
+  pairs_setup_kernel<<<share, 1024, 0, stream>>>(a);
+  const char* err = problem(cudaGetLastError());
+  if (err) return err;
+  const bool is_short = r->vocab <= (r->dtype == 0 ? warp_row<float>() : warp_row<__half>());
+  if (p->pairs > 0) {
+    Args scores = a;
+    scores.w.label = scores.w.seq = nullptr;
+    scores.stat = is_short ? w.stat : nullptr;
+    err = launch_pass<kScores>(scores, r->dtype, stream);
+    if (err) return err;
+    scores = a;
+    scores.pieces = is_short ? 1 : pieces;
+    scores.stat = is_short ? w.stat : nullptr;
+    if (r->dtype == 0) pairs_kernel<float><<<p->pairs, 128, 0, stream>>>(scores);
+    else if (r->dtype == 1) pairs_kernel<__nv_bfloat16><<<p->pairs, 128, 0, stream>>>(scores);
+    else pairs_kernel<__half><<<p->pairs, 128, 0, stream>>>(scores);
+    err = problem(cudaGetLastError());
+    if (err) return err;
+  }
+  if (!a.g) return nullptr;
+  a.weight = w.coef;
+  a.stat = w.stat;
+  return launch_pass<kGrad>(a, r->dtype, stream);
 }
 
 const char* nmtg_scale_rows(const NmtgRows* r, const float* factor, cudaStream_t stream) {
   if (r->rows <= 0 || r->vocab <= 0) return nullptr;
-  Args a = row_args(r);
-  a.x = a.g;
+  if (r->dtype < 0 || r->dtype > 2) return bad_type;
+  const Args a = row_args(r);
   const int grid = r->rows < 8 * num_sms() ? r->rows : 8 * num_sms();
   if (r->dtype == 0) scale_rows_kernel<float><<<grid, 256, 0, stream>>>(a, factor);
   else if (r->dtype == 1) scale_rows_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(a, factor);

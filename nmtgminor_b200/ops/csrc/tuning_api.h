@@ -23,8 +23,9 @@ struct NmtgRows {
   const float* grad_scale_at;
   float* logprobs;          // [rows] out
   float2* stat;             // [rows] (largest logit, sum of exp((x - largest) / T)): out of the scores, in of their gradient
-  int* status;
+  void* workspace;          // nmtg_rows_workspace bytes (pairs: of the paired loss, otherwise 0), 16-byte aligned
 };
+long nmtg_rows_workspace(int rows, int vocab, int dtype, int pairs);
 // log-probability of every label, and `stat` where it is not null
 const char* nmtg_row_scores(const NmtgRows* r, cudaStream_t stream);
 // grad = weight[row] * d logprob / d logits, from `stat`
@@ -35,7 +36,6 @@ struct NmtgPolicy {
   const float* advantages;     // [rows]
   const float* ref_logprobs;   // [rows] or null
   float clip_low, clip_high, kl_coef;
-  double* row_loss;            // [3, rows] scratch: loss, KL, 1 where the ratio was clipped
   float *loss, *kl, *clipped;  // [1] each, out: sums of losses and KL terms, number of clipped words
 };
 const char* nmtg_policy_loss(const NmtgRows* r, const NmtgPolicy* p, cudaStream_t stream);
@@ -50,9 +50,7 @@ struct NmtgPairs {
   float beta, smoothing, margin, nll_weight;
   float* seq_logprobs;         // [2 pairs] out
   float *loss, *ranked;        // [1] each, out: sum of losses, number of pairs ranked as preferred
-  void* workspace;             // nmtg_pairs_workspace bytes, 16-byte aligned
 };
-long nmtg_pairs_workspace(int rows, int pairs);
 const char* nmtg_preference_loss(const NmtgRows* r, const NmtgPairs* p, cudaStream_t stream);
 // r->grad *= *factor, unless it is 1
 const char* nmtg_scale_rows(const NmtgRows* r, const float* factor, cudaStream_t stream);
