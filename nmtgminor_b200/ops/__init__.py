@@ -723,24 +723,6 @@ class _EmbedFn(torch.autograd.Function):
         return (None,) * 13
 
 
-class _EmbedSortedFn(torch.autograd.Function):
-    """``table[tokens] * scale`` of an ordinary CUDA tensor; its gradient is written whole, in the table's type."""
-
-    @staticmethod
-    def forward(ctx, table, tokens, scale, pad_idx):
-        ctx.save_for_backward(tokens)
-        ctx.cfg = (scale, pad_idx, table.shape)
-        LAUNCHES[0] += 1
-        return ext().embed_rows(tokens, table, scale)
-
-    @staticmethod
-    def backward(ctx, dy):
-        (tokens,) = ctx.saved_tensors
-        scale, pad_idx, shape = ctx.cfg
-        LAUNCHES[0] += 3
-        return ext().embed_grad(tokens, None, dy.contiguous(), None, shape[0], shape[0], scale, 0.0, 0, 0, pad_idx), None, None, None
-
-
 _dummy = {}
 
 
@@ -790,13 +772,14 @@ def _embedding_sorted(tokens, table, positions, pos_table, scale, p, pad_idx):
         raise ValueError("embedding: tokens are on %s, the table on %s" % (tokens.device, table.device))
     on_gpu = table.is_cuda and table.dtype in (torch.bfloat16, torch.float16, torch.float32)
     if on_gpu:
-        out = _EmbedSortedFn.apply(table.contiguous(), tokens.contiguous(), scale, pad_idx)
+        LAUNCHES[0] += 4
+        out = ext().embed_rows_node(table.contiguous(), tokens.contiguous(), scale, pad_idx)
     else:
         out = F.embedding(tokens, table, padding_idx=pad_idx if 0 <= pad_idx < table.shape[0] else None) * scale
     if pos_table is not None:
         pos = (positions if positions is not None else torch.zeros_like(tokens)).clamp(0, pos_table.shape[0] - 1)
         on_gpu = pos_table.is_cuda and pos_table.dtype in (torch.bfloat16, torch.float16, torch.float32)
-        rows = _EmbedSortedFn.apply(pos_table.contiguous(), pos.contiguous(), 1.0, -1) if on_gpu else F.embedding(pos, pos_table)
+        rows = ext().embed_rows_node(pos_table.contiguous(), pos.contiguous(), 1.0, -1) if on_gpu else F.embedding(pos, pos_table)
         out = out + rows.to(out.dtype)
     return F.dropout(out, p, True) if p > 0 else out
 

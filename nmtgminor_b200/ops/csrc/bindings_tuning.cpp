@@ -335,6 +335,111 @@ Tensor kept_backward(const Tensor& dy, const Tensor& codes, const Tensor& scales
   return dz;
 }
 
+// ---- autograd nodes ------------------------------------------------------------------------------------------------------
+// In C++, because a node in Python costs about as much as the kernels of a small call (forward and backward pass of an empty one 57 us).
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::variable_list;
+
+Tensor plain_rows(const Tensor& t) {
+  const bool rows = t.dim() != 2 || (t.stride(1) == 1 && (t.size(0) <= 1 || t.stride(0) >= t.size(1)));
+  return rows ? t : t.contiguous();
+}
+
+struct ScoresNode : Function<ScoresNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, int64_t pad, double temperature) {
+    auto [lp, stat] = row_scores(logits, labels, pad, temperature, true);
+    ctx->save_for_backward({logits, labels, stat});
+    ctx->saved_data["pad"] = pad;
+    ctx->saved_data["temperature"] = temperature;
+    return lp;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor weight = g[0].to(at::kFloat).contiguous();
+    return {row_scores_grad(saved[0], saved[1], saved[2], weight, ctx->saved_data["pad"].toInt(), ctx->saved_data["temperature"].toDouble()),
+            Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// The two losses: the gradient is made with the loss and belongs to the first backward pass
+variable_list loss_backward(AutogradContext* ctx, const variable_list& g, size_t inputs) {
+  variable_list out(inputs);
+  if (!g[0].defined()) return out;
+  TORCH_CHECK(!ctx->saved_data["grad"].isNone(), "a second backward pass through a preference or policy loss: its gradient went to the first one");
+  Tensor grad = ctx->saved_data["grad"].toTensor();
+  ctx->saved_data["grad"] = c10::IValue();
+  if (!ctx->saved_data["prescaled"].toBool()) scale_rows(grad, g[0].to(at::kFloat).contiguous());
+  out[0] = grad;
+  return out;
+}
+void loss_forward(AutogradContext* ctx, const Tensor& logits, const OptTensor& grad, bool inplace, bool prescaled, const variable_list& plain) {
+  ctx->saved_data["grad"] = *grad;
+  ctx->saved_data["prescaled"] = prescaled;
+  ctx->mark_non_differentiable(plain);
+  ctx->set_materialize_grads(false);
+  if (inplace) logits.unsafeGetTensorImpl()->bump_version();      // what another node has saved of the logits is gone
+}
+
+struct PolicyNode : Function<PolicyNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, const Tensor& old_logprobs, const Tensor& advantages,
+                               const OptTensor& ref, double clip_low, double clip_high, double kl_coef, int64_t pad, double temperature, bool inplace,
+                               const OptTensor& scale_at, double scale, bool prescaled) {
+    auto [loss, clipped, kl, lp, grad] = policy_loss(logits, labels, old_logprobs, advantages, ref, clip_low, clip_high, kl_coef, pad, temperature,
+                                                     inplace ? 2 : 1, scale_at, scale);
+    loss_forward(ctx, logits, grad, inplace, prescaled, {clipped, kl, lp});
+    return {loss, clipped, kl, lp};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) { return loss_backward(ctx, g, 14); }
+};
+
+struct PreferenceNode : Function<PreferenceNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, const Tensor& cu, const OptTensor& ref, int64_t kind,
+                               double beta, double smoothing, double margin, double nll_weight, bool average, int64_t pad, double temperature,
+                               bool inplace, const OptTensor& scale_at, double scale, bool prescaled) {
+    auto [loss, ranked, seq, grad] = preference_loss(logits, labels, cu, ref, kind, beta, smoothing, margin, nll_weight, average, pad, temperature,
+                                                     inplace ? 2 : 1, scale_at, scale);
+    loss_forward(ctx, logits, grad, inplace, prescaled, {ranked, seq});
+    return {loss, ranked, seq};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) { return loss_backward(ctx, g, 16); }
+};
+
+struct EmbedNode : Function<EmbedNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& table, const Tensor& tokens, double scale, int64_t pad) {
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["pad"] = pad;
+    ctx->saved_data["words"] = table.size(0);
+    return embed_rows(tokens, table, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    const int64_t words = ctx->saved_data["words"].toInt();
+    return {embed_grad(saved[0], OptTensor(), g[0].contiguous(), OptTensor(), words, words, ctx->saved_data["scale"].toDouble(), 0.0, 0, 0,
+                       ctx->saved_data["pad"].toInt()),
+            Tensor(), Tensor(), Tensor()};
+  }
+};
+
+struct ActivationNode : Function<ActivationNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& z, int64_t act, double p, int64_t seed, int64_t stream_id) {
+    auto [y, codes, scales] = kept_forward(z, act, true, p, seed, stream_id);
+    ctx->save_for_backward({*codes, *scales});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["seed"] = seed;
+    ctx->saved_data["stream"] = stream_id;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    return {kept_backward(plain_rows(g[0]), saved[0], saved[1], ctx->saved_data["act"].toInt(), ctx->saved_data["p"].toDouble(),
+                          ctx->saved_data["seed"].toInt(), ctx->saved_data["stream"].toInt()),
+            Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
 }  // namespace
 
 void bind_tuning_ops(pybind11::module& m) {
@@ -343,6 +448,29 @@ void bind_tuning_ops(pybind11::module& m) {
   m.def("policy_loss", &policy_loss);
   m.def("preference_loss", &preference_loss);
   m.def("scale_rows", &scale_rows);
+  m.def("row_scores_node", [](const Tensor& logits, const Tensor& labels, int64_t pad, double temperature) {
+    return ScoresNode::apply(logits, labels, pad, temperature);
+  });
+  m.def("policy_loss_node", [](const Tensor& logits, const Tensor& labels, const Tensor& old_logprobs, const Tensor& advantages, const OptTensor& ref,
+                               double clip_low, double clip_high, double kl_coef, int64_t pad, double temperature, bool inplace,
+                               const OptTensor& scale_at, double scale, bool prescaled) {
+    auto o = PolicyNode::apply(logits, labels, old_logprobs, advantages, ref, clip_low, clip_high, kl_coef, pad, temperature, inplace, scale_at, scale,
+                               prescaled);
+    return std::make_tuple(o[0], o[1], o[2], o[3]);
+  });
+  m.def("preference_loss_node", [](const Tensor& logits, const Tensor& labels, const Tensor& cu, const OptTensor& ref, int64_t kind, double beta,
+                                   double smoothing, double margin, double nll_weight, bool average, int64_t pad, double temperature, bool inplace,
+                                   const OptTensor& scale_at, double scale, bool prescaled) {
+    auto o = PreferenceNode::apply(logits, labels, cu, ref, kind, beta, smoothing, margin, nll_weight, average, pad, temperature, inplace, scale_at,
+                                   scale, prescaled);
+    return std::make_tuple(o[0], o[1], o[2]);
+  });
+  m.def("embed_rows_node", [](const Tensor& table, const Tensor& tokens, double scale, int64_t pad) {
+    return EmbedNode::apply(table, tokens, scale, pad);
+  });
+  m.def("activation_node", [](const Tensor& z, int64_t act, double p, int64_t seed, int64_t stream_id) {
+    return ActivationNode::apply(z, act, p, seed, stream_id);
+  });
   m.def("embed_rows", &embed_rows);
   m.def("embed_grad", &embed_grad);
   m.def("kept_quantise", &kept_quantise);

@@ -132,20 +132,6 @@ def restore_activated(kept: Kept, act_id: int, p: float, seed: int, stream_id: i
 # ---------------------------------------------------------------------------------------------------
 # activation
 # ---------------------------------------------------------------------------------------------------
-class _ActivationFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, z, act, p, seed, sid):
-        y, codes, scales = _ext().kept_forward(z, act, True, p, seed, sid)
-        ctx.save_for_backward(codes, scales)
-        ctx.cfg = (act, p, seed, sid)
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        codes, scales = ctx.saved_tensors
-        return (_ext().kept_backward(_rows(dy), codes, scales, *ctx.cfg),) + (None,) * 4
-
-
 def activation(z, act="gelu", dropout_p: float = 0.0, training: bool = True):
     """``dropout(act(z))`` of a matrix whose backward pass takes the slope at the kept ``z``; nothing is kept where no gradient is asked for.
     ``act``: "none", "relu", "gelu" (erf) or "silu"."""
@@ -163,5 +149,5 @@ def activation(z, act="gelu", dropout_p: float = 0.0, training: bool = True):
     sid = next_stream() if p > 0 else 0
     x = _rows(z)
     if torch.is_grad_enabled() and z.requires_grad:
-        return _ActivationFn.apply(x, act_id, p, _Rng.seed, sid)
+        return _ext(2).activation_node(x, act_id, p, _Rng.seed, sid)
     return _ext().kept_forward(x, act_id, False, p, _Rng.seed, sid)[0]

@@ -130,22 +130,6 @@ def _scale_args(grad_scale, logits):
 # ---------------------------------------------------------------------------------------------------
 # log-probabilities
 # ---------------------------------------------------------------------------------------------------
-class _TokenLogprobsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, pad_idx, temperature):
-        lp, stat = ext().row_scores(logits, labels, pad_idx, temperature, True)
-        LAUNCHES[0] += 1
-        ctx.save_for_backward(logits, labels, stat)
-        ctx.cfg = (pad_idx, temperature)
-        return lp
-
-    @staticmethod
-    def backward(ctx, g):
-        logits, labels, stat = ctx.saved_tensors
-        LAUNCHES[0] += 1
-        return ext().row_scores_grad(logits, labels, stat, g.float().contiguous(), *ctx.cfg), None, None, None
-
-
 def token_logprobs(logits, labels, pad_idx: int = 0, temperature: float = 1.0):
     """Log-probability of every label under ``softmax(logits / temperature)``: fp32 ``[rows]``, 0 in rows of padding.  Differentiable with
     respect to the logits (any objective over the log-probabilities of words: minimum risk, sequence-level rewards); without gradients one
@@ -154,9 +138,9 @@ def token_logprobs(logits, labels, pad_idx: int = 0, temperature: float = 1.0):
     if not _kernel_takes(logits):
         return token_logprobs_reference(logits, labels.long(), pad_idx, temperature)
     x, y = _as_rows(logits), labels.long().contiguous()
+    LAUNCHES[0] += 2
     if torch.is_grad_enabled() and logits.requires_grad:
-        return _TokenLogprobsFn.apply(x, y, int(pad_idx), float(temperature))
-    LAUNCHES[0] += 1
+        return ext().row_scores_node(x, y, int(pad_idx), float(temperature))
     return ext().row_scores(x, y, int(pad_idx), float(temperature), False)[0]
 
 
@@ -170,39 +154,6 @@ def sequence_logprobs(logprobs, cu):
 # ---------------------------------------------------------------------------------------------------
 # losses
 # ---------------------------------------------------------------------------------------------------
-class _LossFn(torch.autograd.Function):
-    """``call(grad)`` runs the kernel and returns (loss, ..., gradient); the gradient waits for the backward pass."""
-
-    @staticmethod
-    def forward(ctx, logits, call, inplace, prescaled):
-        out = call(2 if inplace else 1)
-        ctx.grad, ctx.prescaled = out[-1], prescaled
-        ctx.mark_non_differentiable(*out[1:-1])
-        ctx.set_materialize_grads(False)
-        if inplace:
-            torch.autograd.graph.increment_version(logits)    # what another node has saved of the logits is gone
-        return out[:-1]
-
-    @staticmethod
-    def backward(ctx, g_loss, *_):
-        grad, ctx.grad = ctx.grad, None
-        if g_loss is None:
-            return None, None, None, None
-        if grad is None:
-            raise RuntimeError("a second backward pass through a preference or policy loss: its gradient went to the first one")
-        if not ctx.prescaled:
-            LAUNCHES[0] += 1
-            ext().scale_rows(grad, g_loss.float().contiguous())
-        return grad, None, None, None
-
-
-def _run_loss(logits, call, inplace, grad_scale):
-    LAUNCHES[0] += 2
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _LossFn.apply(logits, call, bool(inplace), grad_scale is not None)
-    return call(0)[:-1]
-
-
 def _run_reference(out, grad_scale, logits):
     if grad_scale is None or not torch.is_grad_enabled():
         return out
@@ -243,10 +194,11 @@ def preference_loss(logits, labels, cu, ref_logprobs: Optional[torch.Tensor] = N
                                                         average, pad_idx, temperature), grad_scale, logits)
     x, y, c = _as_rows(logits), labels.long().contiguous(), cu.int().contiguous()
     r = None if ref_logprobs is None else ref_logprobs.float().contiguous()
-    data = x.detach()
-    return _run_loss(x, lambda grad: ext().preference_loss(data, y, c, r, KINDS[kind], float(beta), float(smoothing), float(margin),
-                                                           float(nll_weight), bool(average), int(pad_idx), float(temperature), grad,
-                                                           scale_at, scale), inplace, grad_scale)
+    cfg = (x, y, c, r, KINDS[kind], float(beta), float(smoothing), float(margin), float(nll_weight), bool(average), int(pad_idx), float(temperature))
+    LAUNCHES[0] += 4
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return ext().preference_loss_node(*cfg, bool(inplace), scale_at, scale, grad_scale is not None)
+    return ext().preference_loss(*cfg, 0, scale_at, scale)[:-1]
 
 
 def policy_loss(logits, labels, old_logprobs, advantages, ref_logprobs: Optional[torch.Tensor] = None, clip: float = 0.2,
@@ -276,6 +228,8 @@ def policy_loss(logits, labels, old_logprobs, advantages, ref_logprobs: Optional
     x, y = _as_rows(logits), labels.long().contiguous()
     old, adv = old_logprobs.float().contiguous(), advantages.float().contiguous()
     r = None if ref_logprobs is None else ref_logprobs.float().contiguous()
-    data = x.detach()
-    return _run_loss(x, lambda grad: ext().policy_loss(data, y, old, adv, r, float(clip), float(high), float(kl_coef), int(pad_idx),
-                                                       float(temperature), grad, scale_at, scale), inplace, grad_scale)
+    cfg = (x, y, old, adv, r, float(clip), float(high), float(kl_coef), int(pad_idx), float(temperature))
+    LAUNCHES[0] += 2
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return ext().policy_loss_node(*cfg, bool(inplace), scale_at, scale, grad_scale is not None)
+    return ext().policy_loss(*cfg, 0, scale_at, scale)[:-1]
