@@ -698,29 +698,20 @@ def attention(q, k, v, cu_q, cu_k, heads, max_q, max_k, causal=False, dropout_p=
 # ---------------------------------------------------------------------------------------------------
 class _EmbedFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, dummy, tokens, positions, table, pos_table, gtable, gpos, scale, p, seed, sid, pad_idx, sorted_grad=False):
+    def forward(ctx, dummy, tokens, positions, table, pos_table, gtable, gpos, scale, p, seed, sid, pad_idx):
         out = ext().embed_fwd(tokens, positions, table, pos_table, scale, p, seed, sid)
         ctx.save_for_backward(tokens, positions)
-        ctx.cfg = (scale, p, seed, sid, pad_idx, table.shape[0], sorted_grad)
+        ctx.cfg = (scale, p, seed, sid, pad_idx)
         ctx.gtable, ctx.gpos = gtable, gpos
         return out
 
     @staticmethod
     def backward(ctx, dy):
         tokens, positions = ctx.saved_tensors
-        scale, p, seed, sid, pad_idx, vocab, sorted_grad = ctx.cfg
-        if sorted_grad:
-            dy = dy.contiguous()
-            if ctx.gtable is not None:
-                LAUNCHES[0] += 3
-                ext().embed_grad(tokens, None, dy, ctx.gtable, vocab, vocab, scale, p, seed, sid, pad_idx)
-            if ctx.gpos is not None:
-                LAUNCHES[0] += 3
-                pos = torch.zeros_like(tokens) if positions is None else positions
-                ext().embed_grad(tokens, pos, dy, ctx.gpos, vocab, ctx.gpos.shape[0], 1.0, p, seed, sid, pad_idx)
-        elif ctx.gtable is not None:
+        scale, p, seed, sid, pad_idx = ctx.cfg
+        if ctx.gtable is not None:
             ext().embed_bwd(tokens, positions, dy.contiguous(), ctx.gtable, ctx.gpos, scale, p, seed, sid, pad_idx)
-        return (None,) * 13
+        return (None,) * 12
 
 
 _dummy = {}
@@ -756,8 +747,12 @@ def embedding(tokens, table, positions=None, pos_table=None, scale=1.0, dropout_
                 gpos = pos_table.main_grad
         gtable = table.main_grad if table.requires_grad else None
         if torch.is_grad_enabled() and (gtable is not None or gpos is not None):
+            if sorted_grad:
+                LAUNCHES[0] += 1 + 3 * (gtable is not None) + 3 * (gpos is not None)
+                return ext().embed_flat_node(_grad_anchor(tokens.device), tokens, positions, table.work, pt, gtable, gpos, float(scale), p,
+                                             _Rng.seed, sid, int(pad_idx))
             return _EmbedFn.apply(_grad_anchor(tokens.device), tokens, positions, table.work, pt, gtable, gpos, scale, p,
-                                  _Rng.seed, sid, pad_idx, bool(sorted_grad))
+                                  _Rng.seed, sid, pad_idx)
         return ext().embed_fwd(tokens, positions, table.work, pt, scale, p, _Rng.seed, sid)
     if sorted_grad:
         return _embedding_sorted(tokens, table, positions, pos_table, float(scale), p, int(pad_idx))

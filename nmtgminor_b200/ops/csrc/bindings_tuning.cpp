@@ -3,6 +3,7 @@
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include "ops_api.h"
 #include "tuning_api.h"
 
 const unsigned long long* nmtg_seed_word(int device);       // bindings.cpp
@@ -192,6 +193,30 @@ Tensor embed_rows(const Tensor& tokens, const Tensor& table, double scale) {
   ck(nmtg_embed_rows(tokens.data_ptr<int64_t>(), table.data_ptr(), out.data_ptr(), static_cast<int>(tokens.numel()),
                      static_cast<int>(table.size(0)), static_cast<int>(table.size(1)), dtype_code(table, "table"), static_cast<float>(scale),
                      cur_stream()));
+  return out;
+}
+
+// dropout(table[tokens] * scale + pos_table[positions]) of bf16 tables whose width is a multiple of 16
+Tensor embed_flat(const Tensor& tokens, const OptTensor& positions, const Tensor& table, const OptTensor& pos_table, double scale, double p,
+                  int64_t seed, int64_t stream_id) {
+  if (!pos_table.has_value() && p == 0.0) return embed_rows(tokens, table, scale);
+  TORCH_CHECK(table.is_cuda() && table.dim() == 2 && table.is_contiguous() && table.scalar_type() == at::kBFloat16, "table must be a dense bf16 matrix on a GPU");
+  const int64_t rows = tokens.numel(), width = table.size(1);
+  need(tokens, table, at::kLong, rows, "tokens");
+  if (positions.has_value()) need(*positions, table, at::kLong, rows, "positions");
+  if (pos_table.has_value()) {
+    need(*pos_table, table, at::kBFloat16, pos_table->numel(), "pos_table");
+    TORCH_CHECK(pos_table->dim() == 2 && pos_table->size(1) == width && pos_table->size(0) >= 1, "pos_table: wrong size");
+  }
+  TORCH_CHECK(rows < (1 << 30) && table.size(0) >= 1 && table.size(0) < (1LL << 31) && width < (1 << 30), "embedding: too large");
+  c10::cuda::CUDAGuard guard(table.device());
+  Tensor out = at::empty({rows, width}, table.options().requires_grad(false));
+  if (rows > 0)
+    ck(nmtg_embed_fwd(tokens.data_ptr<int64_t>(), positions.has_value() ? positions->data_ptr<int64_t>() : nullptr, table.data_ptr(),
+                      pos_table.has_value() ? pos_table->data_ptr() : nullptr, out.data_ptr(), static_cast<int>(rows), static_cast<int>(width),
+                      static_cast<int>(table.size(0)), pos_table.has_value() ? static_cast<int>(pos_table->size(0)) : 1, static_cast<float>(scale),
+                      static_cast<float>(p), static_cast<unsigned long long>(seed), static_cast<unsigned long long>(stream_id),
+                      nmtg_seed_word(table.get_device()), cur_stream()));
   return out;
 }
 
@@ -422,6 +447,38 @@ struct EmbedNode : Function<EmbedNode> {
   }
 };
 
+// A table of the flat store: gradients are added to the store's buffers.  `anchor` is a tensor with a gradient that keeps the node alive.
+struct FlatEmbedNode : Function<FlatEmbedNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& /*anchor*/, const Tensor& tokens, const OptTensor& positions, const Tensor& table,
+                        const OptTensor& pos_table, const OptTensor& gtable, const OptTensor& gpos, double scale, double p, int64_t seed,
+                        int64_t stream_id, int64_t pad) {
+    ctx->saved_data["tokens"] = tokens;
+    ctx->saved_data["positions"] = positions;
+    ctx->saved_data["gtable"] = gtable;
+    ctx->saved_data["gpos"] = gpos;
+    ctx->saved_data["words"] = table.size(0);
+    ctx->saved_data["numbers"] = std::vector<double>{scale, p};
+    ctx->saved_data["ids"] = std::vector<int64_t>{seed, stream_id, pad};
+    ctx->set_materialize_grads(false);
+    return embed_flat(tokens, positions, table, pos_table, scale, p, seed, stream_id);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    variable_list out(12);
+    if (!g[0].defined()) return out;
+    const Tensor dy = g[0].contiguous(), tokens = ctx->saved_data["tokens"].toTensor();
+    const int64_t words = ctx->saved_data["words"].toInt();
+    const auto numbers = ctx->saved_data["numbers"].toDoubleVector();
+    const auto ids = ctx->saved_data["ids"].toIntVector();
+    const auto optional = [&](const char* name) { const c10::IValue& v = ctx->saved_data[name]; return v.isNone() ? OptTensor() : OptTensor(v.toTensor()); };
+    const OptTensor gtable = optional("gtable"), gpos = optional("gpos"), positions = optional("positions");
+    if (gtable.has_value()) embed_grad(tokens, OptTensor(), dy, gtable, words, words, numbers[0], numbers[1], ids[0], ids[1], ids[2]);
+    if (gpos.has_value())
+      embed_grad(tokens, positions.has_value() ? positions : OptTensor(at::zeros_like(tokens)), dy, gpos, words, gpos->size(0), 1.0, numbers[1], ids[0],
+                 ids[1], ids[2]);
+    return out;
+  }
+};
+
 struct ActivationNode : Function<ActivationNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& z, int64_t act, double p, int64_t seed, int64_t stream_id) {
     auto [y, codes, scales] = kept_forward(z, act, true, p, seed, stream_id);
@@ -467,6 +524,10 @@ void bind_tuning_ops(pybind11::module& m) {
   });
   m.def("embed_rows_node", [](const Tensor& table, const Tensor& tokens, double scale, int64_t pad) {
     return EmbedNode::apply(table, tokens, scale, pad);
+  });
+  m.def("embed_flat_node", [](const Tensor& anchor, const Tensor& tokens, const OptTensor& positions, const Tensor& table, const OptTensor& pos_table,
+                              const OptTensor& gtable, const OptTensor& gpos, double scale, double p, int64_t seed, int64_t stream_id, int64_t pad) {
+    return FlatEmbedNode::apply(anchor, tokens, positions, table, pos_table, gtable, gpos, scale, p, seed, stream_id, pad);
   });
   m.def("activation_node", [](const Tensor& z, int64_t act, double p, int64_t seed, int64_t stream_id) {
     return ActivationNode::apply(z, act, p, seed, stream_id);

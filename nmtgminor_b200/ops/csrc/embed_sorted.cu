@@ -2,7 +2,7 @@
 //   1. order:  the rows sorted by key (stable).  Up to kRankRows rows one kernel counts, for every row, the rows before it in the order
 //      (keys and row numbers packed into 32 bits, N^2 comparisons in registers); more rows take stable radix passes of up to 10 bits
 //      (count, scan, scatter).
-//   2. reduce: the sorted rows in chunks of 8 to 32, a group of threads each, whatever the words' frequencies are; a sum that begins and
+//   2. reduce: the sorted rows in chunks of 8 or 16, a group of threads each, whatever the words' frequencies are; a sum that begins and
 //      ends in a chunk goes to its row of the gradient, one that crosses an end leaves its part in the workspace.
 //   3. join:   the parts of a sum, in order.
 // Where the gradient is written whole, its rows are cleared by further blocks of the sorting kernels: these wait on latency, the clearing on memory.
@@ -21,9 +21,9 @@ int num_sms();
 
 namespace {
 
-constexpr int kRankBits = 13, kRankRows = 1 << kRankBits;      // rows that the counting kernel takes
-constexpr int kRankTile = 64;                                  // rows of one of its blocks
-constexpr int kTile = 2048;                                    // rows of a block of a radix pass
+constexpr int kRankBits = 14, kRankRows = 1 << kRankBits;      // rows that the counting kernel takes
+constexpr int kRankEach = 2, kRankTile = 16 * kRankEach;        // rows of a group of 16 threads, and of a block
+constexpr int kTile = 1024;                                    // rows of a block of a radix pass
 constexpr int kDigitBits = 10;                                 // at most
 
 struct Keys {
@@ -31,12 +31,21 @@ struct Keys {
   const int64_t* positions;
   int rows, vocab, keys;
   long pad;
-  __device__ __forceinline__ int of(int r) const {            // `keys`: the row has none
-    const int64_t t = tokens[r];
+  __device__ __forceinline__ int of(int64_t t, int64_t p) const {            // `keys`: the row has none
     if (t == pad || t < 0 || t >= vocab) return keys;
     if (!positions) return static_cast<int>(t);
-    const int64_t p = positions[r];
     return p < 0 ? 0 : p >= keys ? keys - 1 : static_cast<int>(p);
+  }
+  // keys of rows r, r + step, ...: all asked for before the first is looked at
+  template <int kN> __device__ __forceinline__ void of(int r, int step, int end, int (&key)[kN]) const {
+    int64_t t[kN], p[kN];
+#pragma unroll
+    for (int j = 0; j < kN; ++j) {
+      t[j] = r + j * step < end ? tokens[r + j * step] : -1;
+      p[j] = positions && r + j * step < end ? positions[r + j * step] : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < kN; ++j) key[j] = of(t[j], p[j]);
   }
 };
 
@@ -53,25 +62,34 @@ struct Clear {
   }
 };
 
-// order[rank] = row, sorted[rank] = key.  A thread counts for 4 rows over every 16th group of 4 rows.
+// order[rank] = row, sorted[rank] = key.  16 threads count for the same rows, each over every 16th group of 4.
 __global__ void __launch_bounds__(256) rank_kernel(const Keys k, int* __restrict__ order, int* __restrict__ sorted, const Clear clear) {
   if (clear.mine()) { clear.run(); return; }
   extern __shared__ __align__(16) uint32_t all[];
   const int padded = (k.rows + 63) & ~63;
-  for (int i = threadIdx.x; i < padded; i += 256) all[i] = i < k.rows ? static_cast<uint32_t>(k.of(i)) << kRankBits | i : 0xFFFFFFFFu;
-  __syncthreads();
-  const int lane16 = threadIdx.x & 15, first = blockIdx.x * kRankTile + (threadIdx.x >> 4) * 4;
-  uint32_t mine[4];
-  int count[4] = {0, 0, 0, 0};
+  for (int i = threadIdx.x; i < padded; i += 16 * 256) {
+    int key[16];
+    k.of(i, 256, k.rows, key);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) mine[j] = first + j < padded ? all[first + j] : 0xFFFFFFFFu;
+    for (int j = 0; j < 16; ++j) {
+      const int at = i + j * 256;
+      if (at < padded) all[at] = at < k.rows ? static_cast<uint32_t>(key[j]) << kRankBits | at : 0xFFFFFFFFu;
+    }
+  }
+  __syncthreads();
+  const int lane16 = threadIdx.x & 15, first = blockIdx.x * kRankTile + (threadIdx.x >> 4) * kRankEach;
+  uint32_t mine[kRankEach];
+  int count[kRankEach] = {};
+#pragma unroll
+  for (int j = 0; j < kRankEach; ++j) mine[j] = first + j < padded ? all[first + j] : 0xFFFFFFFFu;
+#pragma unroll 4
   for (int i = lane16; i < padded / 4; i += 16) {
     const uint4 u = reinterpret_cast<const uint4*>(all)[i];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) count[j] += (u.x < mine[j]) + (u.y < mine[j]) + (u.z < mine[j]) + (u.w < mine[j]);
+    for (int j = 0; j < kRankEach; ++j) count[j] += (u.x < mine[j]) + (u.y < mine[j]) + (u.z < mine[j]) + (u.w < mine[j]);
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < kRankEach; ++j) {
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) count[j] += __shfl_xor_sync(0xffffffffu, count[j], o);
     if (lane16 == 0 && first + j < k.rows) {
@@ -91,15 +109,23 @@ struct Pass {
   int shift, bins, tiles;
 };
 
-__device__ __forceinline__ int key_at(const Keys& k, const Pass& p, int i) { return p.key ? p.key[i] : k.of(i); }
+template <int kN> __device__ __forceinline__ void keys_at(const Keys& k, const Pass& p, int i, int step, int end, int (&key)[kN]) {
+  if (!p.key) { k.of(i, step, end, key); return; }
+#pragma unroll
+  for (int j = 0; j < kN; ++j) key[j] = i + j * step < end ? p.key[i + j * step] : 0;
+}
 
 __global__ void __launch_bounds__(256) radix_count_kernel(const Keys k, const Pass p, const Clear clear) {
   if (clear.mine()) { clear.run(); return; }
   __shared__ int bins[1 << kDigitBits];
   for (int b = threadIdx.x; b < p.bins; b += 256) bins[b] = 0;
   __syncthreads();
-  for (int i = blockIdx.x * kTile + threadIdx.x; i < min(k.rows, (static_cast<int>(blockIdx.x) + 1) * kTile); i += 256)
-    atomicAdd(&bins[(key_at(k, p, i) >> p.shift) & (p.bins - 1)], 1);
+  const int begin = blockIdx.x * kTile + threadIdx.x;
+  int key[kTile / 256];
+  keys_at(k, p, begin, 256, k.rows, key);
+#pragma unroll
+  for (int j = 0; j < kTile / 256; ++j)
+    if (begin + j * 256 < k.rows) atomicAdd(&bins[(key[j] >> p.shift) & (p.bins - 1)], 1);
   __syncthreads();
   for (int b = threadIdx.x; b < p.bins; b += 256) p.counts[static_cast<long>(b) * p.tiles + blockIdx.x] = bins[b];
 }
@@ -156,8 +182,17 @@ __global__ void __launch_bounds__(256) radix_scatter_kernel(const Keys k, const 
   const int begin = blockIdx.x * kTile + warp * (kTile / 8), end = min(k.rows, begin + kTile / 8);
   int* const mine = at + warp * p.bins;
   const uint32_t below = (1u << lane) - 1;
-  for (int i0 = begin; i0 < end; i0 += 32) {
-    const int i = i0 + lane, d = i < end ? (key_at(k, p, i) >> p.shift) & (p.bins - 1) : -1;
+  constexpr int kRounds = kTile / 256;
+  int key[kRounds], row[kRounds];
+  keys_at(k, p, begin + lane, 32, k.rows, key);
+#pragma unroll
+  for (int j = 0; j < kRounds; ++j) {
+    const int i = begin + j * 32 + lane;
+    row[j] = p.row && i < end ? p.row[i] : i;
+  }
+#pragma unroll
+  for (int j = 0; j < kRounds; ++j) {
+    const int i = begin + j * 32 + lane, d = i < end ? (key[j] >> p.shift) & (p.bins - 1) : -1;
     const uint32_t same = __match_any_sync(0xffffffffu, d);
     if (d >= 0 && (same & below) == 0) mine[d] += __popc(same);
     __syncwarp();
@@ -169,14 +204,15 @@ __global__ void __launch_bounds__(256) radix_scatter_kernel(const Keys k, const 
     for (int w = 0; w < 8; ++w) { const int n = at[w * p.bins + b]; at[w * p.bins + b] = sum; sum += n; }
   }
   __syncthreads();
-  for (int i0 = begin; i0 < end; i0 += 32) {
-    const int i = i0 + lane, key = i < end ? key_at(k, p, i) : 0, d = i < end ? (key >> p.shift) & (p.bins - 1) : -1;
+#pragma unroll
+  for (int j = 0; j < kRounds; ++j) {
+    const int i = begin + j * 32 + lane, d = i < end ? (key[j] >> p.shift) & (p.bins - 1) : -1;
     const uint32_t same = __match_any_sync(0xffffffffu, d);
     const int place = d >= 0 ? mine[d] + __popc(same & below) : 0;
     __syncwarp();
     if (d >= 0) {
-      p.key_out[place] = key;
-      p.row_out[place] = p.row ? p.row[i] : i;
+      p.key_out[place] = key[j];
+      p.row_out[place] = row[j];
       if ((same & below) == 0) mine[d] += __popc(same);
     }
     __syncwarp();
@@ -206,6 +242,7 @@ struct Sum {
   const unsigned long long* seed_dev;
 };
 
+// One addition an element and call: the gradient does not depend on an order, and nothing waits for what was there.
 template <typename T, int kN, bool kAdd>
 __device__ __forceinline__ void to_grad(const Sum& s, int key, int col, const float (&acc)[kN]) {
   const long at = static_cast<long>(key) * s.width + col;
@@ -213,15 +250,12 @@ __device__ __forceinline__ void to_grad(const Sum& s, int key, int col, const fl
     float* g = static_cast<float*>(s.grad) + at;
     if constexpr (kN % 4 == 0) {
 #pragma unroll
-      for (int j = 0; j < kN; j += 4) {
-        float4 v = *reinterpret_cast<float4*>(g + j);
-        v.x = fmaf(acc[j], s.scale, v.x); v.y = fmaf(acc[j + 1], s.scale, v.y);
-        v.z = fmaf(acc[j + 2], s.scale, v.z); v.w = fmaf(acc[j + 3], s.scale, v.w);
-        *reinterpret_cast<float4*>(g + j) = v;
-      }
+      for (int j = 0; j < kN; j += 4)
+        asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(g + j), "f"(acc[j] * s.scale), "f"(acc[j + 1] * s.scale),
+                     "f"(acc[j + 2] * s.scale), "f"(acc[j + 3] * s.scale) : "memory");
     } else {
 #pragma unroll
-      for (int j = 0; j < kN; ++j) g[j] = fmaf(acc[j], s.scale, g[j]);
+      for (int j = 0; j < kN; ++j) asm volatile("red.global.add.f32 [%0], %1;" ::"l"(g + j), "f"(acc[j] * s.scale) : "memory");
     }
   } else {
     Pack<T, kN> o;
@@ -231,22 +265,39 @@ __device__ __forceinline__ void to_grad(const Sum& s, int key, int col, const fl
   }
 }
 
-// blockDim = (column vectors, chunks of this block)
+// blockDim = (column vectors, chunks of this block), whole warps to a chunk; a lane has the key and the row of one of its sorted rows.  Every thread
+// copies its columns of all the chunk's rows to shared memory (kCopy) before it adds up the first: 64 KB a block on their way, and three blocks
+// to an SM, whatever the words' frequencies are.
 template <typename T, int kN, bool kDrop, bool kAdd>
-__global__ void __launch_bounds__(256) reduce_kernel(const Sum s) {
-  constexpr int kAhead = 8;
-  const int c = blockIdx.x * blockDim.y + threadIdx.y;
+__global__ void __launch_bounds__(256, 3) reduce_kernel(const Sum s) {
+  constexpr bool kCopy = sizeof(T) * kN == 16;
+  extern __shared__ __align__(16) uint4 held[];                 // [chunk][256]
+  const int c = blockIdx.x * blockDim.y + threadIdx.y, lane = threadIdx.x & 31, thread = threadIdx.y * blockDim.x + threadIdx.x;
   if (c >= s.chunks) return;
-  const int begin = c * s.chunk, end = min(s.rows, begin + s.chunk);
+  const int begin = c * s.chunk, count = min(s.rows - begin, s.chunk);
   const DropRng rng(s.seed + ((kDrop && s.seed_dev) ? *s.seed_dev : 0ull), s.stream_id, s.p);
-  const int before = begin > 0 ? s.sorted[begin - 1] : -1;
-  const int after = end < s.rows ? s.sorted[end] : -1;
-  if (s.sorted[begin] >= s.keys) return;                        // rows without a key come last
-  for (int col = (blockIdx.y * blockDim.x + threadIdx.x) * kN; col < s.width; col += gridDim.y * blockDim.x * kN) {
+  const int my_key = lane < count ? s.sorted[begin + lane] : s.keys, my_row = lane < count ? s.order[begin + lane] : 0;
+  const int before = begin > 0 ? s.sorted[begin - 1] : -1, after = begin + count < s.rows ? s.sorted[begin + count] : -1;
+  const int first = __shfl_sync(0xffffffffu, my_key, 0);
+  const int with_key = __popc(__ballot_sync(0xffffffffu, my_key < s.keys));       // rows without a key come last
+  if (with_key == 0) return;
+  for (int base = 0; base < s.width; base += blockDim.x * kN) {
+    const int col = base + threadIdx.x * kN;
+    const bool in = col < s.width;
+    const T* const dy = static_cast<const T*>(s.dy) + col;
+    if constexpr (kCopy) {
+#pragma unroll 4
+      for (int j = 0; j < with_key; ++j) {
+        const int row = __shfl_sync(0xffffffffu, my_row, j);
+        if (in) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(held + j * 256 + thread)), "l"(dy + static_cast<long>(row) * s.width) : "memory");
+      }
+      asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+    }
     float acc[kN];
 #pragma unroll
     for (int j = 0; j < kN; ++j) acc[j] = 0.f;
     const auto flush = [&](int key, bool began_before, bool goes_on) {
+      if (!in) return;
       if (began_before || goes_on) {
         float* part = s.parts + (static_cast<long>(c) * 2 + (began_before ? 0 : 1)) * s.width + col;
         if constexpr (kN % 4 == 0) {
@@ -260,35 +311,27 @@ __global__ void __launch_bounds__(256) reduce_kernel(const Sum s) {
         to_grad<T, kN, kAdd>(s, key, col, acc);
       }
     };
-    int key = s.sorted[begin];
+    int key = first;
     bool began_before = key == before;
-    for (int i0 = begin; i0 < end; i0 += kAhead) {
-      Pack<T, kN> v[kAhead];
-      int keys[kAhead], rows[kAhead];
+#pragma unroll 1
+    for (int j = 0; j < with_key; ++j) {
+      const int of = __shfl_sync(0xffffffffu, my_key, j), row = __shfl_sync(0xffffffffu, my_row, j);
+      if (of != key) {
+        flush(key, began_before, false);
+        key = of;
+        began_before = false;
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        keys[j] = i0 + j < end ? s.sorted[i0 + j] : s.keys;
-        rows[j] = i0 + j < end ? s.order[i0 + j] : 0;
+        for (int q = 0; q < kN; ++q) acc[q] = 0.f;
       }
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j)
-        if (keys[j] < s.keys) v[j] = *reinterpret_cast<const Pack<T, kN>*>(static_cast<const T*>(s.dy) + static_cast<long>(rows[j]) * s.width + col);
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        if (i0 + j >= end) break;
-        if (keys[j] != key) {
-          if (key < s.keys) flush(key, began_before, false);
-          key = keys[j];
-          began_before = false;
-#pragma unroll
-          for (int q = 0; q < kN; ++q) acc[q] = 0.f;
-        }
-        if (key >= s.keys) break;
+      if (in) {
+        Pack<T, kN> v;
+        if constexpr (kCopy) v = *reinterpret_cast<const Pack<T, kN>*>(held + j * 256 + thread);
+        else v = *reinterpret_cast<const Pack<T, kN>*>(dy + static_cast<long>(row) * s.width);
 #pragma unroll
         for (int q = 0; q < kN; ++q) {
-          float f = to_f<T>(v[j].v[q]);
+          float f = to_f<T>(v.v[q]);
           if constexpr (kDrop) {
-            const unsigned long long at = static_cast<unsigned long long>(rows[j]) * s.width + col;
+            const unsigned long long at = static_cast<unsigned long long>(row) * s.width + col;
             bool keep;
             if constexpr (kN % 4 == 0) keep = rng.keep(rng.word((at >> 2) + q / 4), q % 4);
             else keep = rng.keep(rng.word((at + q) >> 2), static_cast<int>((at + q) & 3));
@@ -297,61 +340,73 @@ __global__ void __launch_bounds__(256) reduce_kernel(const Sum s) {
           acc[q] += f;
         }
       }
-      if (key >= s.keys) break;
     }
-    if (key < s.keys) flush(key, began_before, key == after);
+    flush(key, began_before, with_key == s.chunk && key == after);
   }
 }
 
-// A block to each chunk in which a sum begins that goes on behind it: its parts, in 8 runs one after another, the runs in order.
+// A block to each chunk in which a sum begins that goes on behind it (and to a share of the columns): its parts, in 8 runs one after another, the
+// runs in order.  One look tells whether there is one; the sum's end is found by 32 looks at a time.
 template <typename T, int kN, bool kAdd>
 __global__ void __launch_bounds__(256) join_kernel(const Sum s) {
   constexpr int kRuns = 8, kCols = 32;
   __shared__ float runs[kRuns][kCols * kN];
-  const int c = blockIdx.x, begin = c * s.chunk, end = begin + s.chunk;
-  if (end >= s.rows) return;
-  const int key = s.sorted[end - 1];
-  if (key >= s.keys || s.sorted[end] != key) return;
-  if (s.sorted[begin] == key && begin > 0 && s.sorted[begin - 1] == key) return;       // began earlier
-  int lo = end, hi = s.rows;                                    // first place behind the sum's last
-  while (lo < hi) { const int mid = lo + (hi - lo) / 2; if (s.sorted[mid] > key) hi = mid; else lo = mid + 1; }
-  const int n = (lo - 1) / s.chunk - c;                         // parts in the chunks behind this one
-  const int x = threadIdx.x & 31, run = threadIdx.x >> 5;
-  const int from = static_cast<int>(static_cast<long>(n + 1) * run / kRuns), to = static_cast<int>(static_cast<long>(n + 1) * (run + 1) / kRuns);
-  for (int base = blockIdx.y * kCols * kN; base < s.width; base += gridDim.y * kCols * kN) {
-    const int col = base + x * kN;
-    float acc[kN];
+  const int x = threadIdx.x & 31, run = threadIdx.x >> 5, c = blockIdx.x;
+  {
+    const int begin = c * s.chunk, end = begin + s.chunk, places[4] = {end - 1, end, begin, begin - 1};
+    int seen[4];
 #pragma unroll
-    for (int j = 0; j < kN; ++j) acc[j] = 0.f;
-    if (col < s.width) {
+    for (int j = 0; j < 4; ++j) seen[j] = places[j] >= 0 && places[j] < s.rows ? s.sorted[places[j]] : -1;
+    const int key = seen[0];
+    if (key < 0 || key >= s.keys || seen[1] != key || (seen[2] == key && seen[3] == key)) return;
+    // a sum that begins here
+    int lo = (c + 1) * s.chunk, hi = s.rows;                    // the first place behind the sum's last is in [lo, hi]
+    while (lo < hi) {
+      const int step = (hi - lo + 31) / 32, at = lo + x * step;
+      const bool same = at < hi && s.sorted[at] == key;
+      const int n = __popc(__ballot_sync(0xffffffffu, same));   // looks that still see the key
+      if (n == 0) break;
+      const int next = lo + n * step;
+      lo = lo + (n - 1) * step + 1;
+      hi = min(hi, next);
+    }
+    const int n = (lo - 1) / s.chunk - c;                       // parts in the chunks behind this one
+    const int from = static_cast<int>(static_cast<long>(n + 1) * run / kRuns), to = static_cast<int>(static_cast<long>(n + 1) * (run + 1) / kRuns);
+    for (int base = blockIdx.y * kCols * kN; base < s.width; base += gridDim.y * kCols * kN) {
+      const int col = base + x * kN;
+      float acc[kN];
+#pragma unroll
+      for (int j = 0; j < kN; ++j) acc[j] = 0.f;
+      if (col < s.width) {
 #pragma unroll 4
-      for (int i = from; i < to; ++i) {
-        const float* part = s.parts + (static_cast<long>(c + i) * 2 + (i == 0 ? 1 : 0)) * s.width + col;
-        if constexpr (kN % 4 == 0) {
+        for (int i = from; i < to; ++i) {
+          const float* part = s.parts + (static_cast<long>(c + i) * 2 + (i == 0 ? 1 : 0)) * s.width + col;
+          if constexpr (kN % 4 == 0) {
 #pragma unroll
-          for (int j = 0; j < kN; j += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(part + j);
-            acc[j] += v.x; acc[j + 1] += v.y; acc[j + 2] += v.z; acc[j + 3] += v.w;
+            for (int j = 0; j < kN; j += 4) {
+              const float4 v = *reinterpret_cast<const float4*>(part + j);
+              acc[j] += v.x; acc[j + 1] += v.y; acc[j + 2] += v.z; acc[j + 3] += v.w;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < kN; ++j) acc[j] += part[j];
           }
-        } else {
-#pragma unroll
-          for (int j = 0; j < kN; ++j) acc[j] += part[j];
         }
       }
-    }
 #pragma unroll
-    for (int j = 0; j < kN; ++j) runs[run][x * kN + j] = acc[j];
-    __syncthreads();
-    if (run == 0 && col < s.width) {
+      for (int j = 0; j < kN; ++j) runs[run][x * kN + j] = acc[j];
+      __syncthreads();
+      if (run == 0 && col < s.width) {
 #pragma unroll
-      for (int j = 0; j < kN; ++j) {
-        acc[j] = 0.f;
+        for (int j = 0; j < kN; ++j) {
+          acc[j] = 0.f;
 #pragma unroll
-        for (int r = 0; r < kRuns; ++r) acc[j] += runs[r][x * kN + j];
+          for (int r = 0; r < kRuns; ++r) acc[j] += runs[r][x * kN + j];
+        }
+        to_grad<T, kN, kAdd>(s, key, col, acc);
       }
-      to_grad<T, kN, kAdd>(s, key, col, acc);
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 
@@ -375,8 +430,8 @@ const char* problem(cudaError_t e) { return e == cudaSuccess ? nullptr : cudaGet
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 long up16(long n) { return (n + 15) & ~15L; }
 
-// Rows of a chunk: enough chunks for every SM where there are few rows, fewer parts to join where there are many
-int chunk_of(int rows) { return rows < 4096 ? 8 : rows < 32768 ? 16 : 32; }
+// Rows of a chunk (at most 32, a lane to each): enough chunks for every SM where there are few rows, fewer parts to join where there are many
+int chunk_of(int rows) { return rows < 4096 ? 8 : 16; }
 int key_bits(int keys) {           // of numbers up to `keys`
   int b = 1;
   while (b < 31 && (1L << b) <= keys) ++b;
@@ -393,8 +448,11 @@ dim3 shape(int width, int n) {
 template <typename T, int kN, bool kDrop, bool kAdd>
 const char* sums(const Sum& s, cudaStream_t stream) {
   const dim3 block = shape(s.width, kN);
-  reduce_kernel<T, kN, kDrop, kAdd><<<dim3((s.chunks + block.y - 1) / block.y), block, 0, stream>>>(s);
-  cudaError_t e = cudaGetLastError();
+  const int smem = sizeof(T) * kN == 16 ? s.chunk * 256 * 16 : 0;
+  cudaError_t e = cudaFuncSetAttribute(reduce_kernel<T, kN, kDrop, kAdd>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return problem(e);
+  reduce_kernel<T, kN, kDrop, kAdd><<<dim3((s.chunks + block.y - 1) / block.y), block, smem, stream>>>(s);
+  e = cudaGetLastError();
   if (e != cudaSuccess || s.chunks < 2) return problem(e);
   const int cols = (s.width + 32 * kN - 1) / (32 * kN);
   join_kernel<T, kN, kAdd><<<dim3(s.chunks, cols < 8 ? cols : 8), 256, 0, stream>>>(s);
@@ -462,7 +520,10 @@ const char* nmtg_embed_grad(const NmtgEmbedGrad* d) {
   cudaError_t e;
   if (n <= kRankRows && bits + kRankBits <= 32) {
     clear.first = (n + kRankTile - 1) / kRankTile;
-    rank_kernel<<<clear.first + extra, 256, ((n + 63) & ~63) * 4, stream>>>(k, row[0], key[0], clear);
+    const int smem = ((n + 63) & ~63) * 4;
+    if (smem > 48 * 1024 && (e = cudaFuncSetAttribute(rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRankRows * 4)) != cudaSuccess)
+      return cudaGetErrorString(e);
+    rank_kernel<<<clear.first + extra, 256, smem, stream>>>(k, row[0], key[0], clear);
     if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
   } else {
     const int passes = (bits + kDigitBits - 1) / kDigitBits, digit = (bits + passes - 1) / passes;

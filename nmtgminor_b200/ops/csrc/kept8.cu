@@ -69,9 +69,9 @@ __device__ __forceinline__ float2 decode2(uint32_t codes) {
 template <typename T> struct Tail {       // Q(a) and exp(-a^2 / 2), a >= 0
   static __device__ __forceinline__ void get(float a, float& q, float& gauss) {
     const float x = -0.72134752f * a * a;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(gauss) : "f"(x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(gauss) : "f"(x));
     float t;
-    asm("rcp.approx.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.360624458f, a, 1.f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.360624458f, a, 1.f)));
     float h = fmaf(0.0472499409f, t, -0.17956728f);
     h = fmaf(h, t, 0.179222625f);
     h = fmaf(h, t, 0.0275265627f);
@@ -90,8 +90,8 @@ template <> struct Tail<float> {
 template <typename T> __device__ __forceinline__ float gate(float z) {        // sigmoid
   if constexpr (sizeof(T) == 4) return 1.f / (1.f + expf(-z));
   float e, r;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(-1.44269504f * z));
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.44269504f * z));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
   return r;
 }
 template <typename T, int kAct> __device__ __forceinline__ float act_of(float z) {
@@ -135,7 +135,7 @@ enum Step { kQuantise = 0, kRestore = 1, kForward = 2, kBackward = 3 };
 
 // elements [col, col + kN) of a row; `index` numbers the first for dropout; `lanes` lanes hold a block
 template <typename T, int kN, int kStep, int kAct, bool kDrop>
-__device__ __forceinline__ void work(const Args& a, const DropRng& rng, long row, long col, bool in_row) {
+__device__ __noinline__ void work(const Args& a, const DropRng& rng, long row, long col, bool in_row) {
   constexpr int kLanes = kBlock / kN;
   const long block = col / kBlock, index = row * a.width + col;
   float f[kN];
@@ -145,7 +145,12 @@ __device__ __forceinline__ void work(const Args& a, const DropRng& rng, long row
     if (!in_row) return;
     unit = power(static_cast<int>(a.scales[row * a.blocks + block]) - 127);
     const uint8_t* c = a.codes + row * a.ld_codes + col;
-    if constexpr (kN == 8) {
+    if constexpr (kN == 16) {
+      const uint4 u = *reinterpret_cast<const uint4*>(c);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) codes[j] = (w[j / 2] >> (16 * (j & 1))) & 0xFFFFu;
+    } else if constexpr (kN == 8) {
       const uint2 u = *reinterpret_cast<const uint2*>(c);
       codes[0] = u.x & 0xFFFFu; codes[1] = u.x >> 16; codes[2] = u.y & 0xFFFFu; codes[3] = u.y >> 16;
     } else if constexpr (kN == 4) {
@@ -175,7 +180,12 @@ __device__ __forceinline__ void work(const Args& a, const DropRng& rng, long row
 #pragma unroll
         for (int j = 0; j < kN; ++j) v[j] = finite(f[j]) ? f[j] * inv : NAN;
         uint8_t* c = a.codes + row * a.ld_codes + col;
-        if constexpr (kN == 8) {
+        if constexpr (kN == 16) {
+          uint32_t w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j] = encode2(v[2 * j], v[2 * j + 1]);
+          *reinterpret_cast<uint4*>(c) = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+        } else if constexpr (kN == 8) {
           *reinterpret_cast<uint2*>(c) = make_uint2(encode2(v[0], v[1]) | encode2(v[2], v[3]) << 16, encode2(v[4], v[5]) | encode2(v[6], v[7]) << 16);
         } else if constexpr (kN == 4) {
           *reinterpret_cast<uint32_t*>(c) = encode2(v[0], v[1]) | encode2(v[2], v[3]) << 16;
@@ -228,16 +238,196 @@ __device__ __forceinline__ void work(const Args& a, const DropRng& rng, long row
     if (a.out2) *reinterpret_cast<Pack<T, kN>*>(static_cast<T*>(a.out2) + index) = o2;
 }
 
+// ---- 16-bit types, whole vectors: two elements to an instruction wherever there is one for two -----------------------------
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)));
+  return *reinterpret_cast<const float2*>(&r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)),
+      "l"(*reinterpret_cast<const uint64_t*>(&c)));
+  return *reinterpret_cast<const float2*>(&r);
+}
+__device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float ex2(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+__device__ __forceinline__ float rcp(float v) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+
+__device__ __forceinline__ float2 unpack2(uint32_t u, __nv_bfloat16) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u)); }
+__device__ __forceinline__ float2 unpack2(uint32_t u, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+__device__ __forceinline__ uint32_t pack2(float2 v, __nv_bfloat16) { const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y); return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ uint32_t pack2(float2 v, __half) { const __half2 h = __floats2half2_rn(v.x, v.y); return *reinterpret_cast<const uint32_t*>(&h); }
+
+// Tail::get for two
+__device__ __forceinline__ void tails(float2 a, float2& q, float2& gauss) {
+  const float2 x = mul2(mul2(a, twice(-0.72134752f)), a);
+  gauss = make_float2(ex2(x.x), ex2(x.y));
+  const float2 d = fma2(a, twice(0.360624458f), twice(1.f)), t = make_float2(rcp(d.x), rcp(d.y));
+  float2 h = fma2(twice(0.0472499409f), t, twice(-0.17956728f));
+  h = fma2(h, t, twice(0.179222625f));
+  h = fma2(h, t, twice(0.0275265627f));
+  h = fma2(h, t, twice(0.139533017f));
+  h = fma2(h, t, twice(0.142076165f));
+  h = fma2(h, t, twice(0.143958751f));
+  q = mul2(mul2(h, t), gauss);
+}
+template <typename T, int kAct> __device__ __forceinline__ float2 acts_of(float2 z) {
+  if constexpr (kAct == 2) {
+    const float2 a = make_float2(fabsf(z.x), fabsf(z.y));
+    float2 q, gauss;
+    tails(a, q, gauss);
+    return make_float2(fmaf(-a.x, q.x, fmaxf(z.x, 0.f)), fmaf(-a.y, q.y, fmaxf(z.y, 0.f)));       // z Q(-z) = max(z, 0) - |z| Q(|z|)
+  }
+  return make_float2(act_of<T, kAct>(z.x), act_of<T, kAct>(z.y));
+}
+// A restored element has 4 significant bits, so that the slopes of GELU and SiLU have few values: a block makes a table of them, for every exponent,
+// 3 bits and sign, and an element costs a look into shared memory.  Between 2^-18 and 2^7 the slopes are computed in full precision; below it is
+// 1/2 but for 2^-18, above 0 or 1.  (33.6 M elements with GELU: 46 us with the arithmetic of the forward pass, 38 with a table of that range and
+// its ends looked after at every element.)
+constexpr int kSlopes = 1 << 12, kSlopeLow = (127 - 18) << 3, kSlopeHigh = (127 + 7) << 3;
+template <int kAct> __device__ __forceinline__ void make_slopes(float* table) {
+  for (int i = threadIdx.x; i < kSlopes; i += 256) {
+    const int at = i & 0x7FF;
+    const bool down = i >> 11;
+    float v = at < kSlopeLow ? 0.5f : down ? 0.f : 1.f;
+    if (at >= kSlopeLow && at < kSlopeHigh) v = slope_of<float, kAct>(__uint_as_float(static_cast<uint32_t>(i) << 20));
+    table[i] = v;
+  }
+  __syncthreads();
+}
+template <typename T, int kAct> __device__ __forceinline__ float2 slopes_of(float2 z, const float* table) {
+  if constexpr (kAct == 2 || kAct == 3) return make_float2(table[__float_as_uint(z.x) >> 20], table[__float_as_uint(z.y) >> 20]);
+  return make_float2(slope_of<T, kAct>(z.x), slope_of<T, kAct>(z.y));
+}
+
+// 16 or 32 bytes at a time
+template <int kWords> __device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[kWords]) {
+  if constexpr (kWords == 8) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
+  } else {
+    const uint4 u = *static_cast<const uint4*>(p);
+    w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+  }
+}
+template <int kWords> __device__ __forceinline__ void store_words(void* p, const uint32_t (&w)[kWords]) {
+  if constexpr (kWords == 8)
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+                 "r"(w[6]), "r"(w[7]) : "memory");
+  else
+    *static_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// `work` for 8 or 16 elements of 16 bits that are all there and ordinary: no infinity or NaN, nothing that leaves the type when it is restored.  What
+// is not ordinary is left to `work`; returns whether it was done.  All lanes of a warp, `in_row` for those with elements.
+template <typename T, int kN, int kStep, int kAct, bool kDrop>
+__device__ __forceinline__ bool work_pairs(const Args& a, const DropRng& rng, const float* table, long row, long col, bool in_row) {
+  constexpr int kWords = kN / 2;
+  const long block = col / kBlock, index = row * a.width + col;
+  uint32_t w[kWords] = {};
+  uint32_t codes[kN / 4] = {};
+  int scale = 0;
+  bool ordinary = true;
+  if constexpr (kStep != kRestore) {
+    if (in_row) load_words(static_cast<const T*>(a.in) + row * a.ld_in + col, w);
+  }
+  if constexpr (kStep == kRestore || kStep == kBackward) {
+    if (in_row) {
+      const uint8_t* const c = a.codes + row * a.ld_codes + col;
+      if constexpr (kN == 16) {
+        const uint4 u = *reinterpret_cast<const uint4*>(c);
+        codes[0] = u.x; codes[1] = u.y; codes[2] = u.z; codes[3] = u.w;
+      } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(c);
+        codes[0] = u.x; codes[1] = u.y;
+      }
+      scale = a.scales[row * a.blocks + block];
+      // restored values go to 448 * 2^(scale - 127): below 2^126 in bf16, 57344 in fp16
+      ordinary = scale <= (most<T>() > 1e6f ? 244 : 134);
+    }
+  }
+  uint32_t top = 0;
+  if constexpr (kStep == kQuantise || kStep == kForward) {
+    // magnitudes order as their bits do; infinity and NaN are above every number
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) top = __vmaxu2(top, w[j] & 0x7FFF7FFFu);
+    top = max(top & 0xFFFFu, top >> 16);
+#pragma unroll
+    for (int o = 1; o < kBlock / kN; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    ordinary = top < (most<T>() > 1e6f ? 0x7F80u : 0x7C00u);
+  }
+  if (!__all_sync(0xffffffffu, ordinary)) return false;
+  if constexpr (kStep == kQuantise || kStep == kForward) {
+    if (a.codes && in_row) {
+      const int e = block_exponent(unpack2(top, T()).x);
+      const float2 inv = twice(inverse_power(e));
+      uint32_t c[kWords];
+#pragma unroll
+      for (int j = 0; j < kWords; ++j) {
+        const float2 v = mul2(unpack2(w[j], T()), inv);
+        c[j] = encode2(v.x, v.y);
+      }
+      uint8_t* const to = a.codes + row * a.ld_codes + col;
+      if constexpr (kN == 16) *reinterpret_cast<uint4*>(to) = make_uint4(c[0] | c[1] << 16, c[2] | c[3] << 16, c[4] | c[5] << 16, c[6] | c[7] << 16);
+      else *reinterpret_cast<uint2*>(to) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+      if (col % kBlock == 0) a.scales[row * a.blocks + block] = static_cast<uint8_t>(e + 127);
+    }
+  }
+  if (!in_row || kStep == kQuantise) return true;
+  const float2 unit = twice(power(scale - 127));
+  uint32_t o[kWords], o2[kWords];
+#pragma unroll
+  for (int j = 0; j < kWords; ++j) {
+    float2 keep = twice(1.f);
+    if constexpr (kDrop) {
+      const uint32_t word = rng.word((static_cast<unsigned long long>(index) >> 2) + j / 2);
+      keep = make_float2(rng.keep(word, 2 * (j & 1)) ? rng.scale : 0.f, rng.keep(word, 2 * (j & 1) + 1) ? rng.scale : 0.f);
+    }
+    float2 z = make_float2(0.f, 0.f);
+    if constexpr (kStep == kRestore || kStep == kBackward) z = mul2(decode2(codes[j / 2] >> (16 * (j & 1))), unit);
+    float2 v;
+    if constexpr (kStep == kRestore) {
+      o[j] = pack2(z, T());
+      if (a.out2) {
+        v = acts_of<T, kAct>(z);
+        o2[j] = pack2(kDrop ? mul2(v, keep) : v, T());
+      }
+    } else if constexpr (kStep == kForward) {
+      v = acts_of<T, kAct>(unpack2(w[j], T()));
+      o[j] = pack2(kDrop ? mul2(v, keep) : v, T());
+    } else {
+      v = unpack2(w[j], T());
+      if constexpr (kDrop) v = mul2(v, keep);
+      o[j] = pack2(mul2(v, slopes_of<T, kAct>(z, table)), T());
+    }
+  }
+  if (a.out) store_words(static_cast<T*>(a.out) + index, o);
+  if constexpr (kStep == kRestore)
+    if (a.out2) store_words(static_cast<T*>(a.out2) + index, o2);
+  return true;
+}
+
+template <typename T, int kN, int kStep, int kAct, bool kDrop>
+__device__ __forceinline__ void any_work(const Args& a, const DropRng& rng, const float* table, long row, long col, bool in_row) {
+  if constexpr (kN >= 8)
+    if (work_pairs<T, kN, kStep, kAct, kDrop>(a, rng, table, row, col, in_row)) return;
+  work<T, kN, kStep, kAct, kDrop>(a, rng, row, col, in_row);
+}
+
 // kFlat: whole blocks one after another.  Otherwise a warp goes along a row, 8 rows to a block of threads; kN = 1 takes any alignment.
 template <typename T, int kN, int kStep, int kAct, bool kDrop, bool kFlat>
 __global__ void __launch_bounds__(256) kept_kernel(const __grid_constant__ Args a) {
   const DropRng rng(a.seed + ((kDrop && a.seed_dev) ? *a.seed_dev : 0ull), a.stream_id, a.p);
+  constexpr bool kTable = kN >= 8 && kStep == kBackward && (kAct == 2 || kAct == 3);
+  __shared__ float table[kTable ? kSlopes : 1];
+  if constexpr (kTable) make_slopes<kAct>(table);
   if constexpr (kFlat) {
     const long n = a.width / kN, step = static_cast<long>(gridDim.x) * 256;
     const long first = blockIdx.x * 256L + (threadIdx.x & ~31);
     for (long base = first; base < n; base += step) {
       const long v = base + (threadIdx.x & 31);
-      work<T, kN, kStep, kAct, kDrop>(a, rng, 0, v * kN, v < n);
+      any_work<T, kN, kStep, kAct, kDrop>(a, rng, table, 0, v * kN, v < n);
     }
   } else {
     const int lane = threadIdx.x & 31;
@@ -245,12 +435,24 @@ __global__ void __launch_bounds__(256) kept_kernel(const __grid_constant__ Args 
     for (long row = blockIdx.y * 8L + (threadIdx.x >> 5); row < a.rows; row += gridDim.y * 8L)
       for (long base = blockIdx.x * 32L; base < per; base += gridDim.x * 32L) {
         const long col = (base + lane) * kN;
-        work<T, kN, kStep, kAct, kDrop>(a, rng, row, col, col < a.width);
+        any_work<T, kN, kStep, kAct, kDrop>(a, rng, table, row, col, col < a.width);
       }
   }
 }
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool wide_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; }
+
+// as many blocks as the GPU holds: all of them go through the same share
+const char* launch_flat(void (*kernel)(const Args), const Args& a, int each, cudaStream_t stream) {
+  int held = 0;
+  cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kernel, 256, 0);
+  if (e != cudaSuccess) return cudaGetErrorString(e);
+  const long blocks = (a.width / each + 255) / 256, most = static_cast<long>(held < 1 ? 1 : held) * num_sms();
+  kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, stream>>>(a);
+  e = cudaGetLastError();
+  return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
+}
 
 template <typename T, int kStep, int kAct, bool kDrop>
 const char* launch(const NmtgKept* k) {
@@ -264,8 +466,10 @@ const char* launch(const NmtgKept* k) {
   const bool vectors = a.width % kN == 0 && (a.rows == 1 || a.ld_in % kN == 0) && aligned(a.in) && aligned(a.out) && aligned(a.out2);
   if (vectors && a.width % kBlock == 0 && (a.rows == 1 || a.ld_in == a.width)) {
     a.width *= a.rows; a.blocks *= a.rows; a.rows = 1;
-    const long blocks = (a.width / kN + 255) / 256, most_blocks = 8L * num_sms();
-    kept_kernel<T, kN, kStep, kAct, kDrop, true><<<static_cast<unsigned>(blocks < most_blocks ? blocks : most_blocks), 256, 0, k->stream>>>(a);
+    constexpr int kWide = sizeof(T) == 2 ? 16 : kN;              // 32 bytes of a 16-bit type
+    const bool wide = kWide > kN && wide_aligned(a.in) && wide_aligned(a.out) && wide_aligned(a.out2) && aligned(a.codes);
+    if (wide) return launch_flat(kept_kernel<T, kWide, kStep, kAct, kDrop, true>, a, kWide, k->stream);
+    return launch_flat(kept_kernel<T, kN, kStep, kAct, kDrop, true>, a, kN, k->stream);
   } else {
     const int each = vectors ? kN : 1;
     const long x = (a.blocks * (kBlock / each) + 31) / 32, y = (a.rows + 7) / 8;

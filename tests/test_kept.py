@@ -184,8 +184,8 @@ def test_activation_and_its_slope(dtype, act):
                 want = 0.5 * z.detach().double() * torch.erfc(z.detach().double() * -math.sqrt(0.5))
             # below 2^-14 a 16-bit float's step is 2^-24; the tail of GELU falls to where exp2 is a denormal
             low = 2 ** -25 if dtype == torch.float16 else 2 ** -126
-            if act == "silu":       # exp(-z) is no number beyond 2^128, z < -88.7: the gate, below 2^-128, is then 0, and |z| gate below 89 * 2^-128
-                low = max(low, 2 ** -121)
+            if act == "silu":       # a gate below 2^-126 (z < -87.3) counts as 0: |z| gate is then below 89 * 2^-126
+                low = max(low, 2 ** -119)
             tail = 2 ** -22 * z.detach().double().square().clamp(max=200.0)
             assert ((y.detach().double() - want).abs() <= (HALF[dtype] + part + tail) * want.abs() + low).all()
             dy = torch.randn(rows, width, generator=torch.Generator().manual_seed(2)).to(dtype).to(DEV)
