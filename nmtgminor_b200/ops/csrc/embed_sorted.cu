@@ -1,7 +1,7 @@
 // Gradient of an embedding lookup, each row's sum taken in the order of the tokens: no atomic additions, the same bits every time.
-//   1. order:  the rows sorted by key (stable).  Up to kRankRows rows one kernel counts, for every row, the rows before it in the order
-//      (keys and row numbers packed into 32 bits, N^2 comparisons in registers); more rows take stable radix passes of up to 10 bits
-//      (count, scan, scatter).
+//   1. order:  the rows sorted by key (stable).  Up to kOneTile rows one kernel counts, for every row, the rows before it; up to kPackedRows it does so in
+//      tiles, and a second one finds each row's place in all tiles; more rows take radix passes of up to 10 bits (count, scan, scatter).
+//      (8200 rows: one tile of all 14.6 us; stable passes of one block in its shared memory 31.5; radix passes 29.)
 //   2. reduce: the sorted rows in chunks of 8 or 16, a group of threads each, whatever the words' frequencies are; a sum that begins and
 //      ends in a chunk goes to its row of the gradient, one that crosses an end leaves its part in the workspace.
 //   3. join:   the parts of a sum, in order.
@@ -21,8 +21,10 @@ int num_sms();
 
 namespace {
 
-constexpr int kRankBits = 14, kRankRows = 1 << kRankBits;      // rows that the counting kernel takes
-constexpr int kRankEach = 2, kRankTile = 16 * kRankEach;        // rows of a group of 16 threads, and of a block
+constexpr int kRowBits = 14, kPackedRows = 1 << kRowBits;      // rows whose number fits beside a key into 32 bits
+constexpr int kOneTile = 2048, kMergeTile = 256;               // rows ranked in one go; of a tile where tiles are merged
+constexpr int kRankEach = 2, kRankRows = 16 * kRankEach;       // rows of a group of 16 threads, and of a block
+constexpr int kMergeRows = 64;                                 // rows of a block that merges, 4 threads to each
 constexpr int kTile = 1024;                                    // rows of a block of a radix pass
 constexpr int kDigitBits = 10;                                 // at most
 
@@ -49,54 +51,104 @@ struct Keys {
   }
 };
 
-// part `at` of `of` of the memory to clear, by the blocks from `first` on
+// parts [at, to) of `of` of the memory to clear, by the blocks from `first` on
 struct Clear {
   uint4* p;
   long n;
-  int first, at, of;
+  int first, at, to, of;
   __device__ __forceinline__ bool mine() const { return static_cast<int>(blockIdx.x) >= first; }
   __device__ __forceinline__ void run() const {
-    const long begin = n * at / of, end = n * (at + 1) / of;
+    const long begin = n * at / of, end = n * to / of;
     const long step = static_cast<long>(gridDim.x - first) * blockDim.x;
-    for (long i = begin + (blockIdx.x - first) * static_cast<long>(blockDim.x) + threadIdx.x; i < end; i += step) p[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll 4
+    for (long i = begin + (blockIdx.x - first) * static_cast<long>(blockDim.x) + threadIdx.x; i < end; i += step) __stcs(p + i, make_uint4(0, 0, 0, 0));
   }
+  void next(int blocks, int parts) { first = blocks; at = to; to += parts; }      // the next kernel's share
 };
 
-// order[rank] = row, sorted[rank] = key.  16 threads count for the same rows, each over every 16th group of 4.
-__global__ void __launch_bounds__(256) rank_kernel(const Keys k, int* __restrict__ order, int* __restrict__ sorted, const Clear clear) {
+// Every row's place in its tile: the number of rows of the tile before it, 16 threads to the same rows, each over every 16th group of 4.  Key and row
+// make one number of 32 bits, so that equal keys are in the order of their rows.  Whole: there is one tile, and the places are the rows' own.
+template <bool kWhole>
+__global__ void __launch_bounds__(256) tile_rank_kernel(const Keys k, int tile, uint32_t* __restrict__ tiles, int* __restrict__ order,
+                                                        int* __restrict__ sorted, int* __restrict__ joins, const Clear clear) {
   if (clear.mine()) { clear.run(); return; }
-  extern __shared__ __align__(16) uint32_t all[];
-  const int padded = (k.rows + 63) & ~63;
-  for (int i = threadIdx.x; i < padded; i += 16 * 256) {
-    int key[16];
-    k.of(i, 256, k.rows, key);
+  __shared__ __align__(16) uint32_t all[kWhole ? kOneTile : kMergeTile];
+  const int base = static_cast<int>(blockIdx.x) * kRankRows / tile * tile, count = min(tile, k.rows - base), padded = (count + 63) & ~63;
+  if (blockIdx.x == 0 && threadIdx.x < 2) joins[threadIdx.x] = 0;
+  constexpr int kLoads = (kWhole ? kOneTile : kMergeTile) / 256;
+  int key[kLoads];
+  k.of(base + threadIdx.x, 256, base + count, key);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const int at = i + j * 256;
-      if (at < padded) all[at] = at < k.rows ? static_cast<uint32_t>(key[j]) << kRankBits | at : 0xFFFFFFFFu;
-    }
+  for (int j = 0; j < kLoads; ++j) {
+    const int at = threadIdx.x + j * 256;
+    if (at < padded) all[at] = at < count ? static_cast<uint32_t>(key[j]) << kRowBits | static_cast<uint32_t>(base + at) : 0xFFFFFFFFu;
   }
   __syncthreads();
-  const int lane16 = threadIdx.x & 15, first = blockIdx.x * kRankTile + (threadIdx.x >> 4) * kRankEach;
+  const int lane16 = threadIdx.x & 15, first = static_cast<int>(blockIdx.x) * kRankRows - base + (threadIdx.x >> 4) * kRankEach;
   uint32_t mine[kRankEach];
-  int count[kRankEach] = {};
+  int before[kRankEach] = {};
 #pragma unroll
   for (int j = 0; j < kRankEach; ++j) mine[j] = first + j < padded ? all[first + j] : 0xFFFFFFFFu;
 #pragma unroll 4
   for (int i = lane16; i < padded / 4; i += 16) {
     const uint4 u = reinterpret_cast<const uint4*>(all)[i];
 #pragma unroll
-    for (int j = 0; j < kRankEach; ++j) count[j] += (u.x < mine[j]) + (u.y < mine[j]) + (u.z < mine[j]) + (u.w < mine[j]);
+    for (int j = 0; j < kRankEach; ++j) before[j] += (u.x < mine[j]) + (u.y < mine[j]) + (u.z < mine[j]) + (u.w < mine[j]);
   }
 #pragma unroll
   for (int j = 0; j < kRankEach; ++j) {
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) count[j] += __shfl_xor_sync(0xffffffffu, count[j], o);
-    if (lane16 == 0 && first + j < k.rows) {
-      order[count[j]] = first + j;
-      sorted[count[j]] = static_cast<int>(mine[j] >> kRankBits);
+    for (int o = 8; o > 0; o >>= 1) before[j] += __shfl_xor_sync(0xffffffffu, before[j], o);
+    if (lane16 == 0 && first + j < count) {
+      if constexpr (kWhole) {
+        order[before[j]] = first + j;
+        sorted[before[j]] = static_cast<int>(mine[j] >> kRowBits);
+      } else {
+        tiles[base + before[j]] = mine[j];
+      }
     }
   }
+}
+
+// A row's place among all: in every sorted tile the rows before it, by bisection (4 threads to a row, every fourth tile each)
+__global__ void __launch_bounds__(256) merge_rank_kernel(const uint32_t* __restrict__ tiles, int rows, int* __restrict__ order, int* __restrict__ sorted,
+                                                         const Clear clear) {
+  if (clear.mine()) { clear.run(); return; }
+  extern __shared__ __align__(16) uint32_t tile_of[];
+  const int count = (rows + kMergeTile - 1) / kMergeTile;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < count * kMergeTile; i += 256) tile_of[i] = i < rows ? tiles[i] : 0xFFFFFFFFu;
+  __syncthreads();
+  const int at = blockIdx.x * kMergeRows + (threadIdx.x >> 2);
+  if (at >= rows) return;
+  const uint32_t mine = tile_of[at];
+  int place = 0;
+#pragma unroll 4
+  for (int t = threadIdx.x & 3; t < count; t += 4) {
+    const uint32_t* const tile = tile_of + t * kMergeTile;
+    int before = 0;
+#pragma unroll
+    for (int step = kMergeTile / 2; step > 0; step >>= 1) before += tile[before + step - 1] < mine ? step : 0;
+    place += before + (tile[before] < mine);
+  }
+  const uint32_t group = 0xFu << (threadIdx.x & 28);
+  place += __shfl_xor_sync(group, place, 1);
+  place += __shfl_xor_sync(group, place, 2);
+  if ((threadIdx.x & 3) == 0) {
+    order[place] = static_cast<int>(mine & (kPackedRows - 1));
+    sorted[place] = static_cast<int>(mine >> kRowBits);
+  }
+}
+
+// Lanes with the same digit among those with one (d >= 0), a vote for each bit: a match of whole words takes several times as long.
+__device__ __forceinline__ uint32_t same_digit(int d, int bits) {
+  uint32_t same = __ballot_sync(0xffffffffu, d >= 0);
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (d >> b) & 1;
+    const uint32_t m = __ballot_sync(0xffffffffu, one);
+    same &= one ? m : ~m;
+  }
+  return same;
 }
 
 // ---- radix passes ----------------------------------------------------------------------------------------------------------
@@ -106,7 +158,7 @@ struct Pass {
   int* key_out;
   int* row_out;
   int* counts;              // [bins][tiles]
-  int shift, bins, tiles;
+  int shift, digit, bins, tiles;
 };
 
 template <int kN> __device__ __forceinline__ void keys_at(const Keys& k, const Pass& p, int i, int step, int end, int (&key)[kN]) {
@@ -115,8 +167,9 @@ template <int kN> __device__ __forceinline__ void keys_at(const Keys& k, const P
   for (int j = 0; j < kN; ++j) key[j] = i + j * step < end ? p.key[i + j * step] : 0;
 }
 
-__global__ void __launch_bounds__(256) radix_count_kernel(const Keys k, const Pass p, const Clear clear) {
+__global__ void __launch_bounds__(256) radix_count_kernel(const Keys k, const Pass p, int* __restrict__ joins, const Clear clear) {
   if (clear.mine()) { clear.run(); return; }
+  if (blockIdx.x == 0 && threadIdx.x < 2) joins[threadIdx.x] = 0;
   __shared__ int bins[1 << kDigitBits];
   for (int b = threadIdx.x; b < p.bins; b += 256) bins[b] = 0;
   __syncthreads();
@@ -193,7 +246,7 @@ __global__ void __launch_bounds__(256) radix_scatter_kernel(const Keys k, const 
 #pragma unroll
   for (int j = 0; j < kRounds; ++j) {
     const int i = begin + j * 32 + lane, d = i < end ? (key[j] >> p.shift) & (p.bins - 1) : -1;
-    const uint32_t same = __match_any_sync(0xffffffffu, d);
+    const uint32_t same = same_digit(d, p.digit);
     if (d >= 0 && (same & below) == 0) mine[d] += __popc(same);
     __syncwarp();
   }
@@ -207,7 +260,7 @@ __global__ void __launch_bounds__(256) radix_scatter_kernel(const Keys k, const 
 #pragma unroll
   for (int j = 0; j < kRounds; ++j) {
     const int i = begin + j * 32 + lane, d = i < end ? (key[j] >> p.shift) & (p.bins - 1) : -1;
-    const uint32_t same = __match_any_sync(0xffffffffu, d);
+    const uint32_t same = same_digit(d, p.digit);
     const int place = d >= 0 ? mine[d] + __popc(same & below) : 0;
     __syncwarp();
     if (d >= 0) {
@@ -236,6 +289,7 @@ struct Sum {
   const void* dy;
   void* grad;
   float* parts;             // [chunks][2][width]: of a sum that began before the chunk, of one that goes on behind it
+  int* joins;               // chunks in which a sum begins that goes on behind them: numbers of those that end in the next and of the others; both lists
   int rows, keys, width, chunk, chunks;
   float scale, p;
   unsigned long long seed, stream_id;
@@ -341,25 +395,38 @@ __global__ void __launch_bounds__(256, 3) reduce_kernel(const Sum s) {
         }
       }
     }
-    flush(key, began_before, with_key == s.chunk && key == after);
+    const bool goes_on = with_key == s.chunk && key == after;
+    flush(key, began_before, goes_on);
+    if (base == 0 && threadIdx.x == 0 && goes_on && !began_before) {
+      const int at = begin + 2 * s.chunk;                       // behind the next chunk
+      const bool is_long = at < s.rows && s.sorted[at - 1] == key && s.sorted[at] == key;
+      s.joins[2 + (is_long ? s.chunks : 0) + atomicAdd(s.joins + is_long, 1)] = c;
+    }
   }
 }
 
-// A block to each chunk in which a sum begins that goes on behind it (and to a share of the columns): its parts, in 8 runs one after another, the
-// runs in order.  One look tells whether there is one; the sum's end is found by 32 looks at a time.
+// The sums that begin in a chunk and go on behind it.  Most end in the next chunk: two parts, a warp to each sum.  The others take a block and a share
+// of the columns each, the parts in 8 runs one after another, the runs in order; their end is found by 32 looks at a time.  (The list's order does not
+// matter: every sum is joined by itself.)
 template <typename T, int kN, bool kAdd>
 __global__ void __launch_bounds__(256) join_kernel(const Sum s) {
   constexpr int kRuns = 8, kCols = 32;
   __shared__ float runs[kRuns][kCols * kN];
-  const int x = threadIdx.x & 31, run = threadIdx.x >> 5, c = blockIdx.x;
-  {
-    const int begin = c * s.chunk, end = begin + s.chunk, places[4] = {end - 1, end, begin, begin - 1};
-    int seen[4];
+  const int x = threadIdx.x & 31, run = threadIdx.x >> 5, sums = s.joins[0], long_sums = s.joins[1];
+  for (int i = (blockIdx.y * gridDim.x + blockIdx.x) * kRuns + run; i < sums; i += gridDim.x * gridDim.y * kRuns) {
+    const int c = s.joins[2 + i], key = s.sorted[(c + 1) * s.chunk];
+    const float* const first = s.parts + (static_cast<long>(c) * 2 + 1) * s.width;
+    const float* const second = s.parts + static_cast<long>(c + 1) * 2 * s.width;
+#pragma unroll 2
+    for (int col = x * kN; col < s.width; col += 32 * kN) {
+      float acc[kN];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) seen[j] = places[j] >= 0 && places[j] < s.rows ? s.sorted[places[j]] : -1;
-    const int key = seen[0];
-    if (key < 0 || key >= s.keys || seen[1] != key || (seen[2] == key && seen[3] == key)) return;
-    // a sum that begins here
+      for (int j = 0; j < kN; ++j) acc[j] = first[col + j] + second[col + j];
+      to_grad<T, kN, kAdd>(s, key, col, acc);
+    }
+  }
+  for (int i = blockIdx.x; i < long_sums; i += gridDim.x) {
+    const int c = s.joins[2 + s.chunks + i], key = s.sorted[(c + 1) * s.chunk];
     int lo = (c + 1) * s.chunk, hi = s.rows;                    // the first place behind the sum's last is in [lo, hi]
     while (lo < hi) {
       const int step = (hi - lo + 31) / 32, at = lo + x * step;
@@ -379,8 +446,8 @@ __global__ void __launch_bounds__(256) join_kernel(const Sum s) {
       for (int j = 0; j < kN; ++j) acc[j] = 0.f;
       if (col < s.width) {
 #pragma unroll 4
-        for (int i = from; i < to; ++i) {
-          const float* part = s.parts + (static_cast<long>(c + i) * 2 + (i == 0 ? 1 : 0)) * s.width + col;
+        for (int q = from; q < to; ++q) {
+          const float* part = s.parts + (static_cast<long>(c + q) * 2 + (q == 0 ? 1 : 0)) * s.width + col;
           if constexpr (kN % 4 == 0) {
 #pragma unroll
             for (int j = 0; j < kN; j += 4) {
@@ -454,8 +521,8 @@ const char* sums(const Sum& s, cudaStream_t stream) {
   reduce_kernel<T, kN, kDrop, kAdd><<<dim3((s.chunks + block.y - 1) / block.y), block, smem, stream>>>(s);
   e = cudaGetLastError();
   if (e != cudaSuccess || s.chunks < 2) return problem(e);
-  const int cols = (s.width + 32 * kN - 1) / (32 * kN);
-  join_kernel<T, kN, kAdd><<<dim3(s.chunks, cols < 8 ? cols : 8), 256, 0, stream>>>(s);
+  const int cols = (s.width + 32 * kN - 1) / (32 * kN), across = cols < 8 ? cols : 8, want = (s.chunks + 7) / 8, most = 16 * num_sms() / across;
+  join_kernel<T, kN, kAdd><<<dim3(want < most ? want : most, across), 256, 0, stream>>>(s);
   return problem(cudaGetLastError());
 }
 
@@ -491,7 +558,7 @@ using namespace b200;
 
 long nmtg_embed_grad_workspace(int rows, int keys, int width) {
   const long n = rows, chunks = (n + chunk_of(rows) - 1) / chunk_of(rows), tiles = (n + kTile - 1) / kTile;
-  return 4 * up16(4 * n) + up16(4 * tiles << kDigitBits) + up16(8 * chunks * width);
+  return 4 * up16(4 * n) + up16(4 * tiles << kDigitBits) + up16(4 * (2 * chunks + 2)) + up16(8 * chunks * width);
 }
 
 const char* nmtg_embed_grad(const NmtgEmbedGrad* d) {
@@ -508,47 +575,55 @@ const char* nmtg_embed_grad(const NmtgEmbedGrad* d) {
   for (int i = 0; i < 2; ++i) { key[i] = take(4L * n); row[i] = take(4L * n); }
   const int tiles = (n + kTile - 1) / kTile;
   int* counts = take(4L * tiles << kDigitBits);
+  const int chunk = chunk_of(n), chunks = (n + chunk - 1) / chunk;
+  int* joins = take(4L * (2 * chunks + 2));
   // whole vectors are cleared beside the sort, the last bytes by themselves
-  Clear clear = {static_cast<uint4*>(d->accumulate ? nullptr : d->grad), bytes / 16, 0, 0, 1};
+  Clear clear = {static_cast<uint4*>(d->accumulate ? nullptr : d->grad), bytes / 16, 0, 0, 0, 1};
   if (bytes % 16) {
     const cudaError_t e = cudaMemsetAsync(static_cast<char*>(d->grad) + bytes / 16 * 16, 0, bytes % 16, stream);
     if (e != cudaSuccess) return cudaGetErrorString(e);
   }
-  const long want = (clear.n + 1023) / 1024, most = 4L * num_sms();
+  const long want = (clear.n + 1023) / 1024, most = 6L * num_sms();
   const int extra = static_cast<int>(want < most ? want : most);
   int last = 0;
   cudaError_t e;
-  if (n <= kRankRows && bits + kRankBits <= 32) {
-    clear.first = (n + kRankTile - 1) / kRankTile;
-    const int smem = ((n + 63) & ~63) * 4;
-    if (smem > 48 * 1024 && (e = cudaFuncSetAttribute(rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRankRows * 4)) != cudaSuccess)
+  const int blocks = (n + kRankRows - 1) / kRankRows;
+  if (n <= kOneTile && bits + kRowBits <= 32) {
+    clear.next(blocks, 1);
+    tile_rank_kernel<true><<<blocks + extra, 256, 0, stream>>>(k, kOneTile, nullptr, row[0], key[0], joins, clear);
+    if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
+  } else if (n <= kPackedRows && bits + kRowBits <= 32) {
+    const int smem = (n + kMergeTile - 1) / kMergeTile * kMergeTile * 4;
+    if ((e = cudaFuncSetAttribute(merge_rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPackedRows * 4)) != cudaSuccess)
       return cudaGetErrorString(e);
-    rank_kernel<<<clear.first + extra, 256, smem, stream>>>(k, row[0], key[0], clear);
+    uint32_t* const tiles = reinterpret_cast<uint32_t*>(key[1]);
+    clear.of = 2;
+    clear.next(blocks, 1);
+    tile_rank_kernel<false><<<blocks + extra, 256, 0, stream>>>(k, kMergeTile, tiles, nullptr, nullptr, joins, clear);
+    if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
+    clear.next((n + kMergeRows - 1) / kMergeRows, 1);
+    merge_rank_kernel<<<clear.first + extra, 256, smem, stream>>>(tiles, n, row[0], key[0], clear);
     if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
   } else {
     const int passes = (bits + kDigitBits - 1) / kDigitBits, digit = (bits + passes - 1) / passes;
     const size_t smem = 8 * sizeof(int) << digit;
-    clear.of = 3 * passes;
+    clear.of = 5 * passes;               // the scan, one block and short, beside a fifth
     for (int i = 0; i < passes; ++i) {
-      Pass p = {i ? key[(i - 1) & 1] : nullptr, i ? row[(i - 1) & 1] : nullptr, key[i & 1], row[i & 1], counts, i * digit, 1 << digit, tiles};
-      clear.first = tiles;
-      radix_count_kernel<<<tiles + extra, 256, 0, stream>>>(k, p, clear);
+      Pass p = {i ? key[(i - 1) & 1] : nullptr, i ? row[(i - 1) & 1] : nullptr, key[i & 1], row[i & 1], counts, i * digit, digit, 1 << digit, tiles};
+      clear.next(tiles, 2);
+      radix_count_kernel<<<tiles + extra, 256, 0, stream>>>(k, p, joins, clear);
       if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
-      ++clear.at;
-      clear.first = 1;
+      clear.next(1, 1);
       radix_scan_kernel<<<1 + (extra + 3) / 4, 1024, 0, stream>>>(counts, tiles << digit, clear);
       if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
-      ++clear.at;
-      clear.first = tiles;
+      clear.next(tiles, 2);
       radix_scatter_kernel<<<tiles + extra, 256, smem, stream>>>(k, p, clear);
       if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
-      ++clear.at;
       last = i & 1;
     }
   }
-  Sum s = {row[last], key[last], d->dy, d->grad, nullptr, n, d->keys, d->width, chunk_of(n), 0, d->scale, d->p, d->seed, d->stream_id, d->seed_dev};
-  s.chunks = (n + s.chunk - 1) / s.chunk;
-  s.parts = reinterpret_cast<float*>(take(8L * s.chunks * d->width));
+  float* const parts = reinterpret_cast<float*>(take(8L * chunks * d->width));
+  const Sum s = {row[last], key[last], d->dy, d->grad, parts, joins, n, d->keys, d->width, chunk, chunks, d->scale, d->p, d->seed, d->stream_id, d->seed_dev};
   if (d->dtype == 0) return sums_type<float>(s, d->accumulate, stream);
   if (d->dtype == 1) return sums_type<__nv_bfloat16>(s, d->accumulate, stream);
   if (d->dtype == 2) return sums_type<__half>(s, d->accumulate, stream);
