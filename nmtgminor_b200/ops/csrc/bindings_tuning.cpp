@@ -70,13 +70,18 @@ Tensor workspace(const Tensor& logits, NmtgRows& r, int pairs) {
   return t;
 }
 
-std::tuple<Tensor, Tensor> row_scores(const Tensor& logits, const Tensor& labels, int64_t pad, double temperature, bool keep_stat) {
+// -> log-probabilities, and where `keep_stat` what their gradient needs
+std::tuple<Tensor, OptTensor> row_scores(const Tensor& logits, const Tensor& labels, int64_t pad, double temperature, bool keep_stat) {
   NmtgRows r = rows_of(logits, labels, pad, temperature);
   c10::cuda::CUDAGuard guard(logits.device());
   const auto f32 = logits.options().dtype(at::kFloat).requires_grad(false);
-  Tensor lp = at::empty({r.rows}, f32), stat = at::empty({keep_stat ? r.rows : 0, 2}, f32);
+  Tensor lp = at::empty({r.rows}, f32);
+  OptTensor stat;
+  if (keep_stat) {
+    stat = at::empty({r.rows, 2}, f32);
+    r.stat = reinterpret_cast<float2*>(stat->data_ptr<float>());
+  }
   r.logprobs = lp.data_ptr<float>();
-  r.stat = keep_stat ? reinterpret_cast<float2*>(stat.data_ptr<float>()) : nullptr;
   const Tensor work = workspace(logits, r, 0);
   ck(nmtg_row_scores(&r, cur_stream()));
   return {lp, stat};
@@ -374,7 +379,7 @@ Tensor plain_rows(const Tensor& t) {
 struct ScoresNode : Function<ScoresNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, int64_t pad, double temperature) {
     auto [lp, stat] = row_scores(logits, labels, pad, temperature, true);
-    ctx->save_for_backward({logits, labels, stat});
+    ctx->save_for_backward({logits, labels, *stat});
     ctx->saved_data["pad"] = pad;
     ctx->saved_data["temperature"] = temperature;
     return lp;

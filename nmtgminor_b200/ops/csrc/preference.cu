@@ -4,8 +4,8 @@
 // Each loss is a function of the lp of its rows, so a row's gradient is one coefficient times d lp / d x.
 //
 // rows_kernel takes a piece of a row at a time: its sums, or its gradient, or for the policy loss of rows that a block holds both, the logits
-// read once.  The scores, the paired loss and the policy loss of longer rows are two passes, sums and then gradients, with a small kernel between
-// that makes rows of the pieces and coefficients of the rows.  (Both passes at once, the gradients some rows behind the sums so
+// read once.  Scores of rows in one piece are complete with it.  The paired loss, and the scores and the policy loss of longer rows, are two
+// passes, sums and then gradients, with a small kernel between that makes rows of the pieces and coefficients of the rows.  (Both passes at once, the gradients some rows behind the sums so
 // that they would find the logits in L2, were built and measured: 353 us against 272 for 8200 rows of 32000 in bf16.  The coefficient of a pair
 // comes so late that most blocks wait for it.)
 // Bound by memory in 32 bits and in every gradient pass; the sums of 16-bit logits are bound by exponentials, 16 a cycle and SM.
@@ -303,6 +303,7 @@ __global__ void __launch_bounds__(kCompute + 32, kCompute == kBlock ? 3 : 1) row
   if (warp == kWarps) {
     // ------------------------------------------------------------------------------------------------ the last warp
     const float scale = a.scale_at ? *a.scale_at * a.scale : a.scale;
+    const bool whole = kMode == kLocal || (kMode == kScores && !a.w.part);      // an item is a row, and its log-probability wanted
     // What an entry needs comes by asynchronous copies, so that this warp never waits for memory: at step i the label of entry i + kLead + 3, at step
     // i + 2, when its label is there and the entry is published, its logit and the numbers of its row.
     // Items are handed out one by one, asked for a step ahead: SMs do not get at memory equally fast, and equal shares would wait for the slowest
@@ -330,10 +331,12 @@ __global__ void __launch_bounds__(kCompute + 32, kCompute == kBlock ? 3 : 1) row
       }
       ring[i & (kRing - 1)] = e;
       if (e.label >= 0) {
-        if constexpr (kMode == kLocal) {
+        if (whole) {
           const uintptr_t at = reinterpret_cast<uintptr_t>(x0 + static_cast<long>(e.row) * a.ld + e.label);
           m.upper = at & 2;
           copy4(&m.word, reinterpret_cast<const void*>(at & ~static_cast<uintptr_t>(3)));
+        }
+        if constexpr (kMode == kLocal) {
           copy4(&m.old, a.policy.old_logprobs + e.row);
           copy4(&m.adv, a.policy.advantages + e.row);
           if (a.policy.ref_logprobs) copy4(&m.ref, a.policy.ref_logprobs + e.row);
@@ -389,18 +392,18 @@ __global__ void __launch_bounds__(kCompute + 32, kCompute == kBlock ? 3 : 1) row
             join_lanes(m, sum, a.k);
           }
           if (lane == 0) {
-            if constexpr (kMode == kScores) {
+            if (!whole) {
               a.w.part[static_cast<long>(row) * a.pieces + before.piece] = make_float2(m, sum);
             } else {
-              LogProb lp = {0.f, 0.f};
-              float c = 0.f;
-              if (real) {
-                lp = log_probability(logit_of(letter), m, sum, a.inv_t);
-                c = policy_coef(a, lp, letter.old, letter.adv, letter.ref) * a.inv_t * scale;
-              }
-              bc[(i - 1) & 1] = make_float4(m, __fdividef(c, sum), c, 0.f);
+              const LogProb lp = real ? log_probability(logit_of(letter), m, sum, a.inv_t) : LogProb{0.f, 0.f};
               a.logprobs[row] = lp.hi;
-              a.w.lp[row] = lp.wide();
+              if constexpr (kMode == kScores) {
+                if (a.stat) a.stat[row] = real ? make_float2(m, sum) : make_float2(0.f, 1.f);
+              } else {
+                const float c = real ? policy_coef(a, lp, letter.old, letter.adv, letter.ref) * a.inv_t * scale : 0.f;
+                bc[(i - 1) & 1] = make_float4(m, __fdividef(c, sum), c, 0.f);
+                a.w.lp[row] = lp.wide();
+              }
             }
           }
         }
@@ -828,16 +831,17 @@ const char* launch_rows(const Args& from, cudaStream_t stream) {
 template <typename T> constexpr int warp_row() { return 32 * kVecs * Num<T>::kE; }       // elements that a warp holds
 
 // Pieces of a row: as many as hold it; for few rows more, of 4 KB at least, until every block that the GPU holds has one.
-#ifndef NMTG_PIECE
-#define NMTG_PIECE 8
-#endif
 int pieces_of(int rows, int vocab, int dtype) {
   const int vectors = vocab / (dtype == 0 ? 4 : 8);
-  int n = (vectors + kBlock * NMTG_PIECE - 1) / (kBlock * NMTG_PIECE);
+  int n = (vectors + kBlock * kVecs - 1) / (kBlock * kVecs);
   if (n < 1) n = 1;
   while (2L * n * rows <= 2 * num_sms() && vectors >= 512 * n) n *= 2;
   return n;
 }
+
+// Scores of no more rows than there are SMs, each no longer than a block holds, are one launch of a block to a row: (37 rows of 32000 in bf16,
+// call by call: FIXME us, in pieces FIXME)
+bool few_rows(int rows, int vocab, int dtype) { return rows <= num_sms() && vocab <= kWide * kVecs * (dtype == 0 ? 4 : 8); }
 
 template <typename T, int kMode>
 const char* launch_short(const Args& a, cudaStream_t stream) {
@@ -855,11 +859,20 @@ const char* launch_pass(Args a, int dtype, cudaStream_t stream) {
     a.each = a.vocab / (16 / size);
     return dtype == 0 ? launch_short<float, kMode>(a, stream) : dtype == 1 ? launch_short<__nv_bfloat16, kMode>(a, stream) : launch_short<__half, kMode>(a, stream);
   }
+  const bool between = a.pairs.pairs > 0 || a.policy.old_logprobs;         // the paired and the policy loss go on with the sums of the pieces
+  if (kMode == kScores && !between && few_rows(a.rows, a.vocab, dtype)) {
+    a.pieces = 1;
+    a.each = a.vocab / (16 / size);
+    a.w.part = nullptr;
+    return dtype == 0 ? launch_rows<float, kWide, kScores>(a, stream) : dtype == 1 ? launch_rows<__nv_bfloat16, kWide, kScores>(a, stream)
+                                                                                   : launch_rows<__half, kWide, kScores>(a, stream);
+  }
   a.pieces = pieces_of(a.rows, a.vocab, dtype);
   a.each = (a.vocab / (16 / size) + a.pieces - 1) / a.pieces;
+  if (a.pieces == 1 && !between) a.w.part = nullptr;
   const char* err = dtype == 0 ? launch_rows<float, kBlock, kMode>(a, stream) : dtype == 1 ? launch_rows<__nv_bfloat16, kBlock, kMode>(a, stream)
                                                                                           : launch_rows<__half, kBlock, kMode>(a, stream);
-  if (kMode != kScores || err || a.pairs.pairs > 0) return err;
+  if (kMode != kScores || err || a.pairs.pairs > 0 || !a.w.part) return err;
   const int blocks = (a.rows + 127) / 128;
   if (dtype == 0) whole_rows_kernel<float><<<blocks, 128, 0, stream>>>(a);
   else if (dtype == 1) whole_rows_kernel<__nv_bfloat16><<<blocks, 128, 0, stream>>>(a);
