@@ -15,6 +15,7 @@
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <climits>
 #include <stdint.h>
 #include "b200_ptx.cuh"
 #include "tuning_api.h"
@@ -28,14 +29,16 @@ namespace {
 constexpr int kVecs = 8;              // 16-byte vectors of an item that a thread holds
 constexpr int kSlots = 3;             // items in shared memory or on their way there
 constexpr int kRing = 8;              // entries of work known: one behind, kSlots + 3 ahead, and that in hand
+constexpr int kFirst = 6;             // items of a block that it need not ask for
 constexpr int kBlock = 256, kWide = 512;      // threads of a block for the elements; two or three blocks to an SM, and one
 
 // kScores: sums of pieces.  kGrad: gradients from `stat` or `part` and a coefficient.  kLocal: the policy loss of rows that one block holds.
 enum Mode { kScores = 0, kGrad = 1, kLocal = 2 };
 
-struct State { int ticket, pairs_done; };
+struct State { int tickets[2], pairs_done; };      // items asked for in the two passes
 struct Work {
   State* state;
+  int* ticket;              // of this pass, 0 before it; null where every item has its block or warp
   float2* part;             // [rows][pieces] largest logit, sum of exponentials
   float2* stat;             // [rows] the same of a row
   float* coef;              // [2 pairs] or [rows]: d loss / d lp
@@ -230,6 +233,18 @@ __device__ __forceinline__ int single_at(const Shape& s, int thread, int piece, 
   return -1;
 }
 
+// a row's sums from those of its pieces
+__device__ __forceinline__ void join_pieces(const Args& a, int row, float& m, float& s) {
+  const float2* const at = a.w.part + static_cast<long>(row) * a.pieces;
+  for (int p = 0; p < a.pieces; p += 8) {
+    float2 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = p + j < a.pieces ? at[p + j] : make_float2(-INFINITY, 0.f);      // several on their way at a time
+#pragma unroll
+    for (int j = 0; j < 8; ++j) join(m, s, v[j].x, v[j].y, a.k);
+  }
+}
+
 // loss of pair p from the sums of its two sequences: one lane
 __device__ __noinline__ void pair_loss(const Args& a, int p, double sw, double sl, int nw, int nl) {
   const NmtgPairs& q = a.pairs;
@@ -306,11 +321,11 @@ __global__ void __launch_bounds__(kCompute + 32, kCompute == kBlock ? 3 : 1) row
     const bool whole = kMode == kLocal || (kMode == kScores && !a.w.part);      // an item is a row, and its log-probability wanted
     // What an entry needs comes by asynchronous copies, so that this warp never waits for memory: at step i the label of entry i + kLead + 3, at step
     // i + 2, when its label is there and the entry is published, its logit and the numbers of its row.
-    // Items are handed out one by one, asked for a step ahead: SMs do not get at memory equally fast, and equal shares would wait for the slowest
-    // (sums of 8200 rows of 32000: most blocks done after 87 us, the last after 111).
+    // A block's first kFirst items are its own, the others are handed out one by one, asked for a step ahead: SMs do not get at memory equally fast,
+    // and equal shares would wait for the slowest (sums of 8200 rows of 32000: most blocks done after 87 us, the last after 111).
     const auto next_number = [&](int i) -> int {              // of entry i
-      if (a.w.state) return atomicAdd(&a.w.state->ticket, 1);
-      return i == 0 ? static_cast<int>(blockIdx.x) : a.rows * a.pieces;      // an item to each block
+      if (i < kFirst) return static_cast<int>(blockIdx.x) + i * static_cast<int>(gridDim.x);
+      return a.w.ticket ? kFirst * static_cast<int>(gridDim.x) + atomicAdd(a.w.ticket, 1) : a.rows * a.pieces;
     };
     const auto ask = [&](int i, int number) {                 // lane 0
       const int q = a.pieces == 1 ? number : number / a.pieces;
@@ -525,6 +540,129 @@ __global__ void __launch_bounds__(kCompute + 32, kCompute == kBlock ? 3 : 1) row
   copies_wait<0>();
 }
 
+// Sums of pieces of 16-bit rows, a warp to a piece: no barrier, each lane with a running maximum of its own and its own logits on their way by
+// asynchronous copies, so that one warp's exponentials run while another's wait.  A block to a piece (above) keeps neither the memory nor the exponentials
+// busy all the time: 8200 rows of 32000 in bf16 took 109 us there and take 95 here (floor 81).  32-bit rows have half the exponentials to a byte and
+// are at the memory's rate there (159 us; here 165 to 173).
+constexpr int kSumWarps = 16, kSumBlocks = 2;               // warps of a block, blocks to an SM
+constexpr int kSumVecs = 4, kSumStages = 3, kSumStage = 32 * kSumVecs;      // vectors of a lane in a stage, stages on their way, vectors of a stage
+constexpr int kSumRing = 8;                                 // items known: fewer than kSumStages + 3
+template <typename T>
+__global__ void __launch_bounds__(kSumWarps * 32, kSumBlocks) sums_kernel(const __grid_constant__ Args a) {
+  constexpr int kE = Num<T>::kE;
+  extern __shared__ __align__(16) uint4 slots[];            // [kSumWarps][kSumStages][kSumStage]
+  __shared__ int4 rings[kSumWarps][kSumRing];                      // row, piece, label
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const T* const x0 = static_cast<const T*>(a.x);
+  uint4* const mine = slots + warp * (kSumStages * kSumStage) + lane;
+  int4* const ring = rings[warp];
+  const int items = a.rows * a.pieces, warps = static_cast<int>(gridDim.x) * kSumWarps;
+  const bool singles = !a.aligned || a.vocab % kE != 0;
+
+  // The copying side: lane 0 has the next item's number and label and the number after it, asked for an item ahead.  Rows of padding are passed over.
+  int number = static_cast<int>(blockIdx.x) + warp * static_cast<int>(gridDim.x), after = number + warps;
+  int label = -1;
+  const auto label_of = [&](int n) -> int {
+    if (n >= items) return -1;
+    const int row = a.pieces == 1 ? n : n / a.pieces;
+    const int64_t y = a.labels[row];
+    return y == a.pad || y < 0 || y >= a.vocab ? -1 : static_cast<int>(y);
+  };
+  if (lane == 0) label = label_of(number);
+  int filled = 0, at = 0, end = 0, prow = 0;                // entries of `ring`; the next vectors to copy, -1: none
+  const uint4* from = nullptr;
+  const auto fetch = [&]() {
+    for (;;) {
+      const int n = __shfl_sync(0xffffffffu, number, 0), y = __shfl_sync(0xffffffffu, label, 0);
+      if (n >= items) { prow = -1; break; }
+      if (lane == 0) {
+        number = after;
+        label = label_of(number);
+        after = a.w.ticket ? 2 * warps + atomicAdd(a.w.ticket, 1) : items;
+      }
+      if (y < 0) continue;
+      prow = a.pieces == 1 ? n : n / a.pieces;
+      const int piece = n - prow * a.pieces;
+      const T* x = x0 + static_cast<long>(prow) * a.ld;
+      const Shape s = shape_of(a, x, piece);
+      from = reinterpret_cast<const uint4*>(x + s.head) + lane;
+      at = s.v0;
+      end = s.v1;
+      if (lane == 0) ring[filled & (kSumRing - 1)] = make_int4(prow, piece, y, 0);
+      ++filled;
+      return;
+    }
+    if (lane == 0) ring[filled & (kSumRing - 1)] = make_int4(-1, 0, 0, 0);
+    ++filled;
+  };
+  int slot = 0;
+  const auto issue = [&](int to) {
+    if (prow >= 0) {
+#pragma unroll
+      for (int j = 0; j < kSumVecs; ++j)
+        if (at + lane + j * 32 < end) copy16(mine + to * kSumStage + j * 32, from + at + j * 32);
+      at += kSumStage;
+      if (at >= end) fetch();
+    }
+    copies_end();
+  };
+  fetch();
+#pragma unroll
+  for (int i = 0; i < kSumStages; ++i) issue(i);
+  for (int i = 0;; ++i) {
+    __syncwarp();
+    const int4 now = ring[i & (kSumRing - 1)];
+    if (now.x < 0) break;
+    const T* const x = x0 + static_cast<long>(now.x) * a.ld;
+    const Shape s = shape_of(a, x, now.y);
+    float one = -INFINITY, xy = 0.f;
+    if (singles) {
+      const int e = single_at<T>(s, lane, now.y, a.pieces);
+      if (e >= 0) one = Num<T>::get(x[e]);
+    }
+    if (!a.w.part) xy = Num<T>::get(x[now.z]);
+    float m = -INFINITY, sum = 0.f;
+    int v = s.v0;
+    do {
+      copies_wait<kSumStages - 1>();
+      const int left = s.v1 - v - lane;
+      uint4 raw[kSumVecs];
+#pragma unroll
+      for (int j = 0; j < kSumVecs; ++j)
+        raw[j] = j * 32 < left ? mine[slot * kSumStage + j * 32] : make_uint4(Num<T>::kLow, Num<T>::kLow, Num<T>::kLow, Num<T>::kLow);
+      float top = m;
+#pragma unroll
+      for (int j = 0; j < kSumVecs; ++j) top = fmaxf(top, Num<T>::largest(raw[j]));
+      const float base = top == -INFINITY ? 0.f : top;
+      float2 total[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int j = 0; j < kSumVecs; ++j) {
+        if (j > 0 && v + j * 32 >= s.v1) break;
+        float2 e[kE / 2];
+        exps<T>(raw[j], -base, a.k, e);
+#pragma unroll
+        for (int q = 0; q < kE / 2; ++q) total[q & 1] = add2(total[q & 1], e[q]);
+      }
+      total[0] = add2(total[0], total[1]);
+      sum = fmaf(sum, ex2((m - base) * a.k), total[0].x + total[0].y);      // a stage's sum at a time: few roundings in a row
+      m = top;
+      issue(slot);
+      slot = slot + 1 == kSumStages ? 0 : slot + 1;
+      v += kSumStage;
+    } while (v < s.v1);
+    if (singles) join(m, sum, one, one == -INFINITY ? 0.f : 1.f, a.k);
+    join_lanes(m, sum, a.k);
+    if (lane == 0) {
+      if (a.w.part) a.w.part[static_cast<long>(now.x) * a.pieces + now.y] = make_float2(m, sum);
+      else {
+        a.logprobs[now.x] = log_probability(xy, m, sum, a.inv_t).hi;
+        if (a.stat) a.stat[now.x] = make_float2(m, sum);
+      }
+    }
+  }
+  copies_wait<0>();
+}
+
 // Rows that a warp holds (up to 8 vectors a lane): a warp to a row, everything in registers.  kScores, kGrad, kLocal.
 template <typename T, int kMode>
 __global__ void __launch_bounds__(256) short_rows_kernel(const __grid_constant__ Args a) {
@@ -611,7 +749,7 @@ __global__ void __launch_bounds__(1024) pairs_setup_kernel(const __grid_constant
   const auto none = [&](int begin, int end) {                // rows outside every sequence
     for (int r = begin + static_cast<int>(blockIdx.x) * 1024 + t; r < end; r += static_cast<int>(gridDim.x) * 1024) { a.w.seq[r] = -1; a.w.label[r] = -1; }
   };
-  if (blockIdx.x == 0 && t == 0) *a.w.state = State{0, 0};
+  if (blockIdx.x == 0 && t == 0) *a.w.state = State{{0, 0}, 0};
   int carry = 0;
   for (int base = 0; base < n; base += 1024) {
     int v = base + t < n ? min(max(a.pairs.cu[base + t], 0), a.rows) : 0;
@@ -660,10 +798,7 @@ __global__ void __launch_bounds__(128) pairs_kernel(const __grid_constant__ Args
       m = a.stat[r].x;
       s = a.stat[r].y;
     } else {
-      for (int q = 0; q < a.pieces; ++q) {
-        const float2 v = a.w.part[static_cast<long>(r) * a.pieces + q];
-        join(m, s, v.x, v.y, a.k);
-      }
+      join_pieces(a, r, m, s);
       a.w.stat[r] = make_float2(m, s);
     }
     const double lp = log_probability(xy, m, s, a.inv_t).wide();
@@ -715,10 +850,7 @@ __global__ void __launch_bounds__(128) whole_rows_kernel(const __grid_constant__
   LogProb lp = {0.f, 0.f};
   if (real) {
     const float xy = Num<T>::get(static_cast<const T*>(a.x)[static_cast<long>(row) * a.ld + y]);
-    for (int p = 0; p < a.pieces; ++p) {
-      const float2 v = a.w.part[static_cast<long>(row) * a.pieces + p];
-      join(m, s, v.x, v.y, a.k);
-    }
+    join_pieces(a, row, m, s);
     lp = log_probability(xy, m, s, a.inv_t);
   }
   if (a.logprobs) a.logprobs[row] = lp.hi;
@@ -795,6 +927,12 @@ __global__ void __launch_bounds__(256) scale_rows_kernel(const Args a, const flo
 
 const char* problem(cudaError_t e) { return e == cudaSuccess ? nullptr : cudaGetErrorString(e); }
 
+// The ticket of a pass, unless every block has its items without asking; the paired loss has zeroed it before
+const char* set_ticket(Args& a, int pass, bool none, cudaStream_t stream) {
+  a.w.ticket = none ? nullptr : a.w.state->tickets + pass;
+  return none || a.pairs.pairs > 0 ? nullptr : problem(cudaMemsetAsync(a.w.ticket, 0, sizeof(int), stream));
+}
+
 template <typename T, int kCompute, int kMode>
 const char* launch_rows(const Args& from, cudaStream_t stream) {
   Args a = from;
@@ -818,13 +956,23 @@ const char* launch_rows(const Args& from, cudaStream_t stream) {
   const long items = static_cast<long>(a.rows) * a.pieces, most = static_cast<long>(held) * num_sms();
   if (4 * items + (1L << 20) >= 1L << 31) return "preference: too many rows";
   const int grid = static_cast<int>(items < most ? items : most);
-  if (items <= most) {
-    a.w.state = nullptr;
-  } else {
-    e = cudaMemsetAsync(a.w.state, 0, sizeof(State), stream);
-    if (e != cudaSuccess) return cudaGetErrorString(e);
-  }
+  const char* err = set_ticket(a, kMode == kGrad, items <= kFirst * most, stream);
+  if (err) return err;
   kernel<<<grid, kCompute + 32, smem, stream>>>(a);
+  return problem(cudaGetLastError());
+}
+
+template <typename T>
+const char* launch_sums(Args a, cudaStream_t stream) {
+  const int smem = kSumWarps * kSumStages * kSumStage * 16;
+  cudaError_t e = cudaFuncSetAttribute(sums_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return cudaGetErrorString(e);
+  const long items = static_cast<long>(a.rows) * a.pieces, blocks = kSumBlocks * num_sms();
+  if (items > INT_MAX / 2) return "preference: too many rows";
+  const char* err = set_ticket(a, 0, items <= 2 * blocks * kSumWarps, stream);       // two to a warp without asking
+  if (err) return err;
+  const int grid = static_cast<int>(items < blocks ? items : blocks);
+  sums_kernel<T><<<grid, kSumWarps * 32, smem, stream>>>(a);
   return problem(cudaGetLastError());
 }
 
@@ -839,8 +987,19 @@ int pieces_of(int rows, int vocab, int dtype) {
   return n;
 }
 
-// Scores of no more rows than there are SMs, each no longer than a block holds, are one launch of a block to a row: (37 rows of 32000 in bf16,
-// call by call: FIXME us, in pieces FIXME)
+// Sums by warps: 16-bit logits of 128 MB or more.  With fewer a warp has too little to do before its last piece (4000 rows of 8000 in bf16: 31.7 us by warps,
+// 28.0 by blocks; 20000 rows: 64 and 87).
+bool by_warps(int rows, int vocab, int dtype) { return dtype != 0 && static_cast<long>(rows) * vocab >= 1L << 26; }
+// Pieces of a row for its sums: by warps three to a warp at least, where a row has that many stages, and of no more than 32 stages each: a lane's sum
+// is then at most 8 + 32 additions deep, and off by 2^-19 at most
+int sums_pieces(int rows, int vocab, int dtype) {
+  if (!by_warps(rows, vocab, dtype)) return pieces_of(rows, vocab, dtype);
+  const long vectors = vocab / 8, most = vectors / kSumStage > 1 ? vectors / kSumStage : 1, warps = 3L * kSumBlocks * kSumWarps * num_sms();
+  const long n = (warps + rows - 1) / rows, least = vectors / (32 * kSumStage) + 1;
+  return static_cast<int>(n >= most ? most : n >= least ? n : least);
+}
+// Scores of no more rows than there are SMs, each no longer than a block holds, are one launch of a block to a row: 37 rows of 32000 in bf16
+// take 10.4 us a call, in pieces and a second launch 13.9.
 bool few_rows(int rows, int vocab, int dtype) { return rows <= num_sms() && vocab <= kWide * kVecs * (dtype == 0 ? 4 : 8); }
 
 template <typename T, int kMode>
@@ -867,11 +1026,15 @@ const char* launch_pass(Args a, int dtype, cudaStream_t stream) {
     return dtype == 0 ? launch_rows<float, kWide, kScores>(a, stream) : dtype == 1 ? launch_rows<__nv_bfloat16, kWide, kScores>(a, stream)
                                                                                    : launch_rows<__half, kWide, kScores>(a, stream);
   }
-  a.pieces = pieces_of(a.rows, a.vocab, dtype);
+  a.pieces = kMode == kScores ? sums_pieces(a.rows, a.vocab, dtype) : pieces_of(a.rows, a.vocab, dtype);
   a.each = (a.vocab / (16 / size) + a.pieces - 1) / a.pieces;
   if (a.pieces == 1 && !between) a.w.part = nullptr;
-  const char* err = dtype == 0 ? launch_rows<float, kBlock, kMode>(a, stream) : dtype == 1 ? launch_rows<__nv_bfloat16, kBlock, kMode>(a, stream)
-                                                                                          : launch_rows<__half, kBlock, kMode>(a, stream);
+  const char* err;
+  if (kMode == kScores && by_warps(a.rows, a.vocab, dtype))
+    err = dtype == 1 ? launch_sums<__nv_bfloat16>(a, stream) : launch_sums<__half>(a, stream);
+  else
+    err = dtype == 0 ? launch_rows<float, kBlock, kMode>(a, stream) : dtype == 1 ? launch_rows<__nv_bfloat16, kBlock, kMode>(a, stream)
+                                                                                 : launch_rows<__half, kBlock, kMode>(a, stream);
   if (kMode != kScores || err || a.pairs.pairs > 0 || !a.w.part) return err;
   const int blocks = (a.rows + 127) / 128;
   if (dtype == 0) whole_rows_kernel<float><<<blocks, 128, 0, stream>>>(a);
@@ -931,7 +1094,7 @@ using namespace b200;
 
 long nmtg_rows_workspace(int rows, int vocab, int dtype, int pairs) {
   long bytes = 0;
-  workspace(nullptr, rows, pairs, pieces_of(rows, vocab, dtype), &bytes);
+  workspace(nullptr, rows, pairs, sums_pieces(rows, vocab, dtype), &bytes);
   return bytes;
 }
 
@@ -939,7 +1102,7 @@ const char* nmtg_row_scores(const NmtgRows* r, cudaStream_t stream) {
   if (r->dtype < 0 || r->dtype > 2) return bad_type;
   Args a = row_args(r);
   long bytes;
-  const Work w = workspace(static_cast<char*>(r->workspace), r->rows, 0, pieces_of(r->rows, r->vocab, r->dtype), &bytes);
+  const Work w = workspace(static_cast<char*>(r->workspace), r->rows, 0, sums_pieces(r->rows, r->vocab, r->dtype), &bytes);
   a.w.state = w.state;
   a.w.part = w.part;
   return launch_pass<kScores>(a, r->dtype, stream);
@@ -962,7 +1125,7 @@ const char* nmtg_policy_loss(const NmtgRows* r, const NmtgPolicy* p, cudaStream_
   const int size = r->dtype == 0 ? 4 : 2;
   const char* err = nullptr;
   long bytes;
-  const Work w = workspace(static_cast<char*>(r->workspace), r->rows, 0, pieces_of(r->rows, r->vocab, r->dtype), &bytes);
+  const Work w = workspace(static_cast<char*>(r->workspace), r->rows, 0, sums_pieces(r->rows, r->vocab, r->dtype), &bytes);
   a.w.lp = w.lp;
   a.w.state = w.state;
   if (r->rows <= 0) {
@@ -986,7 +1149,7 @@ const char* nmtg_preference_loss(const NmtgRows* r, const NmtgPairs* p, cudaStre
   Args a = row_args(r);
   a.pairs = *p;
   long bytes;
-  const int pieces = pieces_of(r->rows, r->vocab, r->dtype);
+  const int pieces = sums_pieces(r->rows, r->vocab, r->dtype);
   const Work w = workspace(static_cast<char*>(r->workspace), r->rows, p->pairs, pieces, &bytes);
   if (p->pairs == 0) {                    // no loss; every row is outside
     cudaError_t e = cudaMemsetAsync(p->loss, 0, sizeof(float), stream);

@@ -453,3 +453,41 @@ def test_refusals_on_the_gpu():
         ops.ext().row_scores(x[:1].expand(4, 10), y, 0, 1.0, False)
     with pytest.raises(RuntimeError):
         ops.ext().row_scores(x.double(), y, 0, 1.0, False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab,kind,layout", [(8400, 8001, "bf16", "odd"), (8300, 8104, "fp16", "dense"), (2070, 32500, "bf16", "dense"),
+                                                    (270, 250054, "bf16", "padded"), (40, 1700011, "fp16", "odd"), (4500, 9001, "fp32", "odd")])
+def test_large_batches(rows, vocab, kind, layout):
+    """As many rows as keep every SM busy for long: rows handed out as they come, runs of padding among them, a captured graph replayed; the same
+    bits each time."""
+    x, y = _logits(5, vocab, kind, layout)
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    width, skip = x.stride(0), x.storage_offset()
+    x = (torch.randn(rows * width + skip, generator=g, device=DEV, dtype=x.dtype) * 2)[skip:].view(rows, width)[:, :vocab]
+    y = torch.randint(1, vocab, (rows,), generator=g, device=DEV)
+    y[rows // 3:rows // 2] = 0
+    y[-3:] = vocab
+    weight = torch.randn(rows, generator=g, device=DEV)
+    leaf = x.detach().requires_grad_(True)
+    got = pref.token_logprobs(leaf, y, temperature=0.9)
+    grad = torch.autograd.grad(got, leaf, weight)[0]
+    for r in range(0, rows, 500):
+        xd = x[r:r + 500].double().requires_grad_(True)
+        want = pref.token_logprobs(xd, y[r:r + 500], temperature=0.9)
+        _logprobs_close(got.detach()[r:r + 500], want.detach())
+        _grads_close(grad[r:r + 500], torch.autograd.grad(want, xd, weight[r:r + 500].double())[0], weight[r:r + 500] / 0.9, kind)
+    with torch.no_grad():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = pref.token_logprobs(x, y, temperature=0.9)
+        for _ in range(3):
+            out.zero_()
+            graph.replay()
+            assert torch.equal(out, got)
+    cu = torch.linspace(0, rows, 21, device=DEV).int()
+    loss, ranked, scores = pref.preference_loss(leaf, y, cu, temperature=0.9)
+    sums = pref.sequence_logprobs(got.detach(), cu)
+    assert ((scores - sums).abs() <= 2 ** -22 * (pref.sequence_logprobs(-got.detach(), cu) + 1)).all()     # one rounding of each word's, one of the sum
+    assert ranked == (sums[0::2] > sums[1::2]).sum()
+    assert torch.isfinite(torch.autograd.grad(loss, leaf)[0]).all() and ops.check_status() == 0
