@@ -62,6 +62,14 @@ def build_model(opt, dicts, remove_pretrain: bool = False, constants=None):
         for m in model.modules():
             if isinstance(m, FeedForward):
                 m.weight_drop = float(opt.weight_drop)
+    if getattr(opt, "ffn_keep8", False):
+        from .layers import FeedForward
+        blocks = [m for m in model.modules() if isinstance(m, FeedForward)]
+        if not blocks or any(m.glu or m.weight_drop > 0 for m in blocks):
+            raise NotImplementedError("-ffn_keep8 is built for the standard feed-forward blocks (without -ffn_glu, -weight_drop and "
+                                      "-batch_ensemble); model '%s' has none or others" % getattr(opt, "model", "?"))
+        for m in blocks:
+            m.keep8 = True
     if getattr(opt, "no_ffn", False) or getattr(opt, "depthwise_conv", False):
         from .layers import EncoderLayer
         layers = [m for m in getattr(model, "encoder", model).modules() if isinstance(m, EncoderLayer)]

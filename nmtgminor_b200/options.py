@@ -27,6 +27,7 @@ EXTRA_TRAIN_FLAGS = [
     ("trace_nvtx", "flag", False, {}),           # NVTX ranges around layers / buckets
     ("generator_chunk_rows", "int", 0, {}),      # output projection + loss this many rows at a time (logits stay in L2)
     ("fused_conv", "flag", False, {}),
+    ("ffn_keep8", "flag", False, {}),            # feed-forward blocks: what waits for the backward pass waits in 8 bits
     ("ema_decay", "float", 0.999, {}),           # decay of the parameter average kept with -ema
     ("lora_rank", "int", 0, {}),                 # finetune_whisper.py: rank of the LoRA adapters (0 = full fine-tuning)
     ("lora_alpha", "float", 16.0, {}),

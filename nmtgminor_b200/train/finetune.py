@@ -1,6 +1,6 @@
 """Fine-tuning utilities used for the Whisper / pretrained-model recipes: LoRA adapters on the fused Linear layers,
-an exponential moving average of the parameters kept on the flat fp32 vector, teacher-student distillation, and a
-batch-ensemble wrapper.
+an exponential moving average of the parameters kept on the flat fp32 vector, teacher-student distillation, a
+batch-ensemble wrapper, and preference tuning (paired and policy losses over ``ops.preference``).
 
 Reference: whisper/whisper_lora.py / the memory-efficient and EMA trainers of whisper/*.py (Hugging Face
 ``Seq2SeqTrainer`` subclasses; here the same pieces plug into this framework's ``Trainer``), distillation loss
@@ -16,6 +16,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .. import ops
+from ..ops import preference
 from ..models.layers import Linear
 
 
@@ -155,6 +156,86 @@ def distill_step(student, teacher, batch, alpha: float = 0.5, temperature: float
     tgt = s_out["tgt"]
     unpad = lambda o: ops.reference.unpad_packed(o["logprobs"].transpose(0, 1), tgt.cu, tgt.tokens.shape[0])
     return distillation_loss(unpad(s_out), unpad(t_out), s_out["target"], getattr(student, "pad_idx", 0), alpha, temperature)
+
+
+# ---------------------------------------------------------------------------------------------------
+# preference tuning
+# ---------------------------------------------------------------------------------------------------
+def packed_logits(model, batch):
+    """``(logits [rows, V], labels [rows], cu [sentences + 1])`` of a batch: the target words one sentence after another."""
+    out = model(batch, return_logits=False, compute_loss=False)
+    if "hidden_packed" not in out or getattr(model, "copy_generator", None) is not None:
+        raise NotImplementedError("preference tuning takes models whose output is the generator's logits of packed target words")
+    return model.generator(out["hidden_packed"]), out["target"], out["tgt"].cu
+
+
+@torch.no_grad()
+def word_scores(model, batch, temperature: float = 1.0):
+    """``(log-probabilities of the target words [rows], cu)``; rows of padding 0.  What ``policy_step`` takes from the model that the translations
+    were sampled from, and from the frozen one."""
+    logits, labels, cu = packed_logits(model, batch)
+    return preference.token_logprobs(logits, labels, getattr(model, "pad_idx", 0), temperature), cu
+
+
+@torch.no_grad()
+def sentence_scores(model, batch, temperature: float = 1.0):
+    """Log-probability ``[sentences]`` of every target sentence."""
+    return preference.sequence_logprobs(*word_scores(model, batch, temperature))
+
+
+def preference_step(model, batch, ref_logprobs=None, grad_scale=None, **loss):
+    """Paired preference loss of a batch whose target sentences are preferred and rejected translations in turn.  ``ref_logprobs``: the frozen model's
+    ``sentence_scores`` of it; further arguments as of ``ops.preference.preference_loss``.  Returns its three results; the gradient takes the
+    logits' place."""
+    logits, labels, cu = packed_logits(model, batch)
+    return preference.preference_loss(logits, labels, cu, ref_logprobs, pad_idx=getattr(model, "pad_idx", 0), grad_scale=grad_scale,
+                                      inplace=True, **loss)
+
+
+def policy_step(model, batch, old_logprobs, advantages, ref_logprobs=None, grad_scale=None, **loss):
+    """Clipped policy loss of sampled translations.  ``old_logprobs`` and ``ref_logprobs``: ``word_scores`` of the sampling and of the frozen model;
+    ``advantages``: of the sentences or of the words; further arguments as of ``ops.preference.policy_loss``.  Returns its four results; the
+    gradient takes the logits' place."""
+    logits, labels, cu = packed_logits(model, batch)
+    if advantages.dim() == 1 and advantages.shape[0] == cu.shape[0] - 1 and advantages.shape[0] != logits.shape[0]:
+        rows = torch.arange(logits.shape[0], device=cu.device)
+        of = torch.bucketize(rows, cu[1:].long(), right=True)                 # rows behind the last sentence are padding
+        advantages = advantages[of.clamp(max=advantages.shape[0] - 1)]
+    return preference.policy_loss(logits, labels, old_logprobs, advantages, ref_logprobs, pad_idx=getattr(model, "pad_idx", 0),
+                                  grad_scale=grad_scale, inplace=True, **loss)
+
+
+class PreferenceWrapper(nn.Module):
+    """Presents ``model`` to the training engine with the paired preference loss against the frozen ``reference`` (None: without one) as its loss.
+    Batches have preferred and rejected translations in turn; ``out["correct"]`` counts the pairs ranked as preferred.  The frozen model is
+    held outside the module tree, so it is neither trained nor saved; on a GPU it runs on the framework's kernels, and the step can be captured, where
+    its parameters have a ``FlatParameterStore``.  ``loss``: as of ``ops.preference.preference_loss``."""
+
+    def __init__(self, model: nn.Module, reference: Optional[nn.Module] = None, **loss):
+        super().__init__()
+        self.model = model
+        self._reference = [reference.eval() if reference is not None else None]
+        self.loss = loss
+        for p in reference.parameters() if reference is not None else ():
+            p.requires_grad_(False)
+
+    def __getattr__(self, name):
+        try:
+            return super().__getattr__(name)
+        except AttributeError:
+            return getattr(super().__getattr__("model"), name)
+
+    @property
+    def graph_capturable(self):
+        frozen = () if self._reference[0] is None else self._reference[0].parameters()
+        return bool(getattr(self.model, "graph_capturable", False)) and all(hasattr(p, "work") for p in frozen)
+
+    def forward(self, batch, grad_scale=None, **kw):
+        if not self.training:
+            return self.model(batch, **kw)
+        ref = None if self._reference[0] is None else sentence_scores(self._reference[0], batch, self.loss.get("temperature", 1.0))
+        loss, ranked, scores = preference_step(self.model, batch, ref, grad_scale, **self.loss)
+        return {"loss": loss, "correct": ranked, "scores": scores, "reference_scores": ref}
 
 
 class BatchEnsembleLinear(nn.Module):
