@@ -11,7 +11,8 @@
 // meets in shuffles.  For 16-bit types GELU takes one exponential and one division for the function and its slope together: with
 // t = 1 / (1 + p |z|) the tail Q(|z|) = exp(-z^2 / 2) (c1 t + ... + c7 t^7), fitted over the whole range to 1.1e-6 of itself (the
 // form of Hastings' approximation with coefficients of our own), against the 2^-9 and 2^-12 of the rounding that follows; erff and expf
-// would take longer than the bytes.  fp32 results use erfcf and expf.  Compiled without fast math: denormals are kept.
+// would take longer than the bytes.  fp32 results use erfcf and expf.  Compiled without fast math: codes, restored
+// values and fp32 results have their denormals; exponentials of 16-bit results that are below 2^-126 count as 0.
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -283,14 +284,14 @@ template <typename T, int kAct> __device__ __forceinline__ float2 acts_of(float2
 }
 // A restored element has 4 significant bits, so that the slopes of GELU and SiLU have few values: a block makes a table of them, for every exponent,
 // 3 bits and sign, and an element costs a look into shared memory.  Between 2^-18 and 2^7 the slopes are computed in full precision; below it is
-// 1/2 but for 2^-18, above 0 or 1.  (33.6 M elements with GELU: 46 us with the arithmetic of the forward pass, 38 with a table of that range and
+// 1/2 but for 2^-18, above 0 or 1, and of NaN NaN.  (33.6 M elements with GELU: 46 us with the arithmetic of the forward pass, 38 with a table of that range and
 // its ends looked after at every element.)
 constexpr int kSlopes = 1 << 12, kSlopeLow = (127 - 18) << 3, kSlopeHigh = (127 + 7) << 3;
 template <int kAct> __device__ __forceinline__ void make_slopes(float* table) {
   for (int i = threadIdx.x; i < kSlopes; i += 256) {
     const int at = i & 0x7FF;
     const bool down = i >> 11;
-    float v = at < kSlopeLow ? 0.5f : down ? 0.f : 1.f;
+    float v = at < kSlopeLow ? 0.5f : at >= 255 << 3 ? NAN : down ? 0.f : 1.f;
     if (at >= kSlopeLow && at < kSlopeHigh) v = slope_of<float, kAct>(__uint_as_float(static_cast<uint32_t>(i) << 20));
     table[i] = v;
   }

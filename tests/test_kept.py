@@ -331,3 +331,30 @@ def test_refusals_on_the_gpu():
               lambda: ops.ext().kept_quantise(x[:1].expand(4, 64)), lambda: ops.ext().kept_backward(x, k.codes.cpu(), k.scales, 0, 0.0, 0, 0)):
         with pytest.raises(RuntimeError):
             f()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
+def test_infinities_and_nan_reach_the_gradient(dtype, act):
+    """One infinity and one NaN among ordinary elements, in layouts of every path: their own gradients are NaN, and no others."""
+    for rows, width in ((64, 512), (5, 40), (3, 33)):
+        x = _matrix(rows, width, dtype, spread=1.0).clamp(-3, 3).to(DEV)
+        x[1, 7], x[2, 30] = math.inf, math.nan
+        z = x.requires_grad_(True)
+        grad = torch.autograd.grad(kept.activation(z, act), z, torch.ones_like(z))[0]
+        bad = torch.zeros(rows, width, dtype=torch.bool, device=DEV)
+        if act != "none":                    # without a function the gradient does not look at the element
+            bad[1, 7] = bad[2, 30] = True
+        assert torch.equal(torch.isnan(grad), bad)
+        back = kept.restore(kept.quantise(x.detach()))
+        bad[1, 7] = bad[2, 30] = True
+        assert torch.equal(torch.isnan(back), bad)
+
+
+@pytest.mark.gpu
+def test_no_second_derivative():
+    z = torch.randn(4, 64, device=DEV, requires_grad=True)
+    y = kept.activation(z, "gelu")
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y.sum(), z, create_graph=True)
