@@ -376,6 +376,11 @@ Tensor plain_rows(const Tensor& t) {
   return rows ? t : t.contiguous();
 }
 
+// The kernels' gradients are not differentiable again: create_graph would leave their part out without a word
+void once(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what, ": no second derivative (create_graph)");
+}
+
 struct ScoresNode : Function<ScoresNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, int64_t pad, double temperature) {
     auto [lp, stat] = row_scores(logits, labels, pad, temperature, true);
@@ -385,6 +390,7 @@ struct ScoresNode : Function<ScoresNode> {
     return lp;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("token_logprobs");
     const auto saved = ctx->get_saved_variables();
     const Tensor weight = g[0].to(at::kFloat).contiguous();
     return {row_scores_grad(saved[0], saved[1], saved[2], weight, ctx->saved_data["pad"].toInt(), ctx->saved_data["temperature"].toDouble()),
@@ -394,6 +400,7 @@ struct ScoresNode : Function<ScoresNode> {
 
 // The two losses: the gradient is made with the loss and belongs to the first backward pass
 variable_list loss_backward(AutogradContext* ctx, const variable_list& g, size_t inputs) {
+  once("preference or policy loss");
   variable_list out(inputs);
   if (!g[0].defined()) return out;
   TORCH_CHECK(!ctx->saved_data["grad"].isNone(), "a second backward pass through a preference or policy loss: its gradient went to the first one");
@@ -444,6 +451,7 @@ struct EmbedNode : Function<EmbedNode> {
     return embed_rows(tokens, table, scale);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("embedding with a sorted gradient");
     const auto saved = ctx->get_saved_variables();
     const int64_t words = ctx->saved_data["words"].toInt();
     return {embed_grad(saved[0], OptTensor(), g[0].contiguous(), OptTensor(), words, words, ctx->saved_data["scale"].toDouble(), 0.0, 0, 0,
@@ -495,6 +503,7 @@ struct ActivationNode : Function<ActivationNode> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("activation kept in 8 bits");
     const auto saved = ctx->get_saved_variables();
     return {kept_backward(plain_rows(g[0]), saved[0], saved[1], ctx->saved_data["act"].toInt(), ctx->saved_data["p"].toDouble(),
                           ctx->saved_data["seed"].toInt(), ctx->saved_data["stream"].toInt()),

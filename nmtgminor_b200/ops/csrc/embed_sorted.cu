@@ -498,7 +498,8 @@ bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 long up16(long n) { return (n + 15) & ~15L; }
 
 // Rows of a chunk (at most 32, a lane to each): enough chunks for every SM where there are few rows, fewer parts to join where there are many
-int chunk_of(int rows) { return rows < 4096 ? 8 : 16; }
+constexpr int kMostChunk = 16;
+int chunk_of(int rows) { return rows < 4096 ? 8 : kMostChunk; }
 int key_bits(int keys) {           // of numbers up to `keys`
   int b = 1;
   while (b < 31 && (1L << b) <= keys) ++b;
@@ -516,7 +517,7 @@ template <typename T, int kN, bool kDrop, bool kAdd>
 const char* sums(const Sum& s, cudaStream_t stream) {
   const dim3 block = shape(s.width, kN);
   const int smem = sizeof(T) * kN == 16 ? s.chunk * 256 * 16 : 0;
-  cudaError_t e = cudaFuncSetAttribute(reduce_kernel<T, kN, kDrop, kAdd>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = cudaFuncSetAttribute(reduce_kernel<T, kN, kDrop, kAdd>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostChunk * 256 * 16);
   if (e != cudaSuccess) return problem(e);
   reduce_kernel<T, kN, kDrop, kAdd><<<dim3((s.chunks + block.y - 1) / block.y), block, smem, stream>>>(s);
   e = cudaGetLastError();

@@ -580,7 +580,13 @@ __global__ void __launch_bounds__(kSumWarps * 32, kSumBlocks) sums_kernel(const 
         label = label_of(number);
         after = a.w.ticket ? 2 * warps + atomicAdd(a.w.ticket, 1) : items;
       }
-      if (y < 0) continue;
+      if (y < 0) {
+        if (lane == 0 && !a.w.part) {                       // a row in one piece
+          a.logprobs[n] = 0.f;
+          if (a.stat) a.stat[n] = make_float2(0.f, 1.f);
+        }
+        continue;
+      }
       prow = a.pieces == 1 ? n : n / a.pieces;
       const int piece = n - prow * a.pieces;
       const T* x = x0 + static_cast<long>(prow) * a.ld;
@@ -978,12 +984,21 @@ const char* launch_sums(Args a, cudaStream_t stream) {
 
 template <typename T> constexpr int warp_row() { return 32 * kVecs * Num<T>::kE; }       // elements that a warp holds
 
+// SMs of the GPU, those in reserve too: how a row is divided decides the bits of a result and the size of the workspace
+int all_sms() {
+  static const int n = [] {
+    int device = 0, sms = 0;
+    return cudaGetDevice(&device) == cudaSuccess && cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) == cudaSuccess && sms > 0 ? sms : 148;
+  }();
+  return n;
+}
+
 // Pieces of a row: as many as hold it; for few rows more, of 4 KB at least, until every block that the GPU holds has one.
 int pieces_of(int rows, int vocab, int dtype) {
   const int vectors = vocab / (dtype == 0 ? 4 : 8);
   int n = (vectors + kBlock * kVecs - 1) / (kBlock * kVecs);
   if (n < 1) n = 1;
-  while (2L * n * rows <= 2 * num_sms() && vectors >= 512 * n) n *= 2;
+  while (static_cast<long>(n) * rows <= all_sms() && vectors >= 512 * n) n *= 2;
   return n;
 }
 
@@ -994,13 +1009,13 @@ bool by_warps(int rows, int vocab, int dtype) { return dtype != 0 && static_cast
 // is then at most 8 + 32 additions deep, and off by 2^-19 at most
 int sums_pieces(int rows, int vocab, int dtype) {
   if (!by_warps(rows, vocab, dtype)) return pieces_of(rows, vocab, dtype);
-  const long vectors = vocab / 8, most = vectors / kSumStage > 1 ? vectors / kSumStage : 1, warps = 3L * kSumBlocks * kSumWarps * num_sms();
+  const long vectors = vocab / 8, most = vectors / kSumStage > 1 ? vectors / kSumStage : 1, warps = 3L * kSumBlocks * kSumWarps * all_sms();
   const long n = (warps + rows - 1) / rows, least = vectors / (32 * kSumStage) + 1;
   return static_cast<int>(n >= most ? most : n >= least ? n : least);
 }
 // Scores of no more rows than there are SMs, each no longer than a block holds, are one launch of a block to a row: 37 rows of 32000 in bf16
 // take 10.4 us a call, in pieces and a second launch 13.9.
-bool few_rows(int rows, int vocab, int dtype) { return rows <= num_sms() && vocab <= kWide * kVecs * (dtype == 0 ? 4 : 8); }
+bool few_rows(int rows, int vocab, int dtype) { return rows <= all_sms() && vocab <= kWide * kVecs * (dtype == 0 ? 4 : 8); }
 
 template <typename T, int kMode>
 const char* launch_short(const Args& a, cudaStream_t stream) {

@@ -95,8 +95,8 @@ def _check_rows(logits, labels, temperature):
         raise TypeError("logits must be floating-point")
     if labels.device != logits.device:
         raise ValueError("labels are on %s, logits on %s" % (labels.device, logits.device))
-    if not temperature > 0.0 or temperature == float("inf"):
-        raise ValueError("temperature must be positive")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError("temperature must be positive (from 1e-30 to 1e30)")
 
 
 def _check_vector(t, n, logits, name):

@@ -457,7 +457,7 @@ def test_refusals_on_the_gpu():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,vocab,kind,layout", [(8400, 8001, "bf16", "odd"), (8300, 8104, "fp16", "dense"), (2070, 32500, "bf16", "dense"),
-                                                    (270, 250054, "bf16", "padded"), (40, 1700011, "fp16", "odd"), (4500, 9001, "fp32", "odd")])
+                                                    (270, 250054, "bf16", "padded"), (15000, 4700, "bf16", "padded"), (40, 1700011, "fp16", "odd"), (4500, 9001, "fp32", "odd")])
 def test_large_batches(rows, vocab, kind, layout):
     """As many rows as keep every SM busy for long: rows handed out as they come, runs of padding among them, a captured graph replayed; the same
     bits each time."""
@@ -491,3 +491,21 @@ def test_large_batches(rows, vocab, kind, layout):
     assert ((scores - sums).abs() <= 2 ** -22 * (pref.sequence_logprobs(-got.detach(), cu) + 1)).all()     # one rounding of each word's, one of the sum
     assert ranked == (sums[0::2] > sums[1::2]).sum()
     assert torch.isfinite(torch.autograd.grad(loss, leaf)[0]).all() and ops.check_status() == 0
+
+
+@pytest.mark.gpu
+def test_no_second_derivative():
+    x, y = _logits(9, 40, "fp32", "dense")
+    leaf = x.requires_grad_(True)
+    zero = torch.zeros(9, device=DEV)
+    for f in (lambda: pref.token_logprobs(leaf, y).sum(), lambda: pref.policy_loss(leaf, y, zero, zero)[0],
+              lambda: pref.preference_loss(leaf, y, torch.tensor([0, 4, 9], device=DEV))[0]):
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(f(), leaf, create_graph=True)
+
+
+def test_temperatures_out_of_range():
+    x, y = torch.zeros(2, 3), torch.ones(2, dtype=torch.long)
+    for t in (0.0, -1.0, math.nan, math.inf, 1e-39):
+        with pytest.raises(ValueError):
+            pref.token_logprobs(x, y, temperature=t)
