@@ -201,3 +201,19 @@ def test_refusals_on_the_gpu():
               lambda: ops.ext().embed_grad(tok, None, dy, None, 5, 5, 1.0, 1.0, 0, 0, 0)):
         with pytest.raises(RuntimeError):
             f()
+
+
+@pytest.mark.gpu
+def test_tables_of_more_than_2_31_elements():
+    """Offsets beyond 32 bits in the table, its gradient and dy: the words at the end against their rows by themselves."""
+    vocab, width, rows = 270000, 8192, 265000
+    table = torch.nn.Parameter(torch.empty(vocab, width, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(1)))
+    tokens = torch.arange(rows, device="cuda") + (vocab - rows)
+    tokens[-3:] = vocab - 1
+    out = ops.embedding(tokens, table, scale=2.0, pad_idx=0, sorted_grad=True)
+    assert torch.equal(out.detach()[-9:], table.detach()[tokens[-9:]] * 2)
+    dy = torch.empty_like(out).normal_(generator=torch.Generator(device="cuda").manual_seed(2))
+    grad = torch.autograd.grad(out, table, dy)[0]
+    assert torch.equal(grad[-9:-3], dy[-9:-3] * 2) and (grad[:vocab - rows] == 0).all() and (grad[-3:-1] == 0).all()
+    want = 2 * dy[-3:].double().sum(0)
+    assert ((grad[-1].double() - want).abs() <= 2 ** -8 * want.abs() + 2 ** -22 * dy[-3:].double().abs().sum(0)).all()

@@ -358,3 +358,21 @@ def test_no_second_derivative():
     y = kept.activation(z, "gelu")
     with pytest.raises(RuntimeError):
         torch.autograd.grad(y.sum(), z, create_graph=True)
+
+
+@pytest.mark.gpu
+def test_more_than_2_31_elements():
+    """Offsets beyond 32 bits: the last rows of 2.2e9 elements against the same rows by themselves."""
+    for rows, width in ((540000, 4096), (540000, 4100)):
+        x = torch.empty(rows, width, dtype=torch.bfloat16, device=DEV).normal_(generator=torch.Generator(device=DEV).manual_seed(3))
+        few = x[-5:].clone().requires_grad_(True)
+        z = x.requires_grad_(True)
+        y = kept.activation(z, "gelu")
+        want = kept.activation(few, "gelu")
+        assert torch.equal(y.detach()[-5:], want.detach())
+        dy = torch.ones_like(y)
+        del x
+        assert torch.equal(torch.autograd.grad(y, z, dy)[0][-5:], torch.autograd.grad(want, few, dy[-5:])[0])
+        del dy, y
+        assert torch.equal(kept.restore(kept.quantise(z.detach()))[-5:], kept.restore(kept.quantise(few.detach())))
+        del z

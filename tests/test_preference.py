@@ -509,3 +509,26 @@ def test_temperatures_out_of_range():
     for t in (0.0, -1.0, math.nan, math.inf, 1e-39):
         with pytest.raises(ValueError):
             pref.token_logprobs(x, y, temperature=t)
+
+
+@pytest.mark.gpu
+def test_more_than_2_31_logits():
+    """Offsets beyond 32 bits: the last rows of a matrix of 2.2e9 logits against the same rows by themselves."""
+    rows, vocab = 8800, 250054
+    x = torch.empty(rows, 250056, dtype=torch.bfloat16, device=DEV).normal_(generator=torch.Generator(device=DEV).manual_seed(3))[:, :vocab]
+    y = torch.randint(1, vocab, (rows,), generator=torch.Generator().manual_seed(3)).to(DEV)
+    weight = torch.ones(rows, device=DEV)
+    last = x[-7:].clone().double().requires_grad_(True)
+    want = pref.token_logprobs(last, y[-7:])
+    leaf = x.requires_grad_(True)
+    got = pref.token_logprobs(leaf, y)
+    grad = torch.autograd.grad(got, leaf, weight)[0]
+    _logprobs_close(got.detach()[-7:], want.detach())
+    _grads_close(grad[-7:], torch.autograd.grad(want, last, weight[-7:].double())[0], weight[-7:], "bf16")
+    cu = torch.tensor([0, rows - 7, rows], device=DEV)
+    for f in (lambda: pref.preference_loss(leaf, y, cu, inplace=False), lambda: pref.policy_loss(leaf, y, got.detach(), weight)):
+        grad = None
+        grad = torch.autograd.grad(f()[0], leaf)[0]
+        ratio = grad[-7:].float() / torch.autograd.grad(pref.token_logprobs(leaf[-7:], y[-7:]), leaf, weight[-7:])[0][-7:].float()
+        assert (ratio.nan_to_num(ratio[0, 0].item()) / ratio[0, 0] - 1).abs().max() <= 2 ** -6          # one coefficient; four roundings of bf16
+    assert ops.check_status() == 0
