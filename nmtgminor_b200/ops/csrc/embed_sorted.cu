@@ -191,15 +191,17 @@ __global__ void __launch_bounds__(1024) radix_scan_kernel(int* __restrict__ coun
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   if (t == 0) carry = 0;
   __syncthreads();
-  constexpr int kEach = 8;
+  constexpr int kEach = 32;                                     // one wait for 32768 counts: the loads are slow beside the clearing
   for (int base = 0; base < n; base += 1024 * kEach) {
     int v[kEach], sum = 0;
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
+    for (int j = 0; j < kEach; j += 4) {                        // (where n is no multiple of 4, what is behind it counts for nothing)
       const int i = base + t * kEach + j;
-      v[j] = i < n ? counts[i] : 0;
-      sum += v[j];
+      const int4 u = i < n ? *reinterpret_cast<const int4*>(counts + i) : make_int4(0, 0, 0, 0);
+      v[j] = u.x; v[j + 1] = u.y; v[j + 2] = u.z; v[j + 3] = u.w;
     }
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) sum += v[j];
     int before = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += u; }
@@ -214,10 +216,11 @@ __global__ void __launch_bounds__(1024) radix_scan_kernel(int* __restrict__ coun
     __syncthreads();
     int at = carry + before - sum + (warp ? warps[warp - 1] : 0);
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
+    for (int j = 0; j < kEach; j += 4) {
       const int i = base + t * kEach + j;
-      if (i < n) counts[i] = at;
-      at += v[j];
+      const int4 u = make_int4(at, at + v[j], at + v[j] + v[j + 1], at + v[j] + v[j + 1] + v[j + 2]);
+      if (i < n) *reinterpret_cast<int4*>(counts + i) = u;
+      at = u.w + v[j + 3];
     }
     __syncthreads();
     if (t == 1023) carry = at;
@@ -405,27 +408,38 @@ __global__ void __launch_bounds__(256, 3) reduce_kernel(const Sum s) {
   }
 }
 
-// The sums that begin in a chunk and go on behind it.  Most end in the next chunk: two parts, a warp to each sum.  The others take a block and a share
-// of the columns each, the parts in 8 runs one after another, the runs in order; their end is found by 32 looks at a time.  (The list's order does not
+// The sums that begin in a chunk and go on behind it.  Most end in the next chunk: two parts, a warp of the first half of the blocks to each sum.  The others
+// take a block of the second half and a share of the columns each, the parts in 8 runs one after another, the runs in order; their end is found by 32 looks at a time.  (The list's order does not
 // matter: every sum is joined by itself.)
 template <typename T, int kN, bool kAdd>
 __global__ void __launch_bounds__(256) join_kernel(const Sum s) {
   constexpr int kRuns = 8, kCols = 32;
   __shared__ float runs[kRuns][kCols * kN];
-  const int x = threadIdx.x & 31, run = threadIdx.x >> 5, sums = s.joins[0], long_sums = s.joins[1];
-  for (int i = (blockIdx.y * gridDim.x + blockIdx.x) * kRuns + run; i < sums; i += gridDim.x * gridDim.y * kRuns) {
+  const int x = threadIdx.x & 31, run = threadIdx.x >> 5, half = gridDim.x / 2;
+  const bool first_half = static_cast<int>(blockIdx.x) < half;
+  const int sums = first_half ? s.joins[0] : 0, long_sums = first_half ? 0 : s.joins[1];
+  for (int i = (blockIdx.y * half + blockIdx.x) * kRuns + run; i < sums; i += half * gridDim.y * kRuns) {
     const int c = s.joins[2 + i], key = s.sorted[(c + 1) * s.chunk];
     const float* const first = s.parts + (static_cast<long>(c) * 2 + 1) * s.width;
     const float* const second = s.parts + static_cast<long>(c + 1) * 2 * s.width;
-#pragma unroll 2
+#pragma unroll 4
     for (int col = x * kN; col < s.width; col += 32 * kN) {
       float acc[kN];
+      if constexpr (kN % 4 == 0) {
 #pragma unroll
-      for (int j = 0; j < kN; ++j) acc[j] = first[col + j] + second[col + j];
+        for (int j = 0; j < kN; j += 4) {
+          const float4 a = *reinterpret_cast<const float4*>(first + col + j), b = *reinterpret_cast<const float4*>(second + col + j);
+          acc[j] = a.x + b.x; acc[j + 1] = a.y + b.y; acc[j + 2] = a.z + b.z; acc[j + 3] = a.w + b.w;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kN; ++j) acc[j] = first[col + j] + second[col + j];
+      }
       to_grad<T, kN, kAdd>(s, key, col, acc);
     }
   }
-  for (int i = blockIdx.x; i < long_sums; i += gridDim.x) {
+  if (first_half) return;
+  for (int i = static_cast<int>(blockIdx.x) - half; i < long_sums; i += half) {
     const int c = s.joins[2 + s.chunks + i], key = s.sorted[(c + 1) * s.chunk];
     int lo = (c + 1) * s.chunk, hi = s.rows;                    // the first place behind the sum's last is in [lo, hi]
     while (lo < hi) {
@@ -445,7 +459,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Sum s) {
 #pragma unroll
       for (int j = 0; j < kN; ++j) acc[j] = 0.f;
       if (col < s.width) {
-#pragma unroll 4
+#pragma unroll 8
         for (int q = from; q < to; ++q) {
           const float* part = s.parts + (static_cast<long>(c + q) * 2 + (q == 0 ? 1 : 0)) * s.width + col;
           if constexpr (kN % 4 == 0) {
@@ -523,7 +537,7 @@ const char* sums(const Sum& s, cudaStream_t stream) {
   e = cudaGetLastError();
   if (e != cudaSuccess || s.chunks < 2) return problem(e);
   const int cols = (s.width + 32 * kN - 1) / (32 * kN), across = cols < 8 ? cols : 8, want = (s.chunks + 7) / 8, most = 16 * num_sms() / across;
-  join_kernel<T, kN, kAdd><<<dim3(want < most ? want : most, across), 256, 0, stream>>>(s);
+  join_kernel<T, kN, kAdd><<<dim3(2 * (want < most ? want : most), across), 256, 0, stream>>>(s);
   return problem(cudaGetLastError());
 }
 
@@ -608,16 +622,16 @@ const char* nmtg_embed_grad(const NmtgEmbedGrad* d) {
   } else {
     const int passes = (bits + kDigitBits - 1) / kDigitBits, digit = (bits + passes - 1) / passes;
     const size_t smem = 8 * sizeof(int) << digit;
-    clear.of = 5 * passes;               // the scan, one block and short, beside a fifth
+    clear.of = 10 * passes;              // the scan, one block that waits for its loads, beside the largest share
     for (int i = 0; i < passes; ++i) {
       Pass p = {i ? key[(i - 1) & 1] : nullptr, i ? row[(i - 1) & 1] : nullptr, key[i & 1], row[i & 1], counts, i * digit, digit, 1 << digit, tiles};
-      clear.next(tiles, 2);
+      clear.next(tiles, 3);
       radix_count_kernel<<<tiles + extra, 256, 0, stream>>>(k, p, joins, clear);
       if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
-      clear.next(1, 1);
+      clear.next(1, 4);
       radix_scan_kernel<<<1 + (extra + 3) / 4, 1024, 0, stream>>>(counts, tiles << digit, clear);
       if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
-      clear.next(tiles, 2);
+      clear.next(tiles, 3);
       radix_scatter_kernel<<<tiles + extra, 256, smem, stream>>>(k, p, clear);
       if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
       last = i & 1;
