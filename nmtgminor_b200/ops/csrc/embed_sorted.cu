@@ -6,7 +6,8 @@
 //      ends in a chunk goes to its row of the gradient, one that crosses an end leaves its part in the workspace.
 //   3. join:   the parts of a sum, in order.
 // Where the gradient is written whole, its rows are cleared by further blocks of the sorting kernels: these wait on latency, the clearing on memory.
-// Bound by the bytes of dy and of the gradient's rows.  Sums in 32 bits, one rounding at the end.
+// Bound by the bytes of dy and of the gradient's rows: 65536 rows of 1024 in fp32 into 250054 words 248 us (floor 209: dy, the gradient), 8200 rows in
+// bf16 86 (82).  Sums in 32 bits, one rounding at the end.
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -51,19 +52,26 @@ struct Keys {
   }
 };
 
-// parts [at, to) of `of` of the memory to clear, by the blocks from `first` on
+// parts [at, to) of `of` of the memory to clear, by the blocks from `first` on, 16 KB each: short blocks write at 7.2 TB/s, 6 to an SM that go through it
+// all at 5.9 (1 GB)
 struct Clear {
   uint4* p;
   long n;
   int first, at, to, of;
   __device__ __forceinline__ bool mine() const { return static_cast<int>(blockIdx.x) >= first; }
   __device__ __forceinline__ void run() const {
-    const long begin = n * at / of, end = n * to / of;
-    const long step = static_cast<long>(gridDim.x - first) * blockDim.x;
+    const long begin = n * at / of + static_cast<long>(blockIdx.x - first) * 1024, end = n * to / of;
 #pragma unroll 4
-    for (long i = begin + (blockIdx.x - first) * static_cast<long>(blockDim.x) + threadIdx.x; i < end; i += step) __stcs(p + i, make_uint4(0, 0, 0, 0));
+    for (int j = threadIdx.x; j < 1024; j += blockDim.x)
+      if (begin + j < end) p[begin + j] = make_uint4(0, 0, 0, 0);
   }
-  void next(int blocks, int parts) { first = blocks; at = to; to += parts; }      // the next kernel's share
+  // the next kernel's share, behind its own blocks: the blocks in all
+  int next(int blocks, int parts) {
+    first = blocks;
+    at = to;
+    to += parts;
+    return blocks + static_cast<int>((n * to / of - n * at / of + 1023) / 1024);
+  }
 };
 
 // Every row's place in its tile: the number of rows of the tile before it, 16 threads to the same rows, each over every 16th group of 4.  Key and row
@@ -184,14 +192,13 @@ __global__ void __launch_bounds__(256) radix_count_kernel(const Keys k, const Pa
 }
 
 // counts -> their exclusive sums, one block
-__global__ void __launch_bounds__(1024) radix_scan_kernel(int* __restrict__ counts, int n, const Clear clear) {
-  if (clear.mine()) { clear.run(); return; }
+__global__ void __launch_bounds__(1024) radix_scan_kernel(int* __restrict__ counts, int n) {
   __shared__ int warps[32];
   __shared__ int carry;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   if (t == 0) carry = 0;
   __syncthreads();
-  constexpr int kEach = 32;                                     // one wait for 32768 counts: the loads are slow beside the clearing
+  constexpr int kEach = 32;                                     // one wait for 32768 counts
   for (int base = 0; base < n; base += 1024 * kEach) {
     int v[kEach], sum = 0;
 #pragma unroll
@@ -322,13 +329,19 @@ __device__ __forceinline__ void to_grad(const Sum& s, int key, int col, const fl
   }
 }
 
+template <int kBytes> __device__ __forceinline__ void copy_vector(void* to, const void* from) {
+  if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+  else if constexpr (kBytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+
 // blockDim = (column vectors, chunks of this block), whole warps to a chunk; a lane has the key and the row of one of its sorted rows.  Every thread
 // copies its columns of all the chunk's rows to shared memory (kCopy) before it adds up the first: 64 KB a block on their way, and three blocks
 // to an SM, whatever the words' frequencies are.
 template <typename T, int kN, bool kDrop, bool kAdd>
 __global__ void __launch_bounds__(256, 3) reduce_kernel(const Sum s) {
-  constexpr bool kCopy = sizeof(T) * kN == 16;
-  extern __shared__ __align__(16) uint4 held[];                 // [chunk][256]
+  constexpr int kBytes = sizeof(T) * kN;
+  constexpr bool kCopy = kBytes >= 8;
+  extern __shared__ __align__(16) unsigned char held[];         // [chunk][256] vectors
   const int c = blockIdx.x * blockDim.y + threadIdx.y, lane = threadIdx.x & 31, thread = threadIdx.y * blockDim.x + threadIdx.x;
   if (c >= s.chunks) return;
   const int begin = c * s.chunk, count = min(s.rows - begin, s.chunk);
@@ -346,7 +359,7 @@ __global__ void __launch_bounds__(256, 3) reduce_kernel(const Sum s) {
 #pragma unroll 4
       for (int j = 0; j < with_key; ++j) {
         const int row = __shfl_sync(0xffffffffu, my_row, j);
-        if (in) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(held + j * 256 + thread)), "l"(dy + static_cast<long>(row) * s.width) : "memory");
+        if (in) copy_vector<kBytes>(held + (j * 256 + thread) * kBytes, dy + static_cast<long>(row) * s.width);
       }
       asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
     }
@@ -382,7 +395,7 @@ __global__ void __launch_bounds__(256, 3) reduce_kernel(const Sum s) {
       }
       if (in) {
         Pack<T, kN> v;
-        if constexpr (kCopy) v = *reinterpret_cast<const Pack<T, kN>*>(held + j * 256 + thread);
+        if constexpr (kCopy) v = *reinterpret_cast<const Pack<T, kN>*>(held + (j * 256 + thread) * kBytes);
         else v = *reinterpret_cast<const Pack<T, kN>*>(dy + static_cast<long>(row) * s.width);
 #pragma unroll
         for (int q = 0; q < kN; ++q) {
@@ -530,7 +543,7 @@ dim3 shape(int width, int n) {
 template <typename T, int kN, bool kDrop, bool kAdd>
 const char* sums(const Sum& s, cudaStream_t stream) {
   const dim3 block = shape(s.width, kN);
-  const int smem = sizeof(T) * kN == 16 ? s.chunk * 256 * 16 : 0;
+  const int vector = sizeof(T) * kN, smem = vector >= 8 ? s.chunk * 256 * vector : 0;
   cudaError_t e = cudaFuncSetAttribute(reduce_kernel<T, kN, kDrop, kAdd>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostChunk * 256 * 16);
   if (e != cudaSuccess) return problem(e);
   reduce_kernel<T, kN, kDrop, kAdd><<<dim3((s.chunks + block.y - 1) / block.y), block, smem, stream>>>(s);
@@ -546,24 +559,32 @@ const char* sums_drop(const Sum& s, cudaStream_t stream) {
   return s.p > 0.f ? sums<T, kN, true, kAdd>(s, stream) : sums<T, kN, false, kAdd>(s, stream);
 }
 
+// Elements of a vector: 16 bytes, 4 elements of a 16-bit type, or one (34056 rows of 300 in bf16: 50 us with the lookup, one by one 90)
 template <typename T>
 const char* sums_type(const Sum& s, bool add, cudaStream_t stream) {
   constexpr int kN = 16 / sizeof(T);
-  const bool vectors = s.width % kN == 0 && aligned(s.dy) && aligned(s.grad);
-  if (add) return vectors ? sums_drop<T, kN, true>(s, stream) : sums_drop<T, 1, true>(s, stream);
-  return vectors ? sums_drop<T, kN, false>(s, stream) : sums_drop<T, 1, false>(s, stream);
+  const bool on = aligned(s.dy) && aligned(s.grad);
+  if (on && s.width % kN == 0) return add ? sums_drop<T, kN, true>(s, stream) : sums_drop<T, kN, false>(s, stream);
+  if constexpr (kN > 4)
+    if (on && s.width % 4 == 0) return add ? sums_drop<T, 4, true>(s, stream) : sums_drop<T, 4, false>(s, stream);
+  return add ? sums_drop<T, 1, true>(s, stream) : sums_drop<T, 1, false>(s, stream);
 }
 
+template <typename T, int kN>
+const char* gather_by(const int64_t* tokens, const void* table, void* out, int rows, int vocab, int width, float scale, cudaStream_t stream) {
+  const dim3 block = shape(width, kN);
+  const int blocks = (rows + static_cast<int>(block.y) - 1) / static_cast<int>(block.y), most = 32 * num_sms();
+  const int grid = blocks < most ? blocks : most;
+  rows_kernel<T, kN><<<grid, block, 0, stream>>>(tokens, static_cast<const T*>(table), static_cast<T*>(out), rows, vocab, width, scale);
+  return problem(cudaGetLastError());
+}
 template <typename T>
 const char* gather(const int64_t* tokens, const void* table, void* out, int rows, int vocab, int width, float scale, cudaStream_t stream) {
   constexpr int kN = 16 / sizeof(T);
-  const bool vectors = width % kN == 0 && aligned(table) && aligned(out);
-  const dim3 block = shape(width, vectors ? kN : 1);
-  const int blocks = (rows + static_cast<int>(block.y) - 1) / static_cast<int>(block.y), most = 32 * num_sms();
-  const int grid = blocks < most ? blocks : most;
-  if (vectors) rows_kernel<T, kN><<<grid, block, 0, stream>>>(tokens, static_cast<const T*>(table), static_cast<T*>(out), rows, vocab, width, scale);
-  else rows_kernel<T, 1><<<grid, block, 0, stream>>>(tokens, static_cast<const T*>(table), static_cast<T*>(out), rows, vocab, width, scale);
-  return problem(cudaGetLastError());
+  const bool on = aligned(table) && aligned(out);
+  if (on && width % kN == 0) return gather_by<T, kN>(tokens, table, out, rows, vocab, width, scale, stream);
+  if (on && width % 4 == 0) return gather_by<T, 4>(tokens, table, out, rows, vocab, width, scale, stream);
+  return gather_by<T, 1>(tokens, table, out, rows, vocab, width, scale, stream);
 }
 
 }  // namespace
@@ -598,41 +619,38 @@ const char* nmtg_embed_grad(const NmtgEmbedGrad* d) {
     const cudaError_t e = cudaMemsetAsync(static_cast<char*>(d->grad) + bytes / 16 * 16, 0, bytes % 16, stream);
     if (e != cudaSuccess) return cudaGetErrorString(e);
   }
-  const long want = (clear.n + 1023) / 1024, most = 6L * num_sms();
-  const int extra = static_cast<int>(want < most ? want : most);
   int last = 0;
   cudaError_t e;
   const int blocks = (n + kRankRows - 1) / kRankRows;
   if (n <= kOneTile && bits + kRowBits <= 32) {
-    clear.next(blocks, 1);
-    tile_rank_kernel<true><<<blocks + extra, 256, 0, stream>>>(k, kOneTile, nullptr, row[0], key[0], joins, clear);
+    const int grid = clear.next(blocks, 1);
+    tile_rank_kernel<true><<<grid, 256, 0, stream>>>(k, kOneTile, nullptr, row[0], key[0], joins, clear);
     if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
   } else if (n <= kPackedRows && bits + kRowBits <= 32) {
     const int smem = (n + kMergeTile - 1) / kMergeTile * kMergeTile * 4;
     if ((e = cudaFuncSetAttribute(merge_rank_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPackedRows * 4)) != cudaSuccess)
       return cudaGetErrorString(e);
     uint32_t* const tiles = reinterpret_cast<uint32_t*>(key[1]);
-    clear.of = 2;
-    clear.next(blocks, 1);
-    tile_rank_kernel<false><<<blocks + extra, 256, 0, stream>>>(k, kMergeTile, tiles, nullptr, nullptr, joins, clear);
+    clear.of = 4;
+    int grid = clear.next(blocks, 3);
+    tile_rank_kernel<false><<<grid, 256, 0, stream>>>(k, kMergeTile, tiles, nullptr, nullptr, joins, clear);
     if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
-    clear.next((n + kMergeRows - 1) / kMergeRows, 1);
-    merge_rank_kernel<<<clear.first + extra, 256, smem, stream>>>(tiles, n, row[0], key[0], clear);
+    grid = clear.next((n + kMergeRows - 1) / kMergeRows, 1);
+    merge_rank_kernel<<<grid, 256, smem, stream>>>(tiles, n, row[0], key[0], clear);
     if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
   } else {
     const int passes = (bits + kDigitBits - 1) / kDigitBits, digit = (bits + passes - 1) / passes;
     const size_t smem = 8 * sizeof(int) << digit;
-    clear.of = 10 * passes;              // the scan, one block that waits for its loads, beside the largest share
+    clear.of = 2 * passes;               // none beside the scan: its loads would wait behind the writes (4 us without them, 31 with a fifth of 1 GB)
     for (int i = 0; i < passes; ++i) {
       Pass p = {i ? key[(i - 1) & 1] : nullptr, i ? row[(i - 1) & 1] : nullptr, key[i & 1], row[i & 1], counts, i * digit, digit, 1 << digit, tiles};
-      clear.next(tiles, 3);
-      radix_count_kernel<<<tiles + extra, 256, 0, stream>>>(k, p, joins, clear);
+      int grid = clear.next(tiles, 1);
+      radix_count_kernel<<<grid, 256, 0, stream>>>(k, p, joins, clear);
       if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
-      clear.next(1, 4);
-      radix_scan_kernel<<<1 + (extra + 3) / 4, 1024, 0, stream>>>(counts, tiles << digit, clear);
+      radix_scan_kernel<<<1, 1024, 0, stream>>>(counts, tiles << digit);
       if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
-      clear.next(tiles, 3);
-      radix_scatter_kernel<<<tiles + extra, 256, smem, stream>>>(k, p, clear);
+      grid = clear.next(tiles, 1);
+      radix_scatter_kernel<<<grid, 256, smem, stream>>>(k, p, clear);
       if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
       last = i & 1;
     }

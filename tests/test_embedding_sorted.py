@@ -217,3 +217,21 @@ def test_tables_of_more_than_2_31_elements():
     assert torch.equal(grad[-9:-3], dy[-9:-3] * 2) and (grad[:vocab - rows] == 0).all() and (grad[-3:-1] == 0).all()
     want = 2 * dy[-3:].double().sum(0)
     assert ((grad[-1].double() - want).abs() <= 2 ** -8 * want.abs() + 2 ** -22 * dy[-3:].double().abs().sum(0)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("rows,vocab,width", [(300, 50, 12), (9000, 700, 300), (20000, 5000, 20), (40, 9, 2), (600, 30, 6)])
+def test_widths_between_vectors(dtype, rows, vocab, width):
+    g = torch.Generator().manual_seed(width)
+    tokens = _tokens(rows, vocab, "zipf")
+    table = torch.randn(vocab, width, generator=g).to(dtype).to(DEV).requires_grad_(True)
+    dy = torch.randn(rows, width, generator=g).to(dtype).to(DEV)
+    out = ops.embedding(tokens, table, scale=1.5, pad_idx=2, sorted_grad=True)
+    exact = 1.5 * table.detach().double()[tokens]
+    assert ((out.detach().double() - exact).abs() <= HALF[dtype] * exact.abs() + (2 ** -25 if dtype == torch.float16 else 0)).all()
+    grad = torch.autograd.grad(out, table, dy)[0]
+    held = dy.double() * (tokens != 2)[:, None]
+    want, size = (torch.zeros(vocab, width, dtype=torch.float64, device=DEV).index_add_(0, tokens, t) for t in (held, held.abs()))
+    _close(grad, 1.5 * want, 1.5 * size, torch.bincount(tokens, minlength=vocab), dtype)
+    assert torch.equal(grad, torch.autograd.grad(ops.embedding(tokens, table, scale=1.5, pad_idx=2, sorted_grad=True), table, dy)[0])
