@@ -8,7 +8,9 @@
 // passes, sums and then gradients, with a small kernel between that makes rows of the pieces and coefficients of the rows.  (Both passes at once, the gradients some rows behind the sums so
 // that they would find the logits in L2, were built and measured: 353 us against 272 for 8200 rows of 32000 in bf16.  The coefficient of a pair
 // comes so late that most blocks wait for it.)
-// Bound by memory in 32 bits and in every gradient pass; the sums of 16-bit logits are bound by exponentials, 16 a cycle and SM.
+// Bound by memory in 32 bits and in every gradient pass.  The sums of 16-bit logits, two exponentials to a 32-bit word, keep the memory at 0.8 of its
+// rate and the exponentials (16 a cycle and SM) at 0.7 of theirs; the policy loss of whole rows is at 0.85 of the memory's.
+// 8200 rows of 32000 in bf16: scores 98 us (floor 81), gradients 167 (163), policy loss 200 (163), paired loss 276 (163, of the two passes 244).
 //
 // All sums over rows are taken in one order in 64 bits: results do not depend on which block was first.
 // This file is compiled without fast math: expf and logf below are the accurate ones, ex2 where it is asked for.
