@@ -146,9 +146,13 @@ def token_logprobs(logits, labels, pad_idx: int = 0, temperature: float = 1.0):
 
 def sequence_logprobs(logprobs, cu):
     """Sums of the words' log-probabilities over the sequences of ``cu``: what ``preference_loss`` takes from the frozen model.  fp32, summed in
-    64 bits."""
-    ends = torch.cat([logprobs.new_zeros(1, dtype=torch.float64), logprobs.double().cumsum(0)])[cu.long()]
-    return (ends[1:] - ends[:-1]).to(logprobs.dtype)
+    64 bits.  A sequence with a word of probability 0, or with NaN, is that and no other one."""
+    sums = lambda t: torch.diff(torch.cat([t.new_zeros(1), t.cumsum(0)])[cu.long()])
+    lp = logprobs.double()
+    finite = torch.isfinite(lp)
+    total = sums(lp.masked_fill(~finite, 0.0))
+    total = total.masked_fill(sums((lp == -float("inf")).double()) > 0, -float("inf"))
+    return total.masked_fill(sums((~finite & (lp != -float("inf"))).double()) > 0, float("nan")).to(logprobs.dtype)
 
 
 # ---------------------------------------------------------------------------------------------------

@@ -532,3 +532,11 @@ def test_more_than_2_31_logits():
         ratio = grad[-7:].float() / torch.autograd.grad(pref.token_logprobs(leaf[-7:], y[-7:]), leaf, weight[-7:])[0][-7:].float()
         assert (ratio.nan_to_num(ratio[0, 0].item()) / ratio[0, 0] - 1).abs().max() <= 2 ** -6          # one coefficient; four roundings of bf16
     assert ops.check_status() == 0
+
+
+def test_a_word_of_probability_0_stays_in_its_sequence():
+    lp = torch.tensor([-1.0, -2.0, -math.inf, -0.5, -1.5, math.nan, -0.25, -math.inf, -3.0])
+    got = pref.sequence_logprobs(lp, torch.tensor([0, 2, 4, 5, 7, 7, 9]))
+    assert got[:3].tolist() == [-3.0, -math.inf, -1.5] and torch.isnan(got[3]) and got[4] == 0.0 and got[5] == -math.inf
+    leaf = lp[:2].clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(pref.sequence_logprobs(leaf, torch.tensor([0, 1, 2])).sum(), leaf)[0], torch.ones(2))
