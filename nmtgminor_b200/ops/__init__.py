@@ -229,8 +229,11 @@ class _LinearFn(torch.autograd.Function):
         z = empty_rows(M, N, x.device) if act != 0 else None  # pre-activation, needed by act'
         gemm(x, w, y, bias=bias, residual=residual, preact=z, act=act, dropout_p=dropout_p, seed=seed,
              stream_id=stream_id, gather=gather)
-        ctx.keep8 = (_keep8(x) if gw is not None else None, _keep8(z) if act != 0 else None, x.shape[1]) if keep8 else None
-        ctx.save_for_backward(None if keep8 else x, w, None if keep8 else z)
+        if keep8:
+            _save_kept(ctx, (None, w, None), _keep8(x) if gw is not None else None, _keep8(z) if act != 0 else None)
+        else:
+            ctx.save_for_backward(x, w, z)
+            ctx.kept = None
         ctx.cfg = (act, dropout_p, seed, stream_id, residual is not None, bias is not None, need_input_grad)
         ctx.gw, ctx.gb = gw, gb
         ctx.gather = gather
@@ -238,7 +241,7 @@ class _LinearFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        x, w, z = ctx.saved_tensors
+        x, w, z, kept_x, kept_z = _saved_kept(ctx, 3)
         act, p, seed, sid, has_res, has_bias, need_dx = ctx.cfg
         if dy.shape[1] % 8:
             padded = empty_rows(dy.shape[0], dy.shape[1], dy.device)
@@ -248,7 +251,6 @@ class _LinearFn(torch.autograd.Function):
             dy = dy.contiguous()
         want_gb = has_bias and ctx.gb is not None
         fused_gb = want_gb and act == 0 and p > 0.0 and _colsum_fusable(dy)
-        kept_x, kept_z, K = ctx.keep8 if ctx.keep8 is not None else (None, None, x.shape[1])
         if fused_gb:
             dz = ext().dropout_colsum(dy, p, seed, sid, ctx.gb)  # regenerated mask and bias gradient in one pass
         elif kept_z is not None:
@@ -274,7 +276,7 @@ class _LinearFn(torch.autograd.Function):
             ext().colsum(dz, ctx.gb)
         dx = None
         if need_dx:
-            dx = torch.empty((dy.shape[0], K), dtype=torch.bfloat16, device=dy.device)
+            dx = torch.empty((dy.shape[0], w.shape[1]), dtype=torch.bfloat16, device=dy.device)
             gemm(dz, w, dx, b_mn_major=True, gather=ctx.gather)
         return dx, None, None, (dy if has_res else None), None, None, None, None, None, None, None, None, None
 
@@ -282,6 +284,21 @@ class _LinearFn(torch.autograd.Function):
 def _keep8(x):
     from .kept import quantise
     return quantise(x)
+
+
+def _save_kept(ctx, tensors, *kept):
+    """Saves tensors and matrices in 8 bits (or None) for the backward pass, which frees them as it does all others."""
+    ctx.save_for_backward(*tensors, *(t for k in kept for t in ((k.codes, k.scales) if k is not None else (None, None))))
+    ctx.kept = tuple((k.width, k.dtype) if k is not None else None for k in kept)
+
+
+def _saved_kept(ctx, n):
+    """The ``n`` tensors and two matrices of ``_save_kept``; of ``save_for_backward`` without any, the tensors and None twice."""
+    saved = ctx.saved_tensors
+    if ctx.kept is None:
+        return (*saved, None, None)
+    from .kept import Kept
+    return (*saved[:n], *(Kept(*saved[n + 2 * i:n + 2 * i + 2], *k) if k is not None else None for i, k in enumerate(ctx.kept)))
 
 
 def _restore8(kept):
@@ -390,11 +407,10 @@ class _MlpFn(torch.autograd.Function):
         y = torch.empty((M, w2.shape[0]), dtype=torch.bfloat16, device=x.device)
         gemm(h, w2, y, bias=b2, residual=residual, dropout_p=p2, seed=seed, stream_id=sid2, gather=gather2)
         if keep8:
-            ctx.save_for_backward(None, w1, w2, None, bits)
-            ctx.keep8 = (_keep8(x) if g[0] is not None else None, _keep8(h if act == 1 else z))
+            _save_kept(ctx, (None, w1, w2, None, bits), _keep8(x) if g[0] is not None else None, _keep8(h if act == 1 else z))
         else:
             ctx.save_for_backward(x, w1, w2, h, z if z is not None else bits)
-            ctx.keep8 = None
+            ctx.kept = None
         ctx.cfg = (act, p1, p2, seed, sid1, sid2, residual is not None)
         ctx.g = g
         ctx.gathers = (gather1, gather2)
@@ -402,17 +418,17 @@ class _MlpFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        x, w1, w2, h, z = ctx.saved_tensors
+        x, w1, w2, h, z, kept_x, kept_h = _saved_kept(ctx, 5)
         act, p1, p2, seed, sid1, sid2, has_res = ctx.cfg
         gw1, gb1, gw2, gb2 = ctx.g
         dy = dy.contiguous()
-        if ctx.keep8 is not None:
+        if kept_h is not None:
             from .kept import restore_activated
-            x = _restore8(ctx.keep8[0]) if gw1 is not None else None
+            x = _restore8(kept_x) if gw1 is not None else None
             if act == 1:
-                h = _restore8(ctx.keep8[1])
+                h = _restore8(kept_h)
             else:
-                z, h = restore_activated(ctx.keep8[1], act, p1, seed, sid1, True)
+                z, h = restore_activated(kept_h, act, p1, seed, sid1, True)
         fused_gb2 = gb2 is not None and p2 > 0.0 and _colsum_fusable(dy)
         if fused_gb2:
             dz2 = ext().dropout_colsum(dy, p2, seed, sid2, gb2)
@@ -742,11 +758,10 @@ def embedding(tokens, table, positions=None, pos_table=None, scale=1.0, dropout_
     """out = dropout(table[tokens] * scale + pos_table[positions]) for 1-D packed ``tokens``.
 
     ``sorted_grad``: every row of the table's gradient (and of a trainable position table's) is summed in the order of the tokens, without atomic
-    additions, so that it repeats to the last bit (csrc/embed_sorted.cu); None: where ``torch.use_deterministic_algorithms`` asks for it.  It
-    then serves ordinary CUDA tables (bf16, fp16, fp32, any width) as well as those of the flat store.  Rows of padding give no gradient."""
+    additions, so that it repeats to the last bit (csrc/embed_sorted.cu).  True serves ordinary CUDA tables (bf16, fp16, fp32, any width) as well as
+    those of the flat store; rows of padding then give no gradient.  None: tables of the flat store where ``torch.use_deterministic_algorithms``
+    asks for it."""
     p = float(dropout_p) if training else 0.0
-    if sorted_grad is None:
-        sorted_grad = torch.are_deterministic_algorithms_enabled()
     if fused_param(table) and tokens.is_cuda and table.shape[1] % 16 == 0:
         sid = next_stream() if p > 0 else 0
         pt = None
@@ -759,7 +774,7 @@ def embedding(tokens, table, positions=None, pos_table=None, scale=1.0, dropout_
                 gpos = pos_table.main_grad
         gtable = table.main_grad if table.requires_grad else None
         if torch.is_grad_enabled() and (gtable is not None or gpos is not None):
-            if sorted_grad:
+            if torch.are_deterministic_algorithms_enabled() if sorted_grad is None else sorted_grad:
                 LAUNCHES[0] += 1 + 3 * (gtable is not None) + 3 * (gpos is not None)
                 return ext().embed_flat_node(_grad_anchor(tokens.device), tokens, positions, table.work, pt, gtable, gpos, float(scale), p,
                                              _Rng.seed, sid, int(pad_idx))

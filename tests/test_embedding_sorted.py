@@ -235,3 +235,17 @@ def test_widths_between_vectors(dtype, rows, vocab, width):
     want, size = (torch.zeros(vocab, width, dtype=torch.float64, device=DEV).index_add_(0, tokens, t) for t in (held, held.abs()))
     _close(grad, 1.5 * want, 1.5 * size, torch.bincount(tokens, minlength=vocab), dtype)
     assert torch.equal(grad, torch.autograd.grad(ops.embedding(tokens, table, scale=1.5, pad_idx=2, sorted_grad=True), table, dy)[0])
+
+
+def test_plain_tables_keep_their_own_gradient_unless_asked():
+    """Deterministic algorithms change the flat store's gradients alone: an ordinary table's are PyTorch's, padding included, as ever."""
+    table = torch.randn(6, 3, requires_grad=True)
+    tokens = torch.tensor([[1, 0], [2, 1]], dtype=torch.int32)
+    want = torch.autograd.grad(ops.embedding(tokens, table, pad_idx=0).sum(), table)[0]
+    before = torch.are_deterministic_algorithms_enabled()
+    try:
+        torch.use_deterministic_algorithms(True)
+        assert torch.equal(torch.autograd.grad(ops.embedding(tokens, table, pad_idx=0).sum(), table)[0], want)
+    finally:
+        torch.use_deterministic_algorithms(before)
+    assert want[0].sum() != 0

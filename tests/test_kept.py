@@ -376,3 +376,24 @@ def test_more_than_2_31_elements():
         del dy, y
         assert torch.equal(kept.restore(kept.quantise(z.detach()))[-5:], kept.restore(kept.quantise(few.detach())))
         del z
+
+
+@pytest.mark.gpu
+def test_what_waits_is_freed_with_the_pass():
+    """The codes are saved tensors: the backward pass frees them while the result lives, a second one is refused, and a kept graph serves two."""
+    rows, K, N = 2048, 512, 1024
+    x = torch.randn(rows, K, device=DEV).bfloat16().requires_grad_(True)
+    w1, w2 = _Store.param((N, K), 0.04, 1), _Store.param((K, N), 0.02, 2)
+    for f in (lambda: ops.linear(x, w1, None, "gelu", keep8=True), lambda: ops.mlp(x, w1, None, w2, None, "relu", keep8=True),
+              lambda: ops.mlp(x, w1, None, w2, None, "gelu", keep8=True), lambda: kept.activation(x, "silu")):
+        y = f()
+        ones = torch.ones_like(y)
+        first = torch.autograd.grad(y, x, ones, retain_graph=True)[0]
+        assert torch.equal(torch.autograd.grad(y, x, ones, retain_graph=True)[0], first)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        y.backward(ones)
+        x.grad = None
+        assert torch.cuda.memory_allocated() <= before - 33 * rows * K // 32
+        with pytest.raises(RuntimeError):
+            y.backward(ones)
