@@ -776,7 +776,7 @@ def embedding(tokens, table, positions=None, pos_table=None, scale=1.0, dropout_
         if torch.is_grad_enabled() and (gtable is not None or gpos is not None):
             if torch.are_deterministic_algorithms_enabled() if sorted_grad is None else sorted_grad:
                 LAUNCHES[0] += 1 + 3 * (gtable is not None) + 3 * (gpos is not None)
-                return ext().embed_flat_node(_grad_anchor(tokens.device), tokens, positions, table.work, pt, gtable, gpos, float(scale), p,
+                return ext().embed_flat_node(tokens, positions, table.work, pt, gtable, gpos, float(scale), p,
                                              _Rng.seed, sid, int(pad_idx))
             return _EmbedFn.apply(_grad_anchor(tokens.device), tokens, positions, table.work, pt, gtable, gpos, scale, p,
                                   _Rng.seed, sid, pad_idx)

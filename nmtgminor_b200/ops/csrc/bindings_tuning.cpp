@@ -460,7 +460,8 @@ struct EmbedNode : Function<EmbedNode> {
   }
 };
 
-// A table of the flat store: gradients are added to the store's buffers.  `anchor` is a tensor with a gradient that keeps the node alive.
+// A table of the flat store: gradients are added to the store's buffers.  `anchor` is an empty tensor with a gradient that makes autograd record the node:
+// one of the call's own, since a leaf that an eager graph holds, too, could not be passed in a backward pass that is being captured.
 struct FlatEmbedNode : Function<FlatEmbedNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& /*anchor*/, const Tensor& tokens, const OptTensor& positions, const Tensor& table,
                         const OptTensor& pos_table, const OptTensor& gtable, const OptTensor& gpos, double scale, double p, int64_t seed,
@@ -539,8 +540,9 @@ void bind_tuning_ops(pybind11::module& m) {
   m.def("embed_rows_node", [](const Tensor& table, const Tensor& tokens, double scale, int64_t pad) {
     return EmbedNode::apply(table, tokens, scale, pad);
   });
-  m.def("embed_flat_node", [](const Tensor& anchor, const Tensor& tokens, const OptTensor& positions, const Tensor& table, const OptTensor& pos_table,
+  m.def("embed_flat_node", [](const Tensor& tokens, const OptTensor& positions, const Tensor& table, const OptTensor& pos_table,
                               const OptTensor& gtable, const OptTensor& gpos, double scale, double p, int64_t seed, int64_t stream_id, int64_t pad) {
+    const Tensor anchor = at::empty({0}, table.options().dtype(at::kFloat)).requires_grad_(true);
     return FlatEmbedNode::apply(anchor, tokens, positions, table, pos_table, gtable, gpos, scale, p, seed, stream_id, pad);
   });
   m.def("activation_node", [](const Tensor& z, int64_t act, double p, int64_t seed, int64_t stream_id) {

@@ -12,7 +12,8 @@ but -inf have NaN, as ``torch.log_softmax`` has.
 The gradient tensor of the two losses belongs to the backward pass, so a second pass through the same loss (``retain_graph``) is refused.
 ``grad_scale`` (a float, or one fp32 element on the logits' device that is read when the kernel runs) multiplies the gradient where it is
 computed; the upstream gradient of the loss is then taken to be 1, as in ``ops.generator_cross_entropy``.  Without it an upstream gradient
-other than 1 costs another pass over the gradient.  ``inplace`` writes the gradient over the logits, which are consumed (as ``ops.cross_entropy``
+other than 1 costs another pass over the gradient.  A backward pass can be captured in a CUDA graph where, as PyTorch asks of every operator, no graph
+of the same leaves made outside the capture is alive.  ``inplace`` writes the gradient over the logits, which are consumed (as ``ops.cross_entropy``
 consumes its own).
 """
 from __future__ import annotations

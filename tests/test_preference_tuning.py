@@ -223,3 +223,38 @@ def test_wrapper_trains_through_a_captured_step():
         # words of 2^4 each), times beta and the slope of 1 / 2
         assert abs(run[0] - pairs * math.log(2.0)) <= 2 ** -16 * pairs
     assert ops.check_status() == 0
+
+
+@pytest.mark.gpu
+def test_a_captured_pass_beside_a_living_eager_graph():
+    """The flat store's chain has no leaf in common with other calls: its backward pass is captured while an eager graph of the same parameters lives."""
+    g = torch.Generator().manual_seed(4)
+    table, w, out = (_flat(torch.randn(*shape, generator=g).bfloat16() * 0.1) for shape in ((300, 64), (128, 64), (300, 128)))
+    tokens, labels = (torch.randint(1, 300, (90,), generator=g).cuda() for _ in range(2))
+    cu = torch.tensor([0, 30, 50, 70, 90]).int().cuda()
+
+    def forward():
+        x = ops.embedding(tokens, table, sorted_grad=True)
+        return pref.preference_loss(ops.linear(ops.linear(x, w, None, "relu", keep8=True), out, keep8=True), labels, cu, inplace=True)[0]
+
+    def step():
+        for p in (table, w, out):
+            p.main_grad.zero_()
+        loss = forward()
+        loss.backward()
+        return loss.detach()
+
+    alive = forward()
+    want, grads = step().clone(), [p.main_grad.clone() for p in (table, w, out)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = step()
+    for p in (table, w, out):
+        p.main_grad.fill_(7.0)
+    graph.replay()
+    assert torch.equal(loss, want)
+    for p, grad in zip((table, w, out), grads):
+        assert (p.main_grad - grad).norm() <= 2 ** -16 * grad.norm()        # split sums are added in any order
+    alive.backward()
+    assert ops.check_status() == 0
