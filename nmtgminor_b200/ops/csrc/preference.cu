@@ -10,7 +10,7 @@
 // comes so late that most blocks wait for it.)
 // Bound by memory in 32 bits and in every gradient pass.  The sums of 16-bit logits, two exponentials to a 32-bit word, keep the memory at 0.8 of its
 // rate and the exponentials (16 a cycle and SM) at 0.7 of theirs; the policy loss of whole rows is at 0.85 of the memory's.
-// 8200 rows of 32000 in bf16: scores 98 us (floor 81), gradients 167 (163), policy loss 200 (163), paired loss 276 (163, of the two passes 244).
+// 8200 rows of 32000 in bf16: scores 96 us (floor 81), gradients 165 (163), policy loss 206 (163), paired loss 255 (163, of the two passes 244).
 //
 // All sums over rows are taken in one order in 64 bits: results do not depend on which block was first.
 // This file is compiled without fast math: expf and logf below are the accurate ones, ex2 where it is asked for.
@@ -26,6 +26,7 @@
 namespace b200 {
 
 int num_sms();
+bool launch_overlap();
 
 namespace {
 
@@ -61,6 +62,8 @@ struct Args {
   int rows, vocab;
   int pieces, each;         // of a row; vectors of a piece
   int slot;                 // vectors of a slot
+  int behind;               // launched while the kernel before it ends
+  int stays;                // first row that is to stay in L2 after the sums
   int aligned;              // every row starts on a 16-byte boundary
   float k, inv_t;           // log2(e) / T, 1 / T
   float* logprobs;
@@ -163,6 +166,19 @@ __device__ __forceinline__ float warp_max(float v) {
 }
 __device__ __forceinline__ void copy16(uint4* to, const uint4* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+// For the sums, whose rows are read again by the gradients: these go from the last row to the first, and find in L2 what the sums read last, the rows
+// from `stays` on; the rows before pass through it first out.  (Paired loss of 8200 rows of 32000 in bf16: 276 us in one order, 273 with the gradients
+// from the last row, 261 so; 8200 rows of 8000 in fp32 151, 144, 136.  48 to 80 MB alike, 112 of the 126 that L2 has 2 % slower.)
+constexpr long kStaying = 48L << 20;
+__device__ __forceinline__ uint64_t policy_of(bool stay) {
+  uint64_t first, normal;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(first));
+  asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(normal));
+  return stay ? normal : first;
+}
+__device__ __forceinline__ void copy16(uint4* to, const uint4* from, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "l"(policy) : "memory");
 }
 __device__ __forceinline__ void copy4(void* to, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)), "l"(from) : "memory");
@@ -310,6 +326,8 @@ __global__ void __launch_bounds__(kCompute + 32, kCompute == kBlock ? 3 : 1) row
   constexpr bool kSums = kMode != kGrad, kGrads = kMode != kScores;
   constexpr int kLead = kMode == kScores ? kSlots : kSlots - 1;             // entries whose logits are under way
   extern __shared__ __align__(16) uint4 slots[];            // [kSlots][a.slot]
+  if (a.behind) wait_for_previous();
+  if (kMode == kLocal || (kMode == kScores && a.w.part)) let_next_start();
   __shared__ float2 part[2][kWarps];
   __shared__ float4 bc[2];                                  // largest logit, factor of the exponentials, coefficient / T
   __shared__ Entry ring[kRing];
@@ -331,8 +349,8 @@ __global__ void __launch_bounds__(kCompute + 32, kCompute == kBlock ? 3 : 1) row
       return a.w.ticket ? kFirst * static_cast<int>(gridDim.x) + atomicAdd(a.w.ticket, 1) : a.rows * a.pieces;
     };
     const auto ask = [&](int i, int number) {                 // lane 0
-      const int q = a.pieces == 1 ? number : number / a.pieces;
-      const Entry e = {q < a.rows ? q : -1, number - q * a.pieces, -1, 0};
+      const int items = a.rows * a.pieces, n = kMode == kGrad ? items - 1 - number : number, q = a.pieces == 1 ? n : n / a.pieces;
+      const Entry e = {number < items ? q : -1, n - q * a.pieces, -1, 0};
       Mail& m = mail[i & (kRing - 1)];
       if (e.row < 0) m.label = -1;
       else if (a.w.label) copy4(&m.label32, a.w.label + e.row);
@@ -444,9 +462,16 @@ __global__ void __launch_bounds__(kCompute + 32, kCompute == kBlock ? 3 : 1) row
       const uint4* from = reinterpret_cast<const uint4*>(x + s.head) + s.v0 + t;
       uint4* to = slots + (i % kSlots) * a.slot + t;
       const int left = s.v1 - s.v0 - t;
+      if constexpr (kMode == kScores) {
+        const uint64_t policy = policy_of(n.row >= a.stays);
 #pragma unroll
-      for (int j = 0; j < kVecs; ++j)
-        if (j * kCompute < left) copy16(to + j * kCompute, from + j * kCompute);
+        for (int j = 0; j < kVecs; ++j)
+          if (j * kCompute < left) copy16(to + j * kCompute, from + j * kCompute, policy);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j)
+          if (j * kCompute < left) copy16(to + j * kCompute, from + j * kCompute);
+      }
     }
     copies_end();
   };
@@ -554,6 +579,8 @@ template <typename T>
 __global__ void __launch_bounds__(kSumWarps * 32, kSumBlocks) sums_kernel(const __grid_constant__ Args a) {
   constexpr int kE = Num<T>::kE;
   extern __shared__ __align__(16) uint4 slots[];            // [kSumWarps][kSumStages][kSumStage]
+  if (a.behind) wait_for_previous();
+  if (a.w.part) let_next_start();
   __shared__ int4 rings[kSumWarps][kSumRing];                      // row, piece, label
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const T* const x0 = static_cast<const T*>(a.x);
@@ -607,9 +634,10 @@ __global__ void __launch_bounds__(kSumWarps * 32, kSumBlocks) sums_kernel(const 
   int slot = 0;
   const auto issue = [&](int to) {
     if (prow >= 0) {
+      const uint64_t policy = policy_of(prow >= a.stays);
 #pragma unroll
       for (int j = 0; j < kSumVecs; ++j)
-        if (at + lane + j * 32 < end) copy16(mine + to * kSumStage + j * 32, from + at + j * 32);
+        if (at + lane + j * 32 < end) copy16(mine + to * kSumStage + j * 32, from + at + j * 32, policy);
       at += kSumStage;
       if (at >= end) fetch();
     }
@@ -755,6 +783,7 @@ __global__ void __launch_bounds__(1024) pairs_setup_kernel(const __grid_constant
   __shared__ int bounds[1025];
   __shared__ int warp_top[32];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, n = 2 * a.pairs.pairs + 1;
+  let_next_start();
   const auto none = [&](int begin, int end) {                // rows outside every sequence
     for (int r = begin + static_cast<int>(blockIdx.x) * 1024 + t; r < end; r += static_cast<int>(gridDim.x) * 1024) { a.w.seq[r] = -1; a.w.label[r] = -1; }
   };
@@ -795,6 +824,8 @@ __global__ void __launch_bounds__(128) pairs_kernel(const __grid_constant__ Args
   __shared__ int counts[2][4];
   __shared__ int last;
   const int p = static_cast<int>(blockIdx.x), t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  wait_for_previous();
+  let_next_start();
   const int begin = a.w.cu[2 * p], middle = a.w.cu[2 * p + 1], end = a.w.cu[2 * p + 2];
   double sum[2] = {0.0, 0.0};
   int count[2] = {0, 0};
@@ -852,6 +883,7 @@ __global__ void __launch_bounds__(128) pairs_kernel(const __grid_constant__ Args
 template <typename T>
 __global__ void __launch_bounds__(128) whole_rows_kernel(const __grid_constant__ Args a) {
   const int row = static_cast<int>(blockIdx.x * 128 + threadIdx.x);
+  wait_for_previous();
   if (row >= a.rows) return;
   const int64_t y = a.labels[row];
   const bool real = y != a.pad && y >= 0 && y < a.vocab;
@@ -876,6 +908,7 @@ constexpr int kSumThreads = 512, kSumEach = 4;
 __global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(kSumThreads) policy_sums_kernel(const __grid_constant__ Args a) {
   __shared__ double warps[3][kSumThreads / 32];
   __shared__ double block_sums[3];
+  wait_for_previous();
   double sums[3] = {0.0, 0.0, 0.0};                             // the loss, the KL terms, the clipped words
   for (int r0 = blockIdx.x * kSumThreads + threadIdx.x; r0 < a.rows; r0 += kSumEach * 8 * kSumThreads) {
     int64_t y[kSumEach];
@@ -952,6 +985,24 @@ __global__ void __launch_bounds__(256) scale_rows_kernel(const Args a, const flo
 
 const char* problem(cudaError_t e) { return e == cudaSuccess ? nullptr : cudaGetErrorString(e); }
 
+// `kernel` calls wait_for_previous() before it touches memory.  It may be scheduled before the kernel of this call in front of it has ended, where that one lets
+// it: its start, 2 to 3 us, then costs nothing (paired loss of 8200 rows of 32000 in bf16 260 -> 255 us, of 300 rows of 8000 29 -> 23; policy
+// loss of 20000 rows of 8000 145 -> 135).  Not behind a cleared ticket, which is no kernel.
+template <typename... P, typename... A>
+const char* launch_behind(bool may, void (*kernel)(P...), int grid, int threads, int smem, cudaStream_t stream, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = may && launch_overlap() ? 1 : 0;
+  return problem(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+
 // The ticket of a pass, unless every block has its items without asking; the paired loss has zeroed it before
 const char* set_ticket(Args& a, int pass, bool none, cudaStream_t stream) {
   a.w.ticket = none ? nullptr : a.w.state->tickets + pass;
@@ -983,8 +1034,8 @@ const char* launch_rows(const Args& from, cudaStream_t stream) {
   const int grid = static_cast<int>(items < most ? items : most);
   const char* err = set_ticket(a, kMode == kGrad, items <= kFirst * most, stream);
   if (err) return err;
-  kernel<<<grid, kCompute + 32, smem, stream>>>(a);
-  return problem(cudaGetLastError());
+  a.behind = kMode != kLocal && a.pairs.pairs > 0;          // behind the kernels of the paired loss
+  return launch_behind(a.behind, kernel, grid, kCompute + 32, smem, stream, a);
 }
 
 template <typename T>
@@ -997,8 +1048,8 @@ const char* launch_sums(Args a, cudaStream_t stream) {
   const char* err = set_ticket(a, 0, items <= 2 * blocks * kSumWarps, stream);       // two to a warp without asking
   if (err) return err;
   const int grid = static_cast<int>(items < blocks ? items : blocks);
-  sums_kernel<T><<<grid, kSumWarps * 32, smem, stream>>>(a);
-  return problem(cudaGetLastError());
+  a.behind = a.pairs.pairs > 0;
+  return launch_behind(a.behind, sums_kernel<T>, grid, kSumWarps * 32, smem, stream, a);
 }
 
 template <typename T> constexpr int warp_row() { return 32 * kVecs * Num<T>::kE; }       // elements that a warp holds
@@ -1071,10 +1122,8 @@ const char* launch_pass(Args a, int dtype, cudaStream_t stream) {
                                                                                  : launch_rows<__half, kBlock, kMode>(a, stream);
   if (kMode != kScores || err || a.pairs.pairs > 0 || !a.w.part) return err;
   const int blocks = (a.rows + 127) / 128;
-  if (dtype == 0) whole_rows_kernel<float><<<blocks, 128, 0, stream>>>(a);
-  else if (dtype == 1) whole_rows_kernel<__nv_bfloat16><<<blocks, 128, 0, stream>>>(a);
-  else whole_rows_kernel<__half><<<blocks, 128, 0, stream>>>(a);
-  return problem(cudaGetLastError());
+  return launch_behind(true, dtype == 0 ? whole_rows_kernel<float> : dtype == 1 ? whole_rows_kernel<__nv_bfloat16> : whole_rows_kernel<__half>, blocks, 128, 0,
+                       stream, a);
 }
 
 template <typename T>
@@ -1096,6 +1145,8 @@ Args row_args(const NmtgRows* r) {
   a.logprobs = r->logprobs; a.stat = r->stat;
   a.pieces = 1;
   a.each = a.vocab;
+  const long staying = kStaying / (r->vocab * (r->dtype == 0 ? 4L : 2L));
+  a.stays = r->rows > staying ? static_cast<int>(r->rows - staying) : 0;
   return a;
 }
 
@@ -1174,8 +1225,7 @@ const char* nmtg_policy_loss(const NmtgRows* r, const NmtgPolicy* p, cudaStream_
     if (!err && a.g) err = launch_pass<kGrad>(a, r->dtype, stream);
   }
   if (err) return err;
-  policy_sums_kernel<<<8, kSumThreads, 0, stream>>>(a);
-  return problem(cudaGetLastError());
+  return launch_behind(r->rows > 0, policy_sums_kernel, 8, kSumThreads, 0, stream, a);
 }
 
 const char* nmtg_preference_loss(const NmtgRows* r, const NmtgPairs* p, cudaStream_t stream) {
@@ -1205,10 +1255,8 @@ const char* nmtg_preference_loss(const NmtgRows* r, const NmtgPairs* p, cudaStre
     scores = a;
     scores.pieces = is_short ? 1 : pieces;
     scores.stat = is_short ? w.stat : nullptr;
-    if (r->dtype == 0) pairs_kernel<float><<<p->pairs, 128, 0, stream>>>(scores);
-    else if (r->dtype == 1) pairs_kernel<__nv_bfloat16><<<p->pairs, 128, 0, stream>>>(scores);
-    else pairs_kernel<__half><<<p->pairs, 128, 0, stream>>>(scores);
-    err = problem(cudaGetLastError());
+    err = launch_behind(!is_short, r->dtype == 0 ? pairs_kernel<float> : r->dtype == 1 ? pairs_kernel<__nv_bfloat16> : pairs_kernel<__half>, p->pairs, 128, 0,
+                        stream, scores);
     if (err) return err;
   }
   if (!a.g) return nullptr;
