@@ -3,14 +3,15 @@
 //     lp = (x[y] - M) / T - log s          d lp / d x = (onehot(y) - exp((x - M) / T) / s) / T
 // Each loss is a function of the lp of its rows, so a row's gradient is one coefficient times d lp / d x.
 //
-// rows_kernel takes a piece of a row at a time: its sums, or its gradient, or for the policy loss of rows that a block holds both, the logits
-// read once.  Scores of rows in one piece are complete with it.  The paired loss, and the scores and the policy loss of longer rows, are two
-// passes, sums and then gradients, with a small kernel between that makes rows of the pieces and coefficients of the rows.  (Both passes at once, the gradients some rows behind the sums so
-// that they would find the logits in L2, were built and measured: 353 us against 272 for 8200 rows of 32000 in bf16.  The coefficient of a pair
-// comes so late that most blocks wait for it.)
-// Bound by memory in 32 bits and in every gradient pass.  The sums of 16-bit logits, two exponentials to a 32-bit word, keep the memory at 0.8 of its
-// rate and the exponentials (16 a cycle and SM) at 0.7 of theirs; the policy loss of whole rows is at 0.85 of the memory's.
-// 8200 rows of 32000 in bf16: scores 96 us (floor 81), gradients 165 (163), policy loss 206 (163), paired loss 255 (163, of the two passes 244).
+// The policy loss of rows that an SM's shared memory holds is one pass, a block to a row (held_rows_kernel), or a warp to a short one.  Scores of rows in one
+// piece are one pass, too.  The paired loss, and the scores and the policy loss of longer rows, are two passes over pieces of rows, sums (sums_kernel, rows_kernel) and
+// then gradients (rows_kernel), with a small kernel between that makes rows of the pieces and coefficients of the rows.  (Both at once, the
+// gradients some rows behind the sums so that they would find the logits in L2, were built and measured: 353 us against 272 for 8200 rows of 32000 in bf16.
+// The coefficient of a pair comes so late that most blocks wait for it.)
+// Bound by memory in 32 bits, in every gradient pass and where one pass does all.  The sums of 16-bit logits, two exponentials to a 32-bit word, keep the
+// memory at 0.8 of its rate and the exponentials (16 a cycle and SM) at 0.7 of theirs.
+// 8200 rows of 32000 in bf16: scores 96 us (floor 81), gradients 165 (163), paired loss 255 (163, of the two passes 244); policy loss of
+// 15360 rows 317 (305).
 //
 // All sums over rows are taken in one order in 64 bits: results do not depend on which block was first.
 // This file is compiled without fast math: expf and logf below are the accurate ones, ex2 where it is asked for.
@@ -35,8 +36,9 @@ constexpr int kSlots = 3;             // items in shared memory or on their way 
 constexpr int kRing = 8;              // entries of work known: one behind, kSlots + 3 ahead, and that in hand
 constexpr int kFirst = 6;             // items of a block that it need not ask for
 constexpr int kBlock = 256, kWide = 512;      // threads of a block for the elements; two or three blocks to an SM, and one
+constexpr int kHeldBytes = 224 * 1024;        // of a row that a block's shared memory holds
 
-// kScores: sums of pieces.  kGrad: gradients from `stat` or `part` and a coefficient.  kLocal: the policy loss of rows that one block holds.
+// kScores: sums of pieces.  kGrad: gradients from `stat` and a coefficient.  kLocal: the policy loss of rows that a warp holds.
 enum Mode { kScores = 0, kGrad = 1, kLocal = 2 };
 
 struct State { int tickets[2], pairs_done; };      // items asked for in the two passes
@@ -306,7 +308,7 @@ struct __align__(16) Mail {
   float2 stat;
   uint32_t word, upper;     // the label's logit, of 16 bits the upper half where `upper`
   int seq;
-  float old, adv, ref;      // kGrad: `old` is the weight
+  float weight;
 };
 
 // d loss / d lp of a row under the policy loss
@@ -323,11 +325,11 @@ __device__ __forceinline__ float policy_coef(const Args& a, LogProb lp, float ol
 template <typename T, int kCompute, int kMode>
 __global__ void __launch_bounds__(kCompute + 32, kCompute == kBlock ? 3 : 1) rows_kernel(const __grid_constant__ Args a) {
   constexpr int kE = Num<T>::kE, kWarps = kCompute / 32;
-  constexpr bool kSums = kMode != kGrad, kGrads = kMode != kScores;
+  constexpr bool kSums = kMode == kScores, kGrads = kMode == kGrad;
   constexpr int kLead = kMode == kScores ? kSlots : kSlots - 1;             // entries whose logits are under way
   extern __shared__ __align__(16) uint4 slots[];            // [kSlots][a.slot]
   if (a.behind) wait_for_previous();
-  if (kMode == kLocal || (kMode == kScores && a.w.part)) let_next_start();
+  if (kMode == kScores && a.w.part) let_next_start();
   __shared__ float2 part[2][kWarps];
   __shared__ float4 bc[2];                                  // largest logit, factor of the exponentials, coefficient / T
   __shared__ Entry ring[kRing];
@@ -339,7 +341,7 @@ __global__ void __launch_bounds__(kCompute + 32, kCompute == kBlock ? 3 : 1) row
   if (warp == kWarps) {
     // ------------------------------------------------------------------------------------------------ the last warp
     const float scale = a.scale_at ? *a.scale_at * a.scale : a.scale;
-    const bool whole = kMode == kLocal || (kMode == kScores && !a.w.part);      // an item is a row, and its log-probability wanted
+    const bool whole = kMode == kScores && !a.w.part;        // an item is a row, and its log-probability wanted
     // What an entry needs comes by asynchronous copies, so that this warp never waits for memory: at step i the label of entry i + kLead + 3, at step
     // i + 2, when its label is there and the entry is published, its logit and the numbers of its row.
     // A block's first kFirst items are its own, the others are handed out one by one, asked for a step ahead: SMs do not get at memory equally fast,
@@ -372,14 +374,9 @@ __global__ void __launch_bounds__(kCompute + 32, kCompute == kBlock ? 3 : 1) row
           m.upper = at & 2;
           copy4(&m.word, reinterpret_cast<const void*>(at & ~static_cast<uintptr_t>(3)));
         }
-        if constexpr (kMode == kLocal) {
-          copy4(&m.old, a.policy.old_logprobs + e.row);
-          copy4(&m.adv, a.policy.advantages + e.row);
-          if (a.policy.ref_logprobs) copy4(&m.ref, a.policy.ref_logprobs + e.row);
-        }
         if constexpr (kMode == kGrad) {
           copy8(&m.stat, a.stat + e.row);
-          copy4(&m.old, a.weight + (a.w.seq ? m.seq : e.row));
+          copy4(&m.weight, a.weight + (a.w.seq ? m.seq : e.row));
         }
       }
     };
@@ -418,7 +415,7 @@ __global__ void __launch_bounds__(kCompute + 32, kCompute == kBlock ? 3 : 1) row
         if constexpr (kMode == kGrad) {
           if (lane == 0) {
             const float2 st = letter.stat;
-            const float c = real ? letter.old * a.inv_t * scale : 0.f;
+            const float c = real ? letter.weight * a.inv_t * scale : 0.f;
             bc[(i - 1) & 1] = make_float4(st.x, __fdividef(c, st.y), c, 0.f);
           }
         } else {
@@ -433,13 +430,7 @@ __global__ void __launch_bounds__(kCompute + 32, kCompute == kBlock ? 3 : 1) row
             } else {
               const LogProb lp = real ? log_probability(logit_of(letter), m, sum, a.inv_t) : LogProb{0.f, 0.f};
               a.logprobs[row] = lp.hi;
-              if constexpr (kMode == kScores) {
-                if (a.stat) a.stat[row] = real ? make_float2(m, sum) : make_float2(0.f, 1.f);
-              } else {
-                const float c = real ? policy_coef(a, lp, letter.old, letter.adv, letter.ref) * a.inv_t * scale : 0.f;
-                bc[(i - 1) & 1] = make_float4(m, __fdividef(c, sum), c, 0.f);
-                a.w.lp[row] = lp.wide();
-              }
+              if (a.stat) a.stat[row] = real ? make_float2(m, sum) : make_float2(0.f, 1.f);
             }
           }
         }
@@ -698,6 +689,114 @@ __global__ void __launch_bounds__(kSumWarps * 32, kSumBlocks) sums_kernel(const 
     }
   }
   copies_wait<0>();
+}
+
+// The policy loss of a row that a block's shared memory holds, a block to a row: every thread copies its vectors, adds them up as they arrive in four
+// groups, and goes over them again for the gradient.  Nothing is carried from row to row: while a block waits for its row, or for the coefficient, others of the SM
+// compute and store, and rows go to SMs as they become free.  (A block that stays and reads the next rows meanwhile, three slots and a warp for the
+// coefficients, was built before: 15360 rows of 32000 in bf16 360 us for 317, 3584 of 51865, which it could not hold, 195 for 138.)
+constexpr int kHeldGroups = 4, kHeldVecs = 4;             // vectors that a thread has in registers
+template <typename T, int kThreads, int kBlocks>
+__global__ void __launch_bounds__(kThreads, kBlocks) held_rows_kernel(const __grid_constant__ Args a) {
+  constexpr int kE = Num<T>::kE, kWarps = kThreads / 32;
+  extern __shared__ __align__(16) uint4 held[];
+  __shared__ float2 part[kWarps];
+  __shared__ float4 bc;
+  let_next_start();
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, row = static_cast<int>(blockIdx.x);
+  const T* const x = static_cast<const T*>(a.x) + static_cast<long>(row) * a.ld;
+  T* const g = a.g ? static_cast<T*>(a.g) + static_cast<long>(row) * a.ld : nullptr;
+  const Shape s = shape_of(a, x, 0);
+  const uint4* const from = reinterpret_cast<const uint4*>(x + s.head);
+  const int64_t y = a.labels[row];
+  const int each = (s.nvec + kHeldGroups * kThreads - 1) / (kHeldGroups * kThreads) * kThreads;      // vectors of a group
+#pragma unroll
+  for (int q = 0; q < kHeldGroups; ++q) {
+    const int end = min(s.nvec, (q + 1) * each);
+#pragma unroll 4
+    for (int v = q * each + t; v < end; v += kThreads) copy16(held + v, from + v);
+    copies_end();
+  }
+  const bool real = y != a.pad && y >= 0 && y < a.vocab;
+  const int label = real ? static_cast<int>(y) : -1, e1 = single_at<T>(s, t, 0, 1);
+  uint4* const out = reinterpret_cast<uint4*>(g + s.head);
+  if (!real) {
+    if (t == 0) { a.logprobs[row] = 0.f; a.w.lp[row] = 0.0; }
+    if (g) {
+      for (int v = t; v < s.nvec; v += kThreads) __stcs(out + v, make_uint4(0, 0, 0, 0));
+      if (e1 >= 0) g[e1] = Num<T>::put(0.f);
+    }
+    copies_wait<0>();
+    return;
+  }
+  const float one = e1 >= 0 ? Num<T>::get(x[e1]) : -INFINITY;
+  float xy = 0.f, old = 0.f, adv = 0.f, ref = 0.f, scale = 0.f;
+  if (warp == 0) {
+    xy = Num<T>::get(x[label]);
+    old = a.policy.old_logprobs[row];
+    adv = a.policy.advantages[row];
+    if (a.policy.ref_logprobs) ref = a.policy.ref_logprobs[row];
+    scale = a.scale_at ? *a.scale_at * a.scale : a.scale;
+  }
+  float m = one, sum = one == -INFINITY ? 0.f : 1.f;
+#pragma unroll
+  for (int q = 0; q < kHeldGroups; ++q) {
+    if (q == 0) copies_wait<3>(); else if (q == 1) copies_wait<2>(); else if (q == 2) copies_wait<1>(); else copies_wait<0>();
+    const int end = min(s.nvec, (q + 1) * each);
+#pragma unroll 1
+    for (int v = q * each + t; v < end; v += kHeldVecs * kThreads) {
+      uint4 raw[kHeldVecs];
+#pragma unroll
+      for (int j = 0; j < kHeldVecs; ++j)
+        raw[j] = v + j * kThreads < end ? held[v + j * kThreads] : make_uint4(Num<T>::kLow, Num<T>::kLow, Num<T>::kLow, Num<T>::kLow);
+      float top = m;
+#pragma unroll
+      for (int j = 0; j < kHeldVecs; ++j) top = fmaxf(top, Num<T>::largest(raw[j]));
+      const float base = top == -INFINITY ? 0.f : top;
+      float2 total[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int j = 0; j < kHeldVecs; ++j) {
+        if (j > 0 && v + j * kThreads >= end) break;
+        float2 e[kE / 2];
+        exps<T>(raw[j], -base, a.k, e);
+#pragma unroll
+        for (int p = 0; p < kE / 2; ++p) total[p & 1] = add2(total[p & 1], e[p]);
+      }
+      total[0] = add2(total[0], total[1]);
+      sum = fmaf(sum, ex2((m - base) * a.k), total[0].x + total[0].y);
+      m = top;
+    }
+  }
+  join_lanes(m, sum, a.k);
+  if (lane == 0) part[warp] = make_float2(m, sum);
+  __syncthreads();
+  if (warp == 0) {
+    m = lane < kWarps ? part[lane].x : -INFINITY;
+    sum = lane < kWarps ? part[lane].y : 0.f;
+    join_lanes(m, sum, a.k);
+    const LogProb lp = log_probability(xy, m, sum, a.inv_t);
+    const float c = policy_coef(a, lp, old, adv, ref) * a.inv_t * scale;
+    if (lane == 0) {
+      bc = make_float4(m, __fdividef(c, sum), c, 0.f);
+      a.logprobs[row] = lp.hi;
+      a.w.lp[row] = lp.wide();
+    }
+  }
+  __syncthreads();
+  if (!g) return;
+  const float4 c = bc;
+#pragma unroll 4
+  for (int v = t; v < s.nvec; v += kThreads) {
+    float2 e[kE / 2];
+    exps<T>(held[v], -c.x, a.k, e);
+#pragma unroll
+    for (int q = 0; q < kE / 2; ++q) e[q] = mul2(e[q], make_float2(-c.y, -c.y));
+    __stcs(out + v, Num<T>::pack(e));
+  }
+  if (e1 >= 0) g[e1] = Num<T>::put((e1 == label ? c.z : 0.f) - c.y * ex2((one - c.x) * a.k));
+  const int v = (label - s.head) / kE;
+  if (label >= s.head && v < s.nvec && v % kThreads == t)      // the label's element again, by the thread that has just written its vector
+    g[label] = Num<T>::put(c.z - c.y * ex2((Num<T>::get(reinterpret_cast<const T*>(held + v)[(label - s.head) % kE]) - c.x) * a.k));
 }
 
 // Rows that a warp holds (up to 8 vectors a lane): a warp to a row, everything in registers.  kScores, kGrad, kLocal.
@@ -1034,7 +1133,7 @@ const char* launch_rows(const Args& from, cudaStream_t stream) {
   const int grid = static_cast<int>(items < most ? items : most);
   const char* err = set_ticket(a, kMode == kGrad, items <= kFirst * most, stream);
   if (err) return err;
-  a.behind = kMode != kLocal && a.pairs.pairs > 0;          // behind the kernels of the paired loss
+  a.behind = a.pairs.pairs > 0;                             // behind the kernels of the paired loss
   return launch_behind(a.behind, kernel, grid, kCompute + 32, smem, stream, a);
 }
 
@@ -1126,13 +1225,29 @@ const char* launch_pass(Args a, int dtype, cudaStream_t stream) {
                        stream, a);
 }
 
+template <typename T, int kThreads, int kBlocks>
+const char* launch_held(const Args& a, cudaStream_t stream) {
+  auto kernel = held_rows_kernel<T, kThreads, kBlocks>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldBytes);
+  if (e != cudaSuccess) return cudaGetErrorString(e);
+  kernel<<<a.rows, kThreads, a.each * 16, stream>>>(a);
+  return problem(cudaGetLastError());
+}
+
+// Threads to a row so that those of an SM, as many rows as its shared memory holds, are 1000 to 1200, what the registers allow.  600 MB of bf16 logits in
+// rows of 4000 words (64 threads / 128 / 192 / 384 / 512) 230 / 320 / 390 / 566 / 692 us, 12000 210 / 197 / 223 / 331 / 373, 20000 236 / 210 / 188 / 236 / 296, 32000
+// 276 / 228 / 207 / 200 / 242, 56000 338 / 270 / 225 / 213 / 201, 100000 611 / 382 / 329 / 272 / 261.
 template <typename T>
 const char* launch_local(Args a, cudaStream_t stream) {
   a.pieces = 1;
   a.each = a.vocab / Num<T>::kE;
   if (a.vocab <= warp_row<T>()) return launch_short<T, kLocal>(a, stream);
-  if (a.vocab <= kBlock * kVecs * Num<T>::kE) return launch_rows<T, kBlock, kLocal>(a, stream);
-  return launch_rows<T, kWide, kLocal>(a, stream);
+  const int kb = a.each / 64;
+  if (kb < 20) return launch_held<T, 64, 18>(a, stream);
+  if (kb < 28) return launch_held<T, 128, 9>(a, stream);
+  if (kb < 52) return launch_held<T, 192, 6>(a, stream);
+  if (kb < 80) return launch_held<T, 384, 3>(a, stream);
+  return launch_held<T, 512, 2>(a, stream);
 }
 
 Args row_args(const NmtgRows* r) {
@@ -1214,7 +1329,7 @@ const char* nmtg_policy_loss(const NmtgRows* r, const NmtgPolicy* p, cudaStream_
   a.w.lp = w.lp;
   a.w.state = w.state;
   if (r->rows <= 0) {
-  } else if (r->vocab <= kWide * kVecs * (16 / size)) {
+  } else if (static_cast<long>(r->vocab) * size <= kHeldBytes) {          // without a gradient, too: the same bits
     err = r->dtype == 0 ? launch_local<float>(a, stream) : r->dtype == 1 ? launch_local<__nv_bfloat16>(a, stream) : launch_local<__half>(a, stream);
   } else {
     a.w.part = w.part;
