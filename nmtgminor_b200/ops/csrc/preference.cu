@@ -799,19 +799,22 @@ __global__ void __launch_bounds__(kThreads, kBlocks) held_rows_kernel(const __gr
     g[label] = Num<T>::put(c.z - c.y * ex2((Num<T>::get(reinterpret_cast<const T*>(held + v)[(label - s.head) % kE]) - c.x) * a.k));
 }
 
-// Rows that a warp holds (up to 8 vectors a lane): a warp to a row, everything in registers.  kScores, kGrad, kLocal.
-template <typename T, int kMode>
+// Rows that a warp holds, kHeld vectors a lane: a warp to a row, everything in registers.  kScores, kGrad, kLocal.  (20000 rows of 2500 in bf16, 16 vectors a lane: scores
+// 27 us, gradients 44, paired loss 82; by the kernels for longer rows 74, 64 and 136.  Floors 16 and 31.)
+template <typename T, int kMode, int kHeld>
 __global__ void __launch_bounds__(256) short_rows_kernel(const __grid_constant__ Args a) {
   constexpr int kE = Num<T>::kE;
   const int lane = threadIdx.x & 31, row = static_cast<int>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (a.behind) wait_for_previous();
+  if (kMode == kLocal || (kMode == kScores && a.behind)) let_next_start();
   if (row >= a.rows) return;
   const T* const x = static_cast<const T*>(a.x) + static_cast<long>(row) * a.ld;
   T* const g = static_cast<T*>(a.g) + static_cast<long>(row) * a.ld;
   const Shape s = shape_of(a, x, 0);
   const int left = s.nvec - lane, e1 = single_at<T>(s, lane, 0, 1);
-  uint4 raw[kVecs];
+  uint4 raw[kHeld];
 #pragma unroll
-  for (int j = 0; j < kVecs; ++j)
+  for (int j = 0; j < kHeld; ++j)
     raw[j] = j * 32 < left ? reinterpret_cast<const uint4*>(x + s.head)[lane + j * 32] : make_uint4(Num<T>::kLow, Num<T>::kLow, Num<T>::kLow, Num<T>::kLow);
   const float one = e1 >= 0 ? Num<T>::get(x[e1]) : -INFINITY;
   const int64_t y = a.w.label ? a.w.label[row] : a.labels[row];
@@ -834,12 +837,12 @@ __global__ void __launch_bounds__(256) short_rows_kernel(const __grid_constant__
   } else {
     m = one;
 #pragma unroll
-    for (int j = 0; j < kVecs; ++j) m = fmaxf(m, Num<T>::largest(raw[j]));
+    for (int j = 0; j < kHeld; ++j) m = fmaxf(m, Num<T>::largest(raw[j]));
     m = warp_max(m);
     const float base = m == -INFINITY ? 0.f : m;
     float2 total = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int j = 0; j < kVecs; ++j) {
+    for (int j = 0; j < kHeld; ++j) {
       if (j > 0 && j * 32 >= s.nvec) break;
       float2 e[kE / 2];
       exps<T>(raw[j], -base, a.k, e);
@@ -863,7 +866,7 @@ __global__ void __launch_bounds__(256) short_rows_kernel(const __grid_constant__
   const float f = real ? -c / sum : 0.f;
   uint4* const out = reinterpret_cast<uint4*>(g + s.head) + lane;
 #pragma unroll
-  for (int j = 0; j < kVecs; ++j) {
+  for (int j = 0; j < kHeld; ++j) {
     if (j * 32 >= left) break;
     float2 e[kE / 2];
     exps<T>(raw[j], -m, a.k, e);
@@ -1151,7 +1154,7 @@ const char* launch_sums(Args a, cudaStream_t stream) {
   return launch_behind(a.behind, sums_kernel<T>, grid, kSumWarps * 32, smem, stream, a);
 }
 
-template <typename T> constexpr int warp_row() { return 32 * kVecs * Num<T>::kE; }       // elements that a warp holds
+template <typename T> constexpr int warp_row() { return 32 * 2 * kVecs * Num<T>::kE; }       // elements that a warp holds
 
 // SMs of the GPU, those in reserve too: how a row is divided decides the bits of a result and the size of the workspace
 int all_sms() {
@@ -1187,9 +1190,10 @@ int sums_pieces(int rows, int vocab, int dtype) {
 bool few_rows(int rows, int vocab, int dtype) { return rows <= all_sms() && vocab <= kWide * kVecs * (dtype == 0 ? 4 : 8); }
 
 template <typename T, int kMode>
-const char* launch_short(const Args& a, cudaStream_t stream) {
-  short_rows_kernel<T, kMode><<<(a.rows + 7) / 8, 256, 0, stream>>>(a);
-  return problem(cudaGetLastError());
+const char* launch_short(Args a, cudaStream_t stream) {
+  a.behind = kMode != kLocal && a.pairs.pairs > 0;
+  return launch_behind(a.behind, a.vocab <= warp_row<T>() / 2 ? short_rows_kernel<T, kMode, kVecs> : short_rows_kernel<T, kMode, 2 * kVecs>, (a.rows + 7) / 8, 256,
+                       0, stream, a);
 }
 
 // kMode: kScores or kGrad
@@ -1370,7 +1374,7 @@ const char* nmtg_preference_loss(const NmtgRows* r, const NmtgPairs* p, cudaStre
     scores = a;
     scores.pieces = is_short ? 1 : pieces;
     scores.stat = is_short ? w.stat : nullptr;
-    err = launch_behind(!is_short, r->dtype == 0 ? pairs_kernel<float> : r->dtype == 1 ? pairs_kernel<__nv_bfloat16> : pairs_kernel<__half>, p->pairs, 128, 0,
+    err = launch_behind(true, r->dtype == 0 ? pairs_kernel<float> : r->dtype == 1 ? pairs_kernel<__nv_bfloat16> : pairs_kernel<__half>, p->pairs, 128, 0,
                         stream, scores);
     if (err) return err;
   }
