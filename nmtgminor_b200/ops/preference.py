@@ -39,7 +39,7 @@ def _valid(labels, vocab, pad_idx):
 def token_logprobs_reference(logits, labels, pad_idx=0, temperature=1.0):
     lf = (logits if logits.dtype == torch.float64 else logits.float()) * (1.0 / temperature)
     valid = _valid(labels, logits.shape[1], pad_idx)
-    lp = lf.gather(1, labels.masked_fill(~valid, 0)[:, None]).squeeze(1) - torch.logsumexp(lf, -1)
+    lp = torch.log_softmax(lf, -1).gather(1, labels.masked_fill(~valid, 0)[:, None]).squeeze(1)
     return torch.where(valid, lp, torch.zeros_like(lp))
 
 

@@ -540,3 +540,46 @@ def test_a_word_of_probability_0_stays_in_its_sequence():
     assert got[:3].tolist() == [-3.0, -math.inf, -1.5] and torch.isnan(got[3]) and got[4] == 0.0 and got[5] == -math.inf
     leaf = lp[:2].clone().requires_grad_(True)
     assert torch.equal(torch.autograd.grad(pref.sequence_logprobs(leaf, torch.tensor([0, 1, 2])).sum(), leaf)[0], torch.ones(2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,vocab,layout", [("fp32", 5500, "dense"), ("bf16", 12001, "odd"), ("fp16", 13000, "padded"), ("bf16", 20001, "padded"),
+                                               ("bf16", 45000, "odd"), ("bf16", 114688, "dense"), ("bf16", 114689, "odd"), ("fp32", 57344, "dense"),
+                                               ("fp32", 57350, "odd"), ("fp16", 4096, "dense"), ("bf16", 4097, "odd"), ("fp32", 2048, "padded"), ("fp32", 2049, "odd")])
+def test_policy_loss_at_the_sizes_where_its_kernels_change(kind, vocab, layout):
+    """Rows of every number of threads, of all the shared memory that a block has and of a word more; masked logits, padding, an inplace gradient."""
+    rows = 40
+    x, y = _logits(rows, vocab, kind, layout)
+    x[7, 5:] = -math.inf
+    y[7] = 2
+    x[8] = torch.finfo(TYPES[kind]).min
+    g = torch.Generator().manual_seed(vocab)
+    lp = pref.token_logprobs(x.double(), y)
+    old, r = (lp + 0.2 * torch.randn(rows, generator=g).to(DEV).double()).float(), (lp + 0.3 * torch.randn(rows, generator=g).to(DEV).double()).float()
+    adv = torch.randn(rows, generator=g).to(DEV)
+    (loss, clipped, kl, want), grad = _coefs(x, y, lambda t: pref.policy_loss(t, y, old, adv, r, kl_coef=0.1))
+    leaf = x.detach().requires_grad_(True)
+    got = pref.policy_loss(leaf, y, old, adv, r, kl_coef=0.1)
+    mine = torch.autograd.grad(got[0], leaf)[0]
+    _logprobs_close(got[3], want)
+    assert got[1].item() == clipped.item() and abs(got[0].item() - loss.item()) <= rows * 1e-5 and abs(got[2].item() - kl.item()) <= rows * 1e-5
+    half = {"bf16": 2 ** -8, "fp16": 2 ** -11, "fp32": 2 ** -24}[kind]
+    # as in test_policy_loss: the coefficient off by 2^-15 of 4
+    assert ((mine.double() - grad).abs() <= (half + 2 ** -15) * grad.abs() + 2 ** -13).all()
+    assert (mine[1:4] == 0).all()
+    consumed = x.detach().clone(memory_format=torch.contiguous_format).requires_grad_(True)
+    plain = x.detach().clone(memory_format=torch.contiguous_format).requires_grad_(True)
+    over = pref.policy_loss(consumed, y, old, adv, r, kl_coef=0.1, inplace=True)
+    first = torch.autograd.grad(over[0], consumed)[0]
+    assert first.data_ptr() == consumed.data_ptr()
+    assert torch.equal(first, torch.autograd.grad(pref.policy_loss(plain, y, old, adv, r, kl_coef=0.1)[0], plain)[0])
+    assert ops.check_status() == 0
+
+
+def test_logprobs_of_very_large_logits():
+    """Rows of the type's lowest value have every word alike, rows with +inf or nothing but -inf NaN, on the CPU as on a GPU."""
+    for dtype in (torch.float64, torch.float32, torch.bfloat16):
+        x = torch.zeros(4, 50, dtype=dtype)
+        x[0], x[1], x[2], x[3, 7] = torch.finfo(torch.float32 if dtype == torch.float64 else dtype).min, 1e30, -math.inf, math.inf
+        got = pref.token_logprobs(x, torch.full((4,), 3))
+        assert ((got[:2] + math.log(50)).abs() <= 2 ** -19).all() and torch.isnan(got[2:]).all()
