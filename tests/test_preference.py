@@ -583,3 +583,41 @@ def test_logprobs_of_very_large_logits():
         x[0], x[1], x[2], x[3, 7] = torch.finfo(torch.float32 if dtype == torch.float64 else dtype).min, 1e30, -math.inf, math.inf
         got = pref.token_logprobs(x, torch.full((4,), 3))
         assert ((got[:2] + math.log(50)).abs() <= 2 ** -19).all() and torch.isnan(got[2:]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab,kind", [(900, 2500, "bf16"), (700, 1500, "fp32"), (700, 9001, "fp16"), (200, 131073, "bf16"), (2100, 32500, "bf16"), (300, 60000, "fp32")])
+def test_captured_losses_beside_other_work(rows, vocab, kind):
+    """All three operators captured in one graph and replayed while the same operators run on another stream: the bits of eager calls, each time.  Their
+    kernels are scheduled while the ones before them end, in graphs, too."""
+    x, y = _logits(rows, vocab, kind, "padded")
+    g = torch.Generator().manual_seed(rows)
+    cu = torch.linspace(0, rows - 3, 15).int().to(DEV)
+    adv, old = torch.randn(rows, generator=g).to(DEV), pref.token_logprobs(x, y) + 0.1
+    other = x.flip(0).contiguous()
+
+    def step(t):
+        leaf = t.detach().requires_grad_(True)
+        pairs = pref.preference_loss(leaf, y, cu, beta=0.05)
+        policy = pref.policy_loss(leaf, y, old, adv)
+        lp = pref.token_logprobs(leaf, y)
+        return [o.detach() for o in (*pairs, *policy, lp)] + [torch.autograd.grad(f, leaf)[0] for f in (pairs[0], policy[0])] + [torch.autograd.grad(lp, leaf, adv)[0]]
+
+    want, beside = step(x), step(other)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(x)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(4):
+        for o in out:
+            o.fill_(7.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(streams[0]):
+            graph.replay()
+        with torch.cuda.stream(streams[1]):
+            got = step(other)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        assert all(torch.equal(a, b) for a, b in zip(got, beside))
+    assert ops.check_status() == 0
