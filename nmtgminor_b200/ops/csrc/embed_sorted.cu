@@ -14,11 +14,10 @@
 #include <stdint.h>
 #include "b200_ptx.cuh"
 #include "bounds_check.cuh"
+#include "launch.cuh"
 #include "tuning_api.h"
 
 namespace b200 {
-
-int num_sms();
 
 namespace {
 
@@ -79,6 +78,7 @@ struct Clear {
 template <bool kWhole>
 __global__ void __launch_bounds__(256) tile_rank_kernel(const Keys k, int tile, uint32_t* __restrict__ tiles, int* __restrict__ order,
                                                         int* __restrict__ sorted, int* __restrict__ joins, const Clear clear) {
+  let_next_start();
   if (clear.mine()) { clear.run(); return; }
   __shared__ __align__(16) uint32_t all[kWhole ? kOneTile : kMergeTile];
   const int base = static_cast<int>(blockIdx.x) * kRankRows / tile * tile, count = min(tile, k.rows - base), padded = (count + 63) & ~63;
@@ -121,7 +121,9 @@ __global__ void __launch_bounds__(256) tile_rank_kernel(const Keys k, int tile, 
 // A row's place among all: in every sorted tile the rows before it, by bisection (4 threads to a row, every fourth tile each)
 __global__ void __launch_bounds__(256) merge_rank_kernel(const uint32_t* __restrict__ tiles, int rows, int* __restrict__ order, int* __restrict__ sorted,
                                                          const Clear clear) {
+  let_next_start();
   if (clear.mine()) { clear.run(); return; }
+  wait_for_previous();
   extern __shared__ __align__(16) uint32_t tile_of[];
   const int count = (rows + kMergeTile - 1) / kMergeTile;
 #pragma unroll 8
@@ -176,7 +178,9 @@ template <int kN> __device__ __forceinline__ void keys_at(const Keys& k, const P
 }
 
 __global__ void __launch_bounds__(256) radix_count_kernel(const Keys k, const Pass p, int* __restrict__ joins, const Clear clear) {
+  let_next_start();
   if (clear.mine()) { clear.run(); return; }
+  wait_for_previous();
   if (blockIdx.x == 0 && threadIdx.x < 2) joins[threadIdx.x] = 0;
   __shared__ int bins[1 << kDigitBits];
   for (int b = threadIdx.x; b < p.bins; b += 256) bins[b] = 0;
@@ -193,6 +197,8 @@ __global__ void __launch_bounds__(256) radix_count_kernel(const Keys k, const Pa
 
 // counts -> their exclusive sums, one block
 __global__ void __launch_bounds__(1024) radix_scan_kernel(int* __restrict__ counts, int n) {
+  let_next_start();
+  wait_for_previous();
   __shared__ int warps[32];
   __shared__ int carry;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -237,7 +243,9 @@ __global__ void __launch_bounds__(1024) radix_scan_kernel(int* __restrict__ coun
 
 // A warp has kTile / 8 rows one after another: it counts its digits, the warps' counts are summed in order, then rows go to their places.
 __global__ void __launch_bounds__(256) radix_scatter_kernel(const Keys k, const Pass p, const Clear clear) {
+  let_next_start();
   if (clear.mine()) { clear.run(); return; }
+  wait_for_previous();
   extern __shared__ int at[];                                   // [8][bins]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int b = threadIdx.x; b < 8 * p.bins; b += 256) at[b] = 0;
@@ -343,6 +351,8 @@ __global__ void __launch_bounds__(256, 3) reduce_kernel(const Sum s) {
   constexpr bool kCopy = kBytes >= 8;
   extern __shared__ __align__(16) unsigned char held[];         // [chunk][256] vectors
   const int c = blockIdx.x * blockDim.y + threadIdx.y, lane = threadIdx.x & 31, thread = threadIdx.y * blockDim.x + threadIdx.x;
+  let_next_start();
+  wait_for_previous();
   if (c >= s.chunks) return;
   const int begin = c * s.chunk, count = min(s.rows - begin, s.chunk);
   const DropRng rng(s.seed + ((kDrop && s.seed_dev) ? *s.seed_dev : 0ull), s.stream_id, s.p);
@@ -430,6 +440,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Sum s) {
   __shared__ float runs[kRuns][kCols * kN];
   const int x = threadIdx.x & 31, run = threadIdx.x >> 5, half = gridDim.x / 2;
   const bool first_half = static_cast<int>(blockIdx.x) < half;
+  wait_for_previous();
   const int sums = first_half ? s.joins[0] : 0, long_sums = first_half ? 0 : s.joins[1];
   for (int i = (blockIdx.y * half + blockIdx.x) * kRuns + run; i < sums; i += half * gridDim.y * kRuns) {
     const int c = s.joins[2 + i], key = s.sorted[(c + 1) * s.chunk];
@@ -546,12 +557,10 @@ const char* sums(const Sum& s, cudaStream_t stream) {
   const int vector = sizeof(T) * kN, smem = vector >= 8 ? s.chunk * 256 * vector : 0;
   cudaError_t e = cudaFuncSetAttribute(reduce_kernel<T, kN, kDrop, kAdd>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostChunk * 256 * 16);
   if (e != cudaSuccess) return problem(e);
-  reduce_kernel<T, kN, kDrop, kAdd><<<dim3((s.chunks + block.y - 1) / block.y), block, smem, stream>>>(s);
-  e = cudaGetLastError();
-  if (e != cudaSuccess || s.chunks < 2) return problem(e);
+  const char* err = launch_behind(true, reduce_kernel<T, kN, kDrop, kAdd>, dim3((s.chunks + block.y - 1) / block.y), block, smem, stream, s);
+  if (err || s.chunks < 2) return err;
   const int cols = (s.width + 32 * kN - 1) / (32 * kN), across = cols < 8 ? cols : 8, want = (s.chunks + 7) / 8, most = 16 * num_sms() / across;
-  join_kernel<T, kN, kAdd><<<dim3(2 * (want < most ? want : most), across), 256, 0, stream>>>(s);
-  return problem(cudaGetLastError());
+  return launch_behind(true, join_kernel<T, kN, kAdd>, dim3(2 * (want < most ? want : most), across), dim3(256), 0, stream, s);
 }
 
 template <typename T, int kN, bool kAdd>
@@ -636,8 +645,7 @@ const char* nmtg_embed_grad(const NmtgEmbedGrad* d) {
     tile_rank_kernel<false><<<grid, 256, 0, stream>>>(k, kMergeTile, tiles, nullptr, nullptr, joins, clear);
     if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
     grid = clear.next((n + kMergeRows - 1) / kMergeRows, 1);
-    merge_rank_kernel<<<grid, 256, smem, stream>>>(tiles, n, row[0], key[0], clear);
-    if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
+    if (const char* err = launch_behind(true, merge_rank_kernel, grid, 256, smem, stream, tiles, n, row[0], key[0], clear)) return err;
   } else {
     const int passes = (bits + kDigitBits - 1) / kDigitBits, digit = (bits + passes - 1) / passes;
     const size_t smem = 8 * sizeof(int) << digit;
@@ -645,13 +653,11 @@ const char* nmtg_embed_grad(const NmtgEmbedGrad* d) {
     for (int i = 0; i < passes; ++i) {
       Pass p = {i ? key[(i - 1) & 1] : nullptr, i ? row[(i - 1) & 1] : nullptr, key[i & 1], row[i & 1], counts, i * digit, digit, 1 << digit, tiles};
       int grid = clear.next(tiles, 1);
-      radix_count_kernel<<<grid, 256, 0, stream>>>(k, p, joins, clear);
-      if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
-      radix_scan_kernel<<<1, 1024, 0, stream>>>(counts, tiles << digit);
-      if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
+      const char* err = launch_behind(i > 0, radix_count_kernel, grid, 256, 0, stream, k, p, joins, clear);
+      if (err) return err;
+      if ((err = launch_behind(true, radix_scan_kernel, 1, 1024, 0, stream, counts, tiles << digit))) return err;
       grid = clear.next(tiles, 1);
-      radix_scatter_kernel<<<grid, 256, smem, stream>>>(k, p, clear);
-      if ((e = cudaGetLastError()) != cudaSuccess) return cudaGetErrorString(e);
+      if ((err = launch_behind(true, radix_scatter_kernel, grid, 256, smem, stream, k, p, clear))) return err;
       last = i & 1;
     }
   }

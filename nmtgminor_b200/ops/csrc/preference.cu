@@ -22,12 +22,11 @@
 #include <climits>
 #include <stdint.h>
 #include "b200_ptx.cuh"
+#include "launch.cuh"
 #include "tuning_api.h"
 
 namespace b200 {
 
-int num_sms();
-bool launch_overlap();
 
 namespace {
 
@@ -1086,24 +1085,6 @@ __global__ void __launch_bounds__(256) scale_rows_kernel(const Args a, const flo
 }
 
 const char* problem(cudaError_t e) { return e == cudaSuccess ? nullptr : cudaGetErrorString(e); }
-
-// `kernel` calls wait_for_previous() before it touches memory.  It may be scheduled before the kernel of this call in front of it has ended, where that one lets
-// it: its start, 2 to 3 us, then costs nothing (paired loss of 8200 rows of 32000 in bf16 260 -> 255 us, of 300 rows of 8000 29 -> 23; policy
-// loss of 20000 rows of 8000 145 -> 135).  Not behind a cleared ticket, which is no kernel.
-template <typename... P, typename... A>
-const char* launch_behind(bool may, void (*kernel)(P...), int grid, int threads, int smem, cudaStream_t stream, const A&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = may && launch_overlap() ? 1 : 0;
-  return problem(cudaLaunchKernelEx(&cfg, kernel, args...));
-}
 
 // The ticket of a pass, unless every block has its items without asking; the paired loss has zeroed it before
 const char* set_ticket(Args& a, int pass, bool none, cudaStream_t stream) {
