@@ -118,9 +118,9 @@ __global__ void __launch_bounds__(256) tile_rank_kernel(const Keys k, int tile, 
   }
 }
 
-// A row's place among all: in every sorted tile the rows before it, by bisection (4 threads to a row, every fourth tile each)
-__global__ void __launch_bounds__(256) merge_rank_kernel(const uint32_t* __restrict__ tiles, int rows, int* __restrict__ order, int* __restrict__ sorted,
-                                                         const Clear clear) {
+// A row's place among all: in every sorted tile the rows before it, by bisection (4 threads to a row, every fourth tile each).  `tiles` is written while this
+// kernel is already there, so it is not __restrict__: loads of what never changes may be moved in front of the wait.
+__global__ void __launch_bounds__(256) merge_rank_kernel(const uint32_t* tiles, int rows, int* order, int* sorted, const Clear clear) {
   let_next_start();
   if (clear.mine()) { clear.run(); return; }
   wait_for_previous();
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(256) radix_count_kernel(const Keys k, const Pa
 }
 
 // counts -> their exclusive sums, one block
-__global__ void __launch_bounds__(1024) radix_scan_kernel(int* __restrict__ counts, int n) {
+__global__ void __launch_bounds__(1024) radix_scan_kernel(int* counts, int n) {
   let_next_start();
   wait_for_previous();
   __shared__ int warps[32];

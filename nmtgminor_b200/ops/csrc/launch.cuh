@@ -35,7 +35,7 @@ const char* launch_overlapped(void (*kernel)(P...), dim3 grid, int threads, size
 
 // Launches between the kernels of one call.  `kernel` calls wait_for_previous() before it touches memory that the call's earlier kernels use, and may be
 // scheduled before the one in front of it has ended, where that one lets it (let_next_start()): its start, 2 to 3 us, then costs nothing.  Blocks of any
-// number and size: what they wait for is theirs, and ends.  (Paired loss of 8200 rows of 32000 in bf16 260 -> 255 us, of 300 rows of 8000 29 -> 23; policy loss of
+// number and size: what they wait for is theirs, and ends.  What an earlier kernel writes is not read through const __restrict__ pointers.  (Paired loss of 8200 rows of 32000 in bf16 260 -> 255 us, of 300 rows of 8000 29 -> 23; policy loss of
 // 20000 rows of 8000 145 -> 135.)  `may` false: the kernel is the call's first, or behind a copy or a cleared word, which are no kernels.
 template <typename... P, typename... A>
 const char* launch_behind(bool may, void (*kernel)(P...), dim3 grid, dim3 threads, size_t smem, cudaStream_t stream, const A&... args) {
