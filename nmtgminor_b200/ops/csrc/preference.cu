@@ -3,7 +3,7 @@
 //     lp = (x[y] - M) / T - log s          d lp / d x = (onehot(y) - exp((x - M) / T) / s) / T
 // Each loss is a function of the lp of its rows, so a row's gradient is one coefficient times d lp / d x.
 //
-// The policy loss of rows that an SM's shared memory holds is one pass, a block to a row (held_rows_kernel), or a warp to a short one.  Scores of rows in one
+// The policy loss is one pass, a warp, a block or a cluster of blocks to a row, which they hold (rows of up to 896 KB).  Scores of rows in one
 // piece are one pass, too.  The paired loss, and the scores and the policy loss of longer rows, are two passes over pieces of rows, sums (sums_kernel, rows_kernel) and
 // then gradients (rows_kernel), with a small kernel between that makes rows of the pieces and coefficients of the rows.  (Both at once, the
 // gradients some rows behind the sums so that they would find the logits in L2, were built and measured: 353 us against 272 for 8200 rows of 32000 in bf16.
@@ -35,7 +35,7 @@ constexpr int kSlots = 3;             // items in shared memory or on their way 
 constexpr int kRing = 8;              // entries of work known: one behind, kSlots + 3 ahead, and that in hand
 constexpr int kFirst = 6;             // items of a block that it need not ask for
 constexpr int kBlock = 256, kWide = 512;      // threads of a block for the elements; two or three blocks to an SM, and one
-constexpr int kHeldBytes = 224 * 1024;        // of a row that a block's shared memory holds
+constexpr int kHeldBytes = 112 * 1024;        // of a row that a block holds, two blocks to an SM
 
 // kScores: sums of pieces.  kGrad: gradients from `stat` and a coefficient.  kLocal: the policy loss of rows that a warp holds.
 enum Mode { kScores = 0, kGrad = 1, kLocal = 2 };
@@ -690,39 +690,42 @@ __global__ void __launch_bounds__(kSumWarps * 32, kSumBlocks) sums_kernel(const 
   copies_wait<0>();
 }
 
-// The policy loss of a row that a block's shared memory holds, a block to a row: every thread copies its vectors, adds them up as they arrive in four
+// The policy loss of a row that a block's shared memory holds, a block to a row, or a cluster of 2, 4 or 8 to a longer one (kCluster: the blocks read each
+// other's sums from shared memory): every thread copies its vectors, adds them up as they arrive in four
 // groups, and goes over them again for the gradient.  Nothing is carried from row to row: while a block waits for its row, or for the coefficient, others of the SM
 // compute and store, and rows go to SMs as they become free.  (A block that stays and reads the next rows meanwhile, three slots and a warp for the
 // coefficients, was built before: 15360 rows of 32000 in bf16 360 us for 317, 3584 of 51865, which it could not hold, 195 for 138.)
 constexpr int kHeldGroups = 4, kHeldVecs = 4;             // vectors that a thread has in registers
-template <typename T, int kThreads, int kBlocks>
+template <typename T, int kThreads, int kBlocks, bool kCluster>
 __global__ void __launch_bounds__(kThreads, kBlocks) held_rows_kernel(const __grid_constant__ Args a) {
   constexpr int kE = Num<T>::kE, kWarps = kThreads / 32;
   extern __shared__ __align__(16) uint4 held[];
-  __shared__ float2 part[kWarps];
+  __shared__ float2 part[kWarps], whole;
   __shared__ float4 bc;
   let_next_start();
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, row = static_cast<int>(blockIdx.x);
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int pieces = kCluster ? a.pieces : 1, row = static_cast<int>(blockIdx.x) / pieces, piece = static_cast<int>(blockIdx.x) - row * pieces;
   const T* const x = static_cast<const T*>(a.x) + static_cast<long>(row) * a.ld;
   T* const g = a.g ? static_cast<T*>(a.g) + static_cast<long>(row) * a.ld : nullptr;
-  const Shape s = shape_of(a, x, 0);
-  const uint4* const from = reinterpret_cast<const uint4*>(x + s.head);
+  const Shape s = shape_of(a, x, piece);
+  const int nvec = s.v1 - s.v0;                               // of this block
+  const uint4* const from = reinterpret_cast<const uint4*>(x + s.head) + s.v0;
   const int64_t y = a.labels[row];
-  const int each = (s.nvec + kHeldGroups * kThreads - 1) / (kHeldGroups * kThreads) * kThreads;      // vectors of a group
+  const int each = (nvec + kHeldGroups * kThreads - 1) / (kHeldGroups * kThreads) * kThreads;      // vectors of a group
 #pragma unroll
   for (int q = 0; q < kHeldGroups; ++q) {
-    const int end = min(s.nvec, (q + 1) * each);
+    const int end = min(nvec, (q + 1) * each);
 #pragma unroll 4
     for (int v = q * each + t; v < end; v += kThreads) copy16(held + v, from + v);
     copies_end();
   }
   const bool real = y != a.pad && y >= 0 && y < a.vocab;
-  const int label = real ? static_cast<int>(y) : -1, e1 = single_at<T>(s, t, 0, 1);
-  uint4* const out = reinterpret_cast<uint4*>(g + s.head);
-  if (!real) {
-    if (t == 0) { a.logprobs[row] = 0.f; a.w.lp[row] = 0.0; }
+  const int label = real ? static_cast<int>(y) : -1, e1 = single_at<T>(s, t, piece, pieces);
+  uint4* const out = reinterpret_cast<uint4*>(g + s.head) + s.v0;
+  if (!real) {                                                // for all blocks of the row
+    if (t == 0 && piece == 0) { a.logprobs[row] = 0.f; a.w.lp[row] = 0.0; }
     if (g) {
-      for (int v = t; v < s.nvec; v += kThreads) __stcs(out + v, make_uint4(0, 0, 0, 0));
+      for (int v = t; v < nvec; v += kThreads) __stcs(out + v, make_uint4(0, 0, 0, 0));
       if (e1 >= 0) g[e1] = Num<T>::put(0.f);
     }
     copies_wait<0>();
@@ -741,7 +744,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) held_rows_kernel(const __gr
 #pragma unroll
   for (int q = 0; q < kHeldGroups; ++q) {
     if (q == 0) copies_wait<3>(); else if (q == 1) copies_wait<2>(); else if (q == 2) copies_wait<1>(); else copies_wait<0>();
-    const int end = min(s.nvec, (q + 1) * each);
+    const int end = min(nvec, (q + 1) * each);
 #pragma unroll 1
     for (int v = q * each + t; v < end; v += kHeldVecs * kThreads) {
       uint4 raw[kHeldVecs];
@@ -773,19 +776,32 @@ __global__ void __launch_bounds__(kThreads, kBlocks) held_rows_kernel(const __gr
     m = lane < kWarps ? part[lane].x : -INFINITY;
     sum = lane < kWarps ? part[lane].y : 0.f;
     join_lanes(m, sum, a.k);
+    if (kCluster && lane == 0) whole = make_float2(m, sum);
+  }
+  if constexpr (kCluster) cooperative_groups::this_cluster().sync();
+  if (warp == 0) {
+    if constexpr (kCluster) {                                 // every block of the row comes to the same coefficient
+      const float2 of = lane < pieces ? *cooperative_groups::this_cluster().map_shared_rank(&whole, lane) : make_float2(-INFINITY, 0.f);
+      m = of.x;
+      sum = of.y;
+      join_lanes(m, sum, a.k);
+    }
     const LogProb lp = log_probability(xy, m, sum, a.inv_t);
     const float c = policy_coef(a, lp, old, adv, ref) * a.inv_t * scale;
     if (lane == 0) {
       bc = make_float4(m, __fdividef(c, sum), c, 0.f);
-      a.logprobs[row] = lp.hi;
-      a.w.lp[row] = lp.wide();
+      if (piece == 0) {
+        a.logprobs[row] = lp.hi;
+        a.w.lp[row] = lp.wide();
+      }
     }
   }
-  __syncthreads();
+  if constexpr (kCluster) cooperative_groups::this_cluster().sync();         // `whole` of every block is read
+  else __syncthreads();
   if (!g) return;
   const float4 c = bc;
 #pragma unroll 4
-  for (int v = t; v < s.nvec; v += kThreads) {
+  for (int v = t; v < nvec; v += kThreads) {
     float2 e[kE / 2];
     exps<T>(held[v], -c.x, a.k, e);
 #pragma unroll
@@ -793,8 +809,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks) held_rows_kernel(const __gr
     __stcs(out + v, Num<T>::pack(e));
   }
   if (e1 >= 0) g[e1] = Num<T>::put((e1 == label ? c.z : 0.f) - c.y * ex2((one - c.x) * a.k));
-  const int v = (label - s.head) / kE;
-  if (label >= s.head && v < s.nvec && v % kThreads == t)      // the label's element again, by the thread that has just written its vector
+  const int v = (label - s.head) / kE - s.v0;
+  if (label >= s.head && v >= 0 && v < nvec && v % kThreads == t)      // the label's element again, by the thread that has just written its vector
     g[label] = Num<T>::put(c.z - c.y * ex2((Num<T>::get(reinterpret_cast<const T*>(held + v)[(label - s.head) % kE]) - c.x) * a.k));
 }
 
@@ -1210,29 +1226,45 @@ const char* launch_pass(Args a, int dtype, cudaStream_t stream) {
                        stream, a);
 }
 
-template <typename T, int kThreads, int kBlocks>
+template <typename T, int kThreads, int kBlocks, bool kCluster>
 const char* launch_held(const Args& a, cudaStream_t stream) {
-  auto kernel = held_rows_kernel<T, kThreads, kBlocks>;
+  if (static_cast<long>(a.rows) * a.pieces > INT_MAX) return "preference: too many rows";
+  auto kernel = held_rows_kernel<T, kThreads, kBlocks, kCluster>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldBytes);
   if (e != cudaSuccess) return cudaGetErrorString(e);
-  kernel<<<a.rows, kThreads, a.each * 16, stream>>>(a);
-  return problem(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.rows * a.pieces);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = a.each * 16;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = a.pieces;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = kCluster ? 1 : 0;
+  return problem(cudaLaunchKernelEx(&cfg, kernel, a));
 }
 
 // Threads to a row so that those of an SM, as many rows as its shared memory holds, are 1000 to 1200, what the registers allow.  600 MB of bf16 logits in
 // rows of 4000 words (64 threads / 128 / 192 / 384 / 512) 230 / 320 / 390 / 566 / 692 us, 12000 210 / 197 / 223 / 331 / 373, 20000 236 / 210 / 188 / 236 / 296, 32000
-// 276 / 228 / 207 / 200 / 242, 56000 338 / 270 / 225 / 213 / 201, 100000 611 / 382 / 329 / 272 / 261.
+// 276 / 228 / 207 / 200 / 242, 56000 338 / 270 / 225 / 213 / 201.  Rows of more
+// than 112 KB one to a block, which an SM then holds alone, and to clusters: 64000 words 268 / 230, 128000 292 / 243, 250054 by two passes 300, by a cluster 279.
 template <typename T>
 const char* launch_local(Args a, cudaStream_t stream) {
   a.pieces = 1;
   a.each = a.vocab / Num<T>::kE;
   if (a.vocab <= warp_row<T>()) return launch_short<T, kLocal>(a, stream);
+  const int vectors = a.vocab / Num<T>::kE;
+  while (vectors * 16 > kHeldBytes * a.pieces) a.pieces *= 2;          // 2, 4 or 8
+  a.each = (vectors + a.pieces - 1) / a.pieces;
   const int kb = a.each / 64;
-  if (kb < 20) return launch_held<T, 64, 18>(a, stream);
-  if (kb < 28) return launch_held<T, 128, 9>(a, stream);
-  if (kb < 52) return launch_held<T, 192, 6>(a, stream);
-  if (kb < 80) return launch_held<T, 384, 3>(a, stream);
-  return launch_held<T, 512, 2>(a, stream);
+  if (a.pieces > 1) return kb < 80 ? launch_held<T, 384, 3, true>(a, stream) : launch_held<T, 512, 2, true>(a, stream);
+  if (kb < 20) return launch_held<T, 64, 18, false>(a, stream);
+  if (kb < 28) return launch_held<T, 128, 9, false>(a, stream);
+  if (kb < 52) return launch_held<T, 192, 6, false>(a, stream);
+  if (kb < 80) return launch_held<T, 384, 3, false>(a, stream);
+  return launch_held<T, 512, 2, false>(a, stream);
 }
 
 Args row_args(const NmtgRows* r) {
@@ -1314,7 +1346,7 @@ const char* nmtg_policy_loss(const NmtgRows* r, const NmtgPolicy* p, cudaStream_
   a.w.lp = w.lp;
   a.w.state = w.state;
   if (r->rows <= 0) {
-  } else if (static_cast<long>(r->vocab) * size <= kHeldBytes) {          // without a gradient, too: the same bits
+  } else if (static_cast<long>(r->vocab) * size <= 8L * kHeldBytes) {       // without a gradient, too: the same bits
     err = r->dtype == 0 ? launch_local<float>(a, stream) : r->dtype == 1 ? launch_local<__nv_bfloat16>(a, stream) : launch_local<__half>(a, stream);
   } else {
     a.w.part = w.part;

@@ -545,9 +545,12 @@ def test_a_word_of_probability_0_stays_in_its_sequence():
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind,vocab,layout", [("fp32", 5500, "dense"), ("bf16", 12001, "odd"), ("fp16", 13000, "padded"), ("bf16", 20001, "padded"),
                                                ("bf16", 45000, "odd"), ("bf16", 114688, "dense"), ("bf16", 114689, "odd"), ("fp32", 57344, "dense"),
-                                               ("fp32", 57350, "odd"), ("fp16", 4096, "dense"), ("bf16", 4097, "odd"), ("fp32", 2048, "padded"), ("fp32", 2049, "odd")])
+                                               ("fp32", 57350, "odd"), ("fp16", 4096, "dense"), ("bf16", 4097, "odd"), ("fp32", 2048, "padded"), ("fp32", 2049, "odd"),
+                                               ("fp16", 57344, "dense"), ("bf16", 57345, "odd"), ("bf16", 200003, "odd"), ("bf16", 229376, "padded"), ("fp16", 229380, "odd"),
+                                               ("fp32", 120001, "odd"), ("bf16", 458752, "dense"), ("fp16", 458753, "padded")])
 def test_policy_loss_at_the_sizes_where_its_kernels_change(kind, vocab, layout):
-    """Rows of every number of threads, of all the shared memory that a block has and of a word more; masked logits, padding, an inplace gradient."""
+    """Rows of every number of threads and blocks, of all the shared memory that these have and of a word more; masked logits, padding, an inplace
+    gradient."""
     rows = 40
     x, y = _logits(rows, vocab, kind, layout)
     x[7, 5:] = -math.inf
