@@ -64,7 +64,7 @@ struct Args {
   int pieces, each;         // of a row; vectors of a piece
   int slot;                 // vectors of a slot
   int behind;               // launched while the kernel before it ends
-  int stays;                // first row that is to stay in L2 after the sums
+  int stays;                // rows that are to stay in L2 after the sums
   int aligned;              // every row starts on a 16-byte boundary
   float k, inv_t;           // log2(e) / T, 1 / T
   float* logprobs;
@@ -168,9 +168,11 @@ __device__ __forceinline__ float warp_max(float v) {
 __device__ __forceinline__ void copy16(uint4* to, const uint4* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
 }
-// For the sums, whose rows are read again by the gradients: these go from the last row to the first, and find in L2 what the sums read last, the rows
-// from `stays` on; the rows before pass through it first out.  (Paired loss of 8200 rows of 32000 in bf16: 276 us in one order, 273 with the gradients
-// from the last row, 261 so; 8200 rows of 8000 in fp32 151, 144, 136.  48 to 80 MB alike, 112 of the 126 that L2 has 2 % slower.)
+// Rows are gone through from the last to the first where they are read first: whatever has made the logits has left the last ones in L2.  The gradients behind
+// the sums go from the first to the last, and find in L2 what the sums read last, the first `stays` rows; the others pass through it first out.
+// (Paired loss of 8200 rows of 32000 in bf16: 276 us with both in one order, 273 in opposite ones, 261 so; 8200 rows of 8000 in fp32 151, 144, 136.
+// 48 to 80 MB alike, 112 of the 126 that L2 has 2 % slower.  Behind a copy of the logits: scores of
+// the 8200 rows 102 us from the first row on, 94 from the last, paired loss 264 and 253.)
 constexpr long kStaying = 48L << 20;
 __device__ __forceinline__ uint64_t policy_of(bool stay) {
   uint64_t first, normal;
@@ -350,7 +352,7 @@ __global__ void __launch_bounds__(kCompute + 32, kCompute == kBlock ? 3 : 1) row
       return a.w.ticket ? kFirst * static_cast<int>(gridDim.x) + atomicAdd(a.w.ticket, 1) : a.rows * a.pieces;
     };
     const auto ask = [&](int i, int number) {                 // lane 0
-      const int items = a.rows * a.pieces, n = kMode == kGrad ? items - 1 - number : number, q = a.pieces == 1 ? n : n / a.pieces;
+      const int items = a.rows * a.pieces, n = kMode == kScores ? items - 1 - number : number, q = a.pieces == 1 ? n : n / a.pieces;
       const Entry e = {number < items ? q : -1, n - q * a.pieces, -1, 0};
       Mail& m = mail[i & (kRing - 1)];
       if (e.row < 0) m.label = -1;
@@ -453,7 +455,7 @@ __global__ void __launch_bounds__(kCompute + 32, kCompute == kBlock ? 3 : 1) row
       uint4* to = slots + (i % kSlots) * a.slot + t;
       const int left = s.v1 - s.v0 - t;
       if constexpr (kMode == kScores) {
-        const uint64_t policy = policy_of(n.row >= a.stays);
+        const uint64_t policy = policy_of(n.row < a.stays);
 #pragma unroll
         for (int j = 0; j < kVecs; ++j)
           if (j * kCompute < left) copy16(to + j * kCompute, from + j * kCompute, policy);
@@ -582,9 +584,9 @@ __global__ void __launch_bounds__(kSumWarps * 32, kSumBlocks) sums_kernel(const 
   // The copying side: lane 0 has the next item's number and label and the number after it, asked for an item ahead.  Rows of padding are passed over.
   int number = static_cast<int>(blockIdx.x) + warp * static_cast<int>(gridDim.x), after = number + warps;
   int label = -1;
-  const auto label_of = [&](int n) -> int {
-    if (n >= items) return -1;
-    const int row = a.pieces == 1 ? n : n / a.pieces;
+  const auto label_of = [&](int of) -> int {
+    if (of >= items) return -1;
+    const int n = items - 1 - of, row = a.pieces == 1 ? n : n / a.pieces;
     const int64_t y = a.labels[row];
     return y == a.pad || y < 0 || y >= a.vocab ? -1 : static_cast<int>(y);
   };
@@ -593,8 +595,8 @@ __global__ void __launch_bounds__(kSumWarps * 32, kSumBlocks) sums_kernel(const 
   const uint4* from = nullptr;
   const auto fetch = [&]() {
     for (;;) {
-      const int n = __shfl_sync(0xffffffffu, number, 0), y = __shfl_sync(0xffffffffu, label, 0);
-      if (n >= items) { prow = -1; break; }
+      const int n = items - 1 - __shfl_sync(0xffffffffu, number, 0), y = __shfl_sync(0xffffffffu, label, 0);
+      if (n < 0) { prow = -1; break; }
       if (lane == 0) {
         number = after;
         label = label_of(number);
@@ -624,7 +626,7 @@ __global__ void __launch_bounds__(kSumWarps * 32, kSumBlocks) sums_kernel(const 
   int slot = 0;
   const auto issue = [&](int to) {
     if (prow >= 0) {
-      const uint64_t policy = policy_of(prow >= a.stays);
+      const uint64_t policy = policy_of(prow < a.stays);
 #pragma unroll
       for (int j = 0; j < kSumVecs; ++j)
         if (at + lane + j * 32 < end) copy16(mine + to * kSumStage + j * 32, from + at + j * 32, policy);
@@ -704,7 +706,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) held_rows_kernel(const __gr
   __shared__ float4 bc;
   let_next_start();
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const int pieces = kCluster ? a.pieces : 1, row = static_cast<int>(blockIdx.x) / pieces, piece = static_cast<int>(blockIdx.x) - row * pieces;
+  const int pieces = kCluster ? a.pieces : 1, block = static_cast<int>(gridDim.x - 1 - blockIdx.x), row = block / pieces, piece = block - row * pieces;
   const T* const x = static_cast<const T*>(a.x) + static_cast<long>(row) * a.ld;
   T* const g = a.g ? static_cast<T*>(a.g) + static_cast<long>(row) * a.ld : nullptr;
   const Shape s = shape_of(a, x, piece);
@@ -1278,7 +1280,7 @@ Args row_args(const NmtgRows* r) {
   a.pieces = 1;
   a.each = a.vocab;
   const long staying = kStaying / (r->vocab * (r->dtype == 0 ? 4L : 2L));
-  a.stays = r->rows > staying ? static_cast<int>(r->rows - staying) : 0;
+  a.stays = r->rows > staying ? static_cast<int>(staying) : r->rows;
   return a;
 }
 
