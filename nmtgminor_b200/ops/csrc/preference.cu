@@ -321,8 +321,8 @@ __device__ __forceinline__ float policy_coef(const Args& a, LogProb lp, float ol
 }
 
 // kCompute threads do the elements' work; one more warp fetches the entries, joins the partial sums and brings the coefficients.  Step i of the
-// block: the sums of entry i, the barrier, the gradient of entry i - 1 (its logits still in their slot).  Between barriers i - 1 and i the last warp
-// joins the sums of entry i - 1 and brings its coefficient, and publishes entry i + kLead + 1.
+// block: the sums of entry i and the barrier (kScores), or the barrier and the gradient of entry i - 1, its logits in their slot (kGrad).  Between barriers
+// i - 1 and i the last warp joins the sums of entry i - 1, or brings its coefficient, and publishes entry i + kLead + 1.
 template <typename T, int kCompute, int kMode>
 __global__ void __launch_bounds__(kCompute + 32, kCompute == kBlock ? 3 : 1) rows_kernel(const __grid_constant__ Args a) {
   constexpr int kE = Num<T>::kE, kWarps = kCompute / 32;
