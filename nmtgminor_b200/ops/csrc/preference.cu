@@ -287,7 +287,8 @@ __device__ __noinline__ void pair_loss(const Args& a, int p, double sw, double s
     } else {
       const double less = exp(-fabs(z)), soft = log1p(less), eps = q.smoothing;
       const double up = z >= 0.0 ? 1.0 / (1.0 + less) : less / (1.0 + less);      // sigmoid(z)
-      loss = (1.0 - eps) * (soft + fmax(-z, 0.0)) + eps * (soft + fmax(z, 0.0));
+      loss = (1.0 - eps) * (soft + fmax(-z, 0.0));
+      if (eps != 0.0) loss += eps * (soft + fmax(z, 0.0));                        // without smoothing a pair at z = inf costs 0, not 0 * inf
       if (z != z) loss = z;
       const double down = z >= 0.0 ? less / (1.0 + less) : 1.0 / (1.0 + less);    // sigmoid(-z)
       slope = q.beta * (eps * up - (1.0 - eps) * down);

@@ -58,7 +58,9 @@ def preference_loss_reference(logits, labels, cu, ref_logprobs=None, beta=0.1, k
         loss = (h - 0.5 / beta) ** 2
     else:
         z = beta * h - margin
-        loss = torch.relu(1.0 - z) if kind == "hinge" else -(1.0 - smoothing) * F.logsigmoid(z) - smoothing * F.logsigmoid(-z)
+        loss = torch.relu(1.0 - z) if kind == "hinge" else -(1.0 - smoothing) * F.logsigmoid(z)
+        if smoothing:                                           # 0 * inf at z = inf otherwise
+            loss = loss - smoothing * F.logsigmoid(-z)
     if nll_weight:
         loss = loss - nll_weight * (scores * each)[0::2]
     return loss.sum().reshape(1), (h > 0).sum().to(lp.dtype).reshape(1), scores.detach()

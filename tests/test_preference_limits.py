@@ -1,0 +1,77 @@
+"""Losses of preference tuning where their terms leave the numbers: words of probability 0 and ratios beyond 32 bits.  Expected values are written
+out in 64 bits, apart from the restatements, which are tested like the kernels."""
+import math
+
+import pytest
+import torch
+
+from nmtgminor_b200 import ops
+from nmtgminor_b200.ops import preference as pref
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+HALF = {torch.bfloat16: 2 ** -8, torch.float16: 2 ** -11, torch.float32: 2 ** -24, torch.float64: 0.0}
+# rows that a warp holds, a block, a cluster of blocks, and none of them
+SIZES = [("cpu", 40, torch.float32), ("cpu", 40, torch.float64), *(pytest.param("cuda", v, d, marks=pytest.mark.gpu) for v, d in (
+    (40, torch.float32), (40, torch.float16), (9001, torch.bfloat16), (60001, torch.float32), (270005, torch.float32)))]
+
+
+def _rows(device, rows, vocab, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed + vocab)
+    x = (torch.randn(rows, vocab, generator=g) * 2).to(dtype).to(device)
+    return x, torch.randint(1, vocab, (rows,), generator=g).to(device)
+
+
+def _close(got, coef, x, y, slack=0.0):
+    """Gradient rows coef * (onehot - softmax).  Against 64 bits: half a step of the type, 2^-15 of an exponential (its argument's roundings, the sum, the
+    coefficient), at the label of coef p; half of fp16's smallest number.  ``slack``: error of the coefficients themselves."""
+    p = torch.softmax(x.double(), 1)
+    hot = torch.nn.functional.one_hot(y, x.shape[1]).double()
+    c = torch.as_tensor(coef, dtype=torch.float64, device=x.device)[:, None]
+    want = c * (hot - p)
+    low = 2 ** -25 if x.dtype == torch.float16 else 1e-36
+    bound = (HALF[x.dtype] + 2 ** -15) * want.abs() + 2 ** -15 * c.abs() * p * hot + slack * (hot - p).abs() + low
+    assert ((got.double() - want).abs() <= bound).all(), ((got.double() - want).abs() - bound).max()
+
+
+@pytest.mark.parametrize("device,vocab,dtype", SIZES)
+@pytest.mark.parametrize("where", ["preferred", "rejected"])
+@pytest.mark.parametrize("kind,smoothing", [("sigmoid", 0.0), ("sigmoid", 0.1), ("hinge", 0.0), ("ipo", 0.0)])
+def test_a_word_of_probability_0_in_a_pair(device, vocab, dtype, where, kind, smoothing):
+    """z = inf costs a pair nothing and gives it no gradient, unless the smoothed term or the square is infinite; z = -inf costs inf, its gradient is
+    that of a loss linear in z."""
+    x, y = _rows(device, 11, vocab, dtype)
+    x[2 if where == "preferred" else 7, y[2 if where == "preferred" else 7]] = -math.inf
+    cu = torch.tensor([0, 5, 11], device=device)
+    beta, won = 0.3, int(where == "rejected")
+    leaf = x.detach().requires_grad_(True)
+    loss, ranked, scores = pref.preference_loss(leaf, y, cu, None, beta, kind, smoothing, pad_idx=-1)
+    assert loss.item() == (0.0 if won and kind != "ipo" and not smoothing else math.inf) and ranked.item() == won
+    assert scores[won] == -math.inf and torch.isfinite(scores[1 - won])
+    grad = torch.autograd.grad(loss, leaf)[0]
+    if kind == "ipo":
+        assert not torch.isfinite(grad).all()
+        return
+    slope = (beta * smoothing if won else -beta * (1 - smoothing)) if kind == "sigmoid" else (0.0 if won else -beta)
+    _close(grad, [slope] * 5 + [-slope] * 6, x, y)
+
+
+@pytest.mark.parametrize("device,vocab,dtype", SIZES)
+def test_a_pair_at_infinity_leaves_the_others_alone(device, vocab, dtype):
+    x, y = _rows(device, 20, vocab, dtype, 1)
+    x[13, y[13]] = -math.inf
+    cu = torch.tensor([0, 4, 9, 12, 20], device=device)
+    with torch.no_grad():
+        loss, ranked, scores = pref.preference_loss(x, y, cu, pad_idx=-1)
+        alone = pref.preference_loss(x[:9], y[:9], cu[:3], pad_idx=-1)
+    assert loss.item() == pytest.approx(alone[0].item(), rel=1e-5) and ranked.item() == alone[1].item() + 1      # the same rows, dealt out to other threads
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_word_of_probability_0_on_both_sides_is_not_hidden(device):
+    x, y = _rows(device, 8, 50, torch.float32)
+    x[1, y[1]] = x[6, y[6]] = -math.inf
+    cu = torch.tensor([0, 3, 8], device=device)
+    for kind in pref.KINDS:
+        assert math.isnan(pref.preference_loss(x, y, cu, kind=kind, pad_idx=-1)[0].item())
+    if device == "cuda":
+        assert ops.check_status() == 0
