@@ -317,7 +317,7 @@ struct __align__(16) Mail {
 __device__ __forceinline__ float policy_coef(const Args& a, LogProb lp, float old, float adv, float ref) {
   const float ratio = expf(lp.minus(old)), held = fminf(fmaxf(ratio, a.policy.clip_low), a.policy.clip_high);
   const bool free = !(ratio * adv > held * adv);           // NaN counts as free, so that it shows
-  const float up = a.policy.ref_logprobs ? expm1f(-lp.minus(ref)) : 0.f;
+  const float up = a.policy.ref_logprobs && a.policy.kl_coef != 0.f ? expm1f(-lp.minus(ref)) : 0.f;        // a KL term that is only reported may be infinite
   return (free ? -ratio * adv : 0.f) - a.policy.kl_coef * up;
 }
 
@@ -1052,9 +1052,9 @@ __global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(kSumThreads) policy_
       double kl = 0.0;
       if (a.policy.ref_logprobs) {
         const double d = ref[j] - lp[j];
-        kl = static_cast<double>(expm1f(static_cast<float>(d))) - d;
+        kl = d < INFINITY ? static_cast<double>(expm1f(static_cast<float>(d))) - d : d;        // inf, not inf - inf, for a word of probability 0
       }
-      sums[0] += a.policy.kl_coef * kl - static_cast<double>(free ? ratio : held) * adv[j];
+      sums[0] += (a.policy.kl_coef != 0.f ? a.policy.kl_coef * kl : 0.0) - static_cast<double>(free ? ratio : held) * adv[j];
       sums[1] += kl;
       sums[2] += free ? 0.0 : 1.0;
     }

@@ -78,9 +78,10 @@ def policy_loss_reference(logits, labels, old_logprobs, advantages, ref_logprobs
     loss = torch.where(valid, -torch.where(clipped, held.detach(), ratio) * adv, zero)
     kl = zero
     if ref_logprobs is not None:
-        d = torch.where(valid, ref_logprobs.to(lp.dtype) - lp, zero)
-        kl = torch.expm1(d) - d
-        loss = loss + kl_coef * kl
+        d = torch.where(valid, ref_logprobs.to(lp.dtype) - (lp if kl_coef else lp.detach()), zero)
+        kl = torch.where(d == float("inf"), torch.exp(d), torch.expm1(d) - d)      # inf, not inf - inf, for a word of probability 0
+        if kl_coef:                                             # a KL term that is only reported may be infinite
+            loss = loss + kl_coef * kl
     return loss.sum().reshape(1), clipped.sum().to(lp.dtype).reshape(1), kl.detach().sum().reshape(1), lp.detach()
 
 

@@ -75,3 +75,35 @@ def test_a_word_of_probability_0_on_both_sides_is_not_hidden(device):
         assert math.isnan(pref.preference_loss(x, y, cu, kind=kind, pad_idx=-1)[0].item())
     if device == "cuda":
         assert ops.check_status() == 0
+
+
+@pytest.mark.parametrize("device,vocab,dtype", SIZES)
+def test_infinite_kl_terms(device, vocab, dtype):
+    """Words that the frozen model finds e^100 times as probable, and one of probability 0: the reported KL is infinite, the loss and its gradient are
+    without it those of the ratios; with it the loss is infinite.  NaN only where both models give a word probability 0."""
+    x, y = _rows(device, 8, vocab, dtype, 2)
+    x[3, y[3]] = -math.inf
+    lp = torch.log_softmax(x.double(), 1).gather(1, y[:, None]).squeeze(1)
+    adv = torch.linspace(-1, 1, 8, device=device)
+    old = (lp + 0.05).float()
+    old[3] = -3.0
+    ref = (lp + 0.3).float()
+    ref[1] = lp[1].float() + 800.0                              # e^800: beyond 64 bits, too
+    ref[3] = -4.0
+    ratio = torch.exp(lp - old.double())
+    assert ((ratio - 0.8).abs() > 0.01).all() and ((ratio - 1.2).abs() > 0.01).all()
+    held = ratio.clamp(0.8, 1.2)
+    clipped = ratio * adv > held * adv
+    leaf = x.detach().requires_grad_(True)
+    loss, n, kl, got = pref.policy_loss(leaf, y, old, adv, ref, pad_idx=-1)
+    want = -torch.minimum(ratio * adv, held * adv).sum()
+    # 8 ratios, each off by 2^-18 of at most 1.2 (of its log-probability 2^-19 and their difference's rounding), |A| <= 1
+    assert abs(loss.item() - want.item()) <= 8 * 1.2 * 2 ** -18 and n.item() == clipped.sum().item()
+    assert kl.item() == math.inf and got[3] == -math.inf
+    grad = torch.autograd.grad(loss, leaf)[0]
+    _close(grad, torch.where(clipped, 0.0, -ratio * adv), x, y, slack=1.2 * 2 ** -18)
+    with torch.no_grad():
+        loss, _, kl, _ = pref.policy_loss(x, y, old, adv, ref, kl_coef=0.1, pad_idx=-1)
+        assert loss.item() == math.inf and kl.item() == math.inf
+        ref[3] = -math.inf
+        assert math.isnan(pref.policy_loss(x, y, old, adv, ref, pad_idx=-1)[2].item())
