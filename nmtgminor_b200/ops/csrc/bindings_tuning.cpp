@@ -111,11 +111,14 @@ Tensor grad_of(const Tensor& logits, NmtgRows& r, int64_t grad, const OptTensor&
   return g;
 }
 
+// What a gradient that is made in the backward pass takes from the forward pass beside the logits
+struct Later { Tensor stat, coef, work; };
+
 // -> loss, words clipped, KL, log-probabilities, gradient (or nothing)
 std::tuple<Tensor, Tensor, Tensor, Tensor, OptTensor> policy_loss(const Tensor& logits, const Tensor& labels, const Tensor& old_logprobs,
                                                                   const Tensor& advantages, const OptTensor& ref_logprobs, double clip_low,
                                                                   double clip_high, double kl_coef, int64_t pad, double temperature,
-                                                                  int64_t grad, const OptTensor& scale_at, double scale) {
+                                                                  int64_t grad, const OptTensor& scale_at, double scale, Later* later) {
   NmtgRows r = rows_of(logits, labels, pad, temperature);
   c10::cuda::CUDAGuard guard(logits.device());
   NmtgPolicy p = {};
@@ -135,6 +138,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, OptTensor> policy_loss(const Tensor& 
   p.loss = loss.data_ptr<float>();
   p.kl = kl.data_ptr<float>();
   p.clipped = clipped.data_ptr<float>();
+  if (later) {
+    later->stat = at::empty({r.rows, 2}, f32);
+    later->coef = at::empty({r.rows}, f32);
+    r.stat = reinterpret_cast<float2*>(later->stat.data_ptr<float>());
+    p.coef = later->coef.data_ptr<float>();
+  }
   ck(nmtg_policy_loss(&r, &p, cur_stream()));
   return {loss, clipped, kl, lp, g.defined() ? OptTensor(g) : OptTensor()};
 }
@@ -143,7 +152,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, OptTensor> policy_loss(const Tensor& 
 std::tuple<Tensor, Tensor, Tensor, OptTensor> preference_loss(const Tensor& logits, const Tensor& labels, const Tensor& cu, const OptTensor& ref,
                                                               int64_t kind, double beta, double smoothing, double margin, double nll_weight,
                                                               bool average, int64_t pad, double temperature, int64_t grad,
-                                                              const OptTensor& scale_at, double scale) {
+                                                              const OptTensor& scale_at, double scale, Later* later) {
   NmtgRows r = rows_of(logits, labels, pad, temperature);
   c10::cuda::CUDAGuard guard(logits.device());
   TORCH_CHECK(cu.numel() % 2 == 1 && cu.numel() < (1 << 28), "cu must hold 2 * pairs + 1 offsets");
@@ -165,6 +174,7 @@ std::tuple<Tensor, Tensor, Tensor, OptTensor> preference_loss(const Tensor& logi
   p.seq_logprobs = seq.data_ptr<float>();
   p.loss = loss.data_ptr<float>();
   p.ranked = ranked.data_ptr<float>();
+  if (later) later->work = work;
   ck(nmtg_preference_loss(&r, &p, cur_stream()));
   return {loss, ranked, seq, g.defined() ? OptTensor(g) : OptTensor()};
 }
@@ -398,33 +408,71 @@ struct ScoresNode : Function<ScoresNode> {
   }
 };
 
-// The two losses: the gradient is made with the loss and belongs to the first backward pass
+// The two losses: the gradient is made with the loss and belongs to the first backward pass.  Not that of fp16 logits whose upstream factor is still to
+// come: rounded to fp16 without it, entries below 2^-25 would be 0 (a tenth of a vocabulary of 51865 words), whatever the loss is scaled by.  It
+// is made in the backward pass, with the factor, from the rows' sums and coefficients: the second of the paired loss's two passes as before, and one
+// more pass of the policy loss.  bf16 has the range of 32 bits: its entries are rounded once more by a factor that is no power of two.
+bool made_later(const Tensor& logits, bool prescaled) { return !prescaled && logits.scalar_type() == at::kHalf; }
+
 variable_list loss_backward(AutogradContext* ctx, const variable_list& g, size_t inputs) {
   once("preference or policy loss");
   variable_list out(inputs);
   if (!g[0].defined()) return out;
-  TORCH_CHECK(!ctx->saved_data["grad"].isNone(), "a second backward pass through a preference or policy loss: its gradient went to the first one");
-  Tensor grad = ctx->saved_data["grad"].toTensor();
-  ctx->saved_data["grad"] = c10::IValue();
-  if (!ctx->saved_data["prescaled"].toBool()) scale_rows(grad, g[0].to(at::kFloat).contiguous());
-  out[0] = grad;
+  TORCH_CHECK(!ctx->saved_data["spent"].toBool(), "a second backward pass through a preference or policy loss: its gradient went to the first one");
+  if (!ctx->saved_data["later"].toBool()) {
+    Tensor grad = ctx->saved_data["grad"].toTensor();
+    ctx->saved_data["grad"] = c10::IValue();
+    if (!ctx->saved_data["prescaled"].toBool()) scale_rows(grad, g[0].to(at::kFloat).contiguous());
+    out[0] = grad;
+  } else {
+    const auto saved = ctx->get_saved_variables();                // logits, labels, and statistics and coefficients or the workspace
+    const Tensor logits = saved[0].detach(), factor = g[0].to(at::kFloat).contiguous();
+    NmtgRows r = rows_of(logits, saved[1], ctx->saved_data["pad"].toInt(), ctx->saved_data["temperature"].toDouble());
+    c10::cuda::CUDAGuard guard(logits.device());
+    const bool inplace = ctx->saved_data["inplace"].toBool();
+    out[0] = grad_of(logits, r, inplace ? 2 : 1, factor, 1.0);
+    if (saved.size() == 4) {
+      r.stat = reinterpret_cast<float2*>(saved[2].data_ptr<float>());
+      const Tensor work = workspace(logits, r, 0);
+      ck(nmtg_row_scores_grad(&r, saved[3].data_ptr<float>(), cur_stream()));
+    } else {
+      r.workspace = saved[2].data_ptr();
+      ck(nmtg_preference_grad(&r, static_cast<int>(ctx->saved_data["pairs"].toInt()), cur_stream()));
+    }
+    if (inplace) logits.unsafeGetTensorImpl()->bump_version();
+  }
+  ctx->saved_data["spent"] = true;
   return out;
 }
-void loss_forward(AutogradContext* ctx, const Tensor& logits, const OptTensor& grad, bool inplace, bool prescaled, const variable_list& plain) {
-  ctx->saved_data["grad"] = *grad;
-  ctx->saved_data["prescaled"] = prescaled;
+void loss_forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, const OptTensor& grad, const Later& later, int64_t pairs, int64_t pad,
+                  double temperature, bool inplace, bool prescaled, const variable_list& plain) {
+  ctx->saved_data["spent"] = false;
+  ctx->saved_data["later"] = !grad.has_value();
+  if (grad.has_value()) {
+    ctx->saved_data["grad"] = *grad;
+    ctx->saved_data["prescaled"] = prescaled;
+    if (inplace) logits.unsafeGetTensorImpl()->bump_version();    // what another node has saved of the logits is gone
+  } else {
+    if (later.work.defined()) ctx->save_for_backward({logits, labels, later.work});
+    else ctx->save_for_backward({logits, labels, later.stat, later.coef});
+    ctx->saved_data["pairs"] = pairs;
+    ctx->saved_data["pad"] = pad;
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["inplace"] = inplace;
+  }
   ctx->mark_non_differentiable(plain);
   ctx->set_materialize_grads(false);
-  if (inplace) logits.unsafeGetTensorImpl()->bump_version();      // what another node has saved of the logits is gone
 }
 
 struct PolicyNode : Function<PolicyNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, const Tensor& old_logprobs, const Tensor& advantages,
                                const OptTensor& ref, double clip_low, double clip_high, double kl_coef, int64_t pad, double temperature, bool inplace,
                                const OptTensor& scale_at, double scale, bool prescaled) {
+    Later later;
+    const bool wait = made_later(logits, prescaled);
     auto [loss, clipped, kl, lp, grad] = policy_loss(logits, labels, old_logprobs, advantages, ref, clip_low, clip_high, kl_coef, pad, temperature,
-                                                     inplace ? 2 : 1, scale_at, scale);
-    loss_forward(ctx, logits, grad, inplace, prescaled, {clipped, kl, lp});
+                                                     wait ? 0 : inplace ? 2 : 1, scale_at, scale, wait ? &later : nullptr);
+    loss_forward(ctx, logits, labels, grad, later, 0, pad, temperature, inplace, prescaled, {clipped, kl, lp});
     return {loss, clipped, kl, lp};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) { return loss_backward(ctx, g, 14); }
@@ -434,9 +482,11 @@ struct PreferenceNode : Function<PreferenceNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, const Tensor& cu, const OptTensor& ref, int64_t kind,
                                double beta, double smoothing, double margin, double nll_weight, bool average, int64_t pad, double temperature,
                                bool inplace, const OptTensor& scale_at, double scale, bool prescaled) {
+    Later later;
+    const bool wait = made_later(logits, prescaled);
     auto [loss, ranked, seq, grad] = preference_loss(logits, labels, cu, ref, kind, beta, smoothing, margin, nll_weight, average, pad, temperature,
-                                                     inplace ? 2 : 1, scale_at, scale);
-    loss_forward(ctx, logits, grad, inplace, prescaled, {ranked, seq});
+                                                     wait ? 0 : inplace ? 2 : 1, scale_at, scale, wait ? &later : nullptr);
+    loss_forward(ctx, logits, labels, grad, later, cu.numel() / 2, pad, temperature, inplace, prescaled, {ranked, seq});
     return {loss, ranked, seq};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) { return loss_backward(ctx, g, 16); }
@@ -517,8 +567,16 @@ struct ActivationNode : Function<ActivationNode> {
 void bind_tuning_ops(pybind11::module& m) {
   m.def("row_scores", &row_scores);
   m.def("row_scores_grad", &row_scores_grad);
-  m.def("policy_loss", &policy_loss);
-  m.def("preference_loss", &preference_loss);
+  m.def("policy_loss", [](const Tensor& logits, const Tensor& labels, const Tensor& old_logprobs, const Tensor& advantages, const OptTensor& ref,
+                          double clip_low, double clip_high, double kl_coef, int64_t pad, double temperature, int64_t grad, const OptTensor& scale_at,
+                          double scale) {
+    return policy_loss(logits, labels, old_logprobs, advantages, ref, clip_low, clip_high, kl_coef, pad, temperature, grad, scale_at, scale, nullptr);
+  });
+  m.def("preference_loss", [](const Tensor& logits, const Tensor& labels, const Tensor& cu, const OptTensor& ref, int64_t kind, double beta,
+                              double smoothing, double margin, double nll_weight, bool average, int64_t pad, double temperature, int64_t grad,
+                              const OptTensor& scale_at, double scale) {
+    return preference_loss(logits, labels, cu, ref, kind, beta, smoothing, margin, nll_weight, average, pad, temperature, grad, scale_at, scale, nullptr);
+  });
   m.def("scale_rows", &scale_rows);
   m.def("row_scores_node", [](const Tensor& logits, const Tensor& labels, int64_t pad, double temperature) {
     return ScoresNode::apply(logits, labels, pad, temperature);

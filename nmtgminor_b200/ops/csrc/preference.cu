@@ -790,12 +790,13 @@ __global__ void __launch_bounds__(kThreads, kBlocks) held_rows_kernel(const __gr
       join_lanes(m, sum, a.k);
     }
     const LogProb lp = log_probability(xy, m, sum, a.inv_t);
-    const float c = policy_coef(a, lp, old, adv, ref) * a.inv_t * scale;
+    const float slope = policy_coef(a, lp, old, adv, ref), c = slope * a.inv_t * scale;
     if (lane == 0) {
       bc = make_float4(m, __fdividef(c, sum), c, 0.f);
       if (piece == 0) {
         a.logprobs[row] = lp.hi;
         a.w.lp[row] = lp.wide();
+        if (a.stat) { a.stat[row] = make_float2(m, sum); a.w.coef[row] = slope; }
       }
     }
   }
@@ -873,8 +874,13 @@ __global__ void __launch_bounds__(256) short_rows_kernel(const __grid_constant__
     LogProb lp = {0.f, 0.f};
     if (real) lp = log_probability(xy, m, sum, a.inv_t);
     if constexpr (kMode == kLocal) {
-      if (real) c = policy_coef(a, lp, old, adv, ref) * a.inv_t * scale;
-      if (lane == 0) { a.logprobs[row] = lp.hi; a.w.lp[row] = lp.wide(); }
+      const float slope = real ? policy_coef(a, lp, old, adv, ref) : 0.f;
+      c = slope * a.inv_t * scale;
+      if (lane == 0) {
+        a.logprobs[row] = lp.hi;
+        a.w.lp[row] = lp.wide();
+        if (a.stat) { a.stat[row] = make_float2(m, sum); a.w.coef[row] = slope; }
+      }
     } else if (lane == 0) {
       if (a.logprobs) a.logprobs[row] = lp.hi;
       if (a.stat) a.stat[row] = real ? make_float2(m, sum) : make_float2(0.f, 1.f);
@@ -1348,14 +1354,14 @@ const char* nmtg_policy_loss(const NmtgRows* r, const NmtgPolicy* p, cudaStream_
   const Work w = workspace(static_cast<char*>(r->workspace), r->rows, 0, sums_pieces(r->rows, r->vocab, r->dtype), &bytes);
   a.w.lp = w.lp;
   a.w.state = w.state;
+  a.w.coef = p->coef;
   if (r->rows <= 0) {
   } else if (static_cast<long>(r->vocab) * size <= 8L * kHeldBytes) {       // without a gradient, too: the same bits
     err = r->dtype == 0 ? launch_local<float>(a, stream) : r->dtype == 1 ? launch_local<__nv_bfloat16>(a, stream) : launch_local<__half>(a, stream);
   } else {
     a.w.part = w.part;
-    a.w.coef = w.coef;
-    a.weight = w.coef;
-    a.stat = w.stat;
+    if (!a.stat) { a.stat = w.stat; a.w.coef = w.coef; }
+    a.weight = a.w.coef;
     err = launch_pass<kScores>(a, r->dtype, stream);
     if (!err && a.g) err = launch_pass<kGrad>(a, r->dtype, stream);
   }
@@ -1397,6 +1403,16 @@ const char* nmtg_preference_loss(const NmtgRows* r, const NmtgPairs* p, cudaStre
   if (!a.g) return nullptr;
   a.weight = w.coef;
   a.stat = w.stat;
+  return launch_pass<kGrad>(a, r->dtype, stream);
+}
+
+const char* nmtg_preference_grad(const NmtgRows* r, int pairs, cudaStream_t stream) {
+  if (r->dtype < 0 || r->dtype > 2) return bad_type;
+  Args a = row_args(r);
+  long bytes;
+  a.w = workspace(static_cast<char*>(r->workspace), r->rows, pairs, sums_pieces(r->rows, r->vocab, r->dtype), &bytes);
+  a.weight = a.w.coef;
+  a.stat = a.w.stat;
   return launch_pass<kGrad>(a, r->dtype, stream);
 }
 

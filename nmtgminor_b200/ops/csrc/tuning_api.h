@@ -22,13 +22,14 @@ struct NmtgRows {
   float grad_scale;         // factor of the gradient of the two losses, times *grad_scale_at where that is not null
   const float* grad_scale_at;
   float* logprobs;          // [rows] out
-  float2* stat;             // [rows] (largest logit, sum of exp((x - largest) / T)): out of the scores, in of their gradient
+  float2* stat;             // [rows] (largest logit, sum of exp((x - largest) / T)): out of the scores and, where not null, of the policy loss; in of their
+                            // gradient
   void* workspace;          // nmtg_rows_workspace bytes (pairs: of the paired loss, otherwise 0), 16-byte aligned
 };
 long nmtg_rows_workspace(int rows, int vocab, int dtype, int pairs);
 // log-probability of every label, and `stat` where it is not null
 const char* nmtg_row_scores(const NmtgRows* r, cudaStream_t stream);
-// grad = weight[row] * d logprob / d logits, from `stat`
+// grad = weight[row] * d logprob / d logits, from `stat`; times *grad_scale_at where that is not null
 const char* nmtg_row_scores_grad(const NmtgRows* r, const float* weight, cudaStream_t stream);
 
 struct NmtgPolicy {
@@ -37,6 +38,7 @@ struct NmtgPolicy {
   const float* ref_logprobs;   // [rows] or null
   float clip_low, clip_high, kl_coef;
   float *loss, *kl, *clipped;  // [1] each, out: sums of losses and KL terms, number of clipped words
+  float* coef;                 // [rows], there where r->stat is: d loss / d logprob, the weights of a gradient that is made later
 };
 const char* nmtg_policy_loss(const NmtgRows* r, const NmtgPolicy* p, cudaStream_t stream);
 
@@ -52,6 +54,8 @@ struct NmtgPairs {
   float *loss, *ranked;        // [1] each, out: sum of losses, number of pairs ranked as preferred
 };
 const char* nmtg_preference_loss(const NmtgRows* r, const NmtgPairs* p, cudaStream_t stream);
+// the gradient by itself, from the workspace that nmtg_preference_loss has left for the same logits and `pairs` pairs
+const char* nmtg_preference_grad(const NmtgRows* r, int pairs, cudaStream_t stream);
 // r->grad *= *factor, unless it is 1
 const char* nmtg_scale_rows(const NmtgRows* r, const float* factor, cudaStream_t stream);
 

@@ -12,9 +12,10 @@ but -inf have NaN, as ``torch.log_softmax`` has.
 The gradient tensor of the two losses belongs to the backward pass, so a second pass through the same loss (``retain_graph``) is refused.
 ``grad_scale`` (a float, or one fp32 element on the logits' device that is read when the kernel runs) multiplies the gradient where it is
 computed; the upstream gradient of the loss is then taken to be 1, as in ``ops.generator_cross_entropy``.  Without it an upstream gradient
-other than 1 costs another pass over the gradient.  A backward pass can be captured in a CUDA graph where, as PyTorch asks of every operator, no graph
+other than 1 costs another pass over the gradient of fp32 and bf16 logits, and a second rounding where it is no power of two; the gradient of fp16 logits is then
+made in the backward pass, so that a scaled loss keeps what fp16 would lose.  A backward pass can be captured in a CUDA graph where, as PyTorch asks of every operator, no graph
 of the same leaves made outside the capture is alive.  ``inplace`` writes the gradient over the logits, which are consumed (as ``ops.cross_entropy``
-consumes its own).
+consumes its own): nothing else may read or change them behind the call.
 """
 from __future__ import annotations
 
