@@ -516,8 +516,7 @@ struct FlatEmbedNode : Function<FlatEmbedNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& /*anchor*/, const Tensor& tokens, const OptTensor& positions, const Tensor& table,
                         const OptTensor& pos_table, const OptTensor& gtable, const OptTensor& gpos, double scale, double p, int64_t seed,
                         int64_t stream_id, int64_t pad) {
-    ctx->saved_data["tokens"] = tokens;
-    ctx->saved_data["positions"] = positions;
+    ctx->save_for_backward({tokens, positions.has_value() ? *positions : Tensor()});      // the buffers are added to, and so not among them
     ctx->saved_data["gtable"] = gtable;
     ctx->saved_data["gpos"] = gpos;
     ctx->saved_data["words"] = table.size(0);
@@ -529,12 +528,14 @@ struct FlatEmbedNode : Function<FlatEmbedNode> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     variable_list out(12);
     if (!g[0].defined()) return out;
-    const Tensor dy = g[0].contiguous(), tokens = ctx->saved_data["tokens"].toTensor();
+    const auto saved = ctx->get_saved_variables();
+    const Tensor dy = g[0].contiguous(), tokens = saved[0];
+    const OptTensor positions = saved[1].defined() ? OptTensor(saved[1]) : OptTensor();
     const int64_t words = ctx->saved_data["words"].toInt();
     const auto numbers = ctx->saved_data["numbers"].toDoubleVector();
     const auto ids = ctx->saved_data["ids"].toIntVector();
     const auto optional = [&](const char* name) { const c10::IValue& v = ctx->saved_data[name]; return v.isNone() ? OptTensor() : OptTensor(v.toTensor()); };
-    const OptTensor gtable = optional("gtable"), gpos = optional("gpos"), positions = optional("positions");
+    const OptTensor gtable = optional("gtable"), gpos = optional("gpos");
     if (gtable.has_value()) embed_grad(tokens, OptTensor(), dy, gtable, words, words, numbers[0], numbers[1], ids[0], ids[1], ids[2]);
     if (gpos.has_value())
       embed_grad(tokens, positions.has_value() ? positions : OptTensor(at::zeros_like(tokens)), dy, gpos, words, gpos->size(0), 1.0, numbers[1], ids[0],
