@@ -37,6 +37,11 @@ def _valid(labels, vocab, pad_idx):
     return (labels != pad_idx) & (labels >= 0) & (labels < vocab)
 
 
+def _bounds(cu, rows):
+    """Offsets within the rows and in order, as the kernels take them."""
+    return cu.long().clamp(0, rows).cummax(0).values
+
+
 def token_logprobs_reference(logits, labels, pad_idx=0, temperature=1.0):
     lf = (logits if logits.dtype == torch.float64 else logits.float()) * (1.0 / temperature)
     valid = _valid(labels, logits.shape[1], pad_idx)
@@ -48,7 +53,7 @@ def preference_loss_reference(logits, labels, cu, ref_logprobs=None, beta=0.1, k
                               average=False, pad_idx=0, temperature=1.0):
     lp = token_logprobs_reference(logits, labels, pad_idx, temperature)
     valid = _valid(labels, logits.shape[1], pad_idx)
-    cu_l = cu.tolist()
+    cu_l = _bounds(cu, logits.shape[0]).tolist()
     bounds = list(zip(cu_l[:-1], cu_l[1:]))
     scores = torch.stack([lp[a:b].sum() for a, b in bounds]) if bounds else lp.new_zeros(0)
     count = torch.tensor([max(int(valid[a:b].sum()), 1) for a, b in bounds], dtype=lp.dtype, device=lp.device)
@@ -151,8 +156,11 @@ def token_logprobs(logits, labels, pad_idx: int = 0, temperature: float = 1.0):
 
 def sequence_logprobs(logprobs, cu):
     """Sums of the words' log-probabilities over the sequences of ``cu``: what ``preference_loss`` takes from the frozen model.  fp32, summed in
-    64 bits.  A sequence with a word of probability 0, or with NaN, is that and no other one."""
-    sums = lambda t: torch.diff(torch.cat([t.new_zeros(1), t.cumsum(0)])[cu.long()])
+    64 bits.  A sequence with a word of probability 0, or with NaN, is that and no other one.  Offsets are put in order as there."""
+    if logprobs.dim() != 1 or cu.dim() != 1 or cu.shape[0] < 1 or cu.dtype not in (torch.int32, torch.int64) or cu.device != logprobs.device:
+        raise ValueError("sequence_logprobs: log-probabilities [rows] and integer offsets [sequences + 1] on their device")
+    bounds = _bounds(cu, logprobs.shape[0])
+    sums = lambda t: torch.diff(torch.cat([t.new_zeros(1), t.cumsum(0)])[bounds])
     lp = logprobs.double()
     finite = torch.isfinite(lp)
     total = sums(lp.masked_fill(~finite, 0.0))
@@ -174,7 +182,8 @@ def preference_loss(logits, labels, cu, ref_logprobs: Optional[torch.Tensor] = N
                     smoothing: float = 0.0, margin: float = 0.0, nll_weight: float = 0.0, average: bool = False, pad_idx: int = 0,
                     temperature: float = 1.0, grad_scale=None, inplace: bool = False):
     """Paired preference loss.  The rows are packed sequences with offsets ``cu [2 * pairs + 1]``: sequence ``2i`` is the preferred
-    translation of pair ``i``, sequence ``2i + 1`` the rejected one; rows outside every sequence count as padding.  With ``lp`` a sequence's
+    translation of pair ``i``, sequence ``2i + 1`` the rejected one; rows outside every sequence count as padding, and
+    offsets that fall or leave the rows are put in order (running maximum, clamped).  With ``lp`` a sequence's
     summed log-probability and ``ref_logprobs [2 * pairs]`` the frozen model's (None: no reference),
 
         ``h = (lp_w - ref_w) - (lp_l - ref_l)``,  ``z = beta * h - margin``
@@ -201,7 +210,8 @@ def preference_loss(logits, labels, cu, ref_logprobs: Optional[torch.Tensor] = N
     if not _kernel_takes(logits):
         return _run_reference(preference_loss_reference(logits, labels.long(), cu, ref_logprobs, beta, kind, smoothing, margin, nll_weight,
                                                         average, pad_idx, temperature), grad_scale, logits)
-    x, y, c = _as_rows(logits), labels.long().contiguous(), cu.int().contiguous()
+    x, y = _as_rows(logits), labels.long().contiguous()
+    c = (cu if cu.dtype == torch.int32 else cu.clamp(0, logits.shape[0]).int()).contiguous()
     r = None if ref_logprobs is None else ref_logprobs.float().contiguous()
     cfg = (x, y, c, r, KINDS[kind], float(beta), float(smoothing), float(margin), float(nll_weight), bool(average), int(pad_idx), float(temperature))
     LAUNCHES[0] += 4

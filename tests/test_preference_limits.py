@@ -107,3 +107,22 @@ def test_infinite_kl_terms(device, vocab, dtype):
         assert loss.item() == math.inf and kl.item() == math.inf
         ref[3] = -math.inf
         assert math.isnan(pref.policy_loss(x, y, old, adv, ref, pad_idx=-1)[2].item())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_offsets_of_sequence_scores(device):
+    """Offsets that fall or leave the rows, as ``preference_loss`` takes them: an index out of range otherwise.  No sequences, no rows."""
+    lp = -torch.arange(1.0, 21.0, device=device)
+    bad, good = (torch.tensor(c, device=device) for c in ([-3, 5, 2, 90, 11], [0, 5, 5, 20, 20]))
+    want = torch.tensor([-15.0, 0.0, -195.0, 0.0], device=device)
+    assert torch.equal(pref.sequence_logprobs(lp, bad), want) and torch.equal(pref.sequence_logprobs(lp, good.int()), want)
+    assert pref.sequence_logprobs(lp, bad[:1]).shape == (0,)
+    assert torch.equal(pref.sequence_logprobs(lp[:0], good), torch.zeros(4, device=device))
+    x, y = _rows(device, 20, 40, torch.float32)
+    scores = pref.preference_loss(x, y, bad, pad_idx=-1)[2]
+    assert ((pref.sequence_logprobs(pref.token_logprobs(x, y, -1), bad) - scores).abs() <= 20 * 2 ** -23 * (scores.abs() + 1)).all()
+    far = torch.tensor([0, 5, 2, 2 ** 32 + 3, 11], device=device)
+    assert torch.equal(pref.preference_loss(x, y, far, pad_idx=-1)[2], scores)
+    for words, cu in ((lp[None], good), (lp, good.float()), (lp, good[:0]), (lp, good[None])):
+        with pytest.raises(ValueError):
+            pref.sequence_logprobs(words, cu)
