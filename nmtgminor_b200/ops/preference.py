@@ -45,15 +45,19 @@ def _bounds(cu, rows):
 def token_logprobs_reference(logits, labels, pad_idx=0, temperature=1.0):
     lf = (logits if logits.dtype == torch.float64 else logits.float()) * (1.0 / temperature)
     valid = _valid(labels, logits.shape[1], pad_idx)
+    lf = lf.masked_fill(~valid[:, None], 0.0)                   # NaN in rows of padding would reach their gradient
     lp = torch.log_softmax(lf, -1).gather(1, labels.masked_fill(~valid, 0)[:, None]).squeeze(1)
     return torch.where(valid, lp, torch.zeros_like(lp))
 
 
 def preference_loss_reference(logits, labels, cu, ref_logprobs=None, beta=0.1, kind="sigmoid", smoothing=0.0, margin=0.0, nll_weight=0.0,
                               average=False, pad_idx=0, temperature=1.0):
+    rows = torch.arange(logits.shape[0], device=cu.device)
+    ends = _bounds(cu, logits.shape[0])
+    labels = labels.masked_fill((rows < ends[0]) | (rows >= ends[-1]), pad_idx)
     lp = token_logprobs_reference(logits, labels, pad_idx, temperature)
     valid = _valid(labels, logits.shape[1], pad_idx)
-    cu_l = _bounds(cu, logits.shape[0]).tolist()
+    cu_l = ends.tolist()
     bounds = list(zip(cu_l[:-1], cu_l[1:]))
     scores = torch.stack([lp[a:b].sum() for a, b in bounds]) if bounds else lp.new_zeros(0)
     count = torch.tensor([max(int(valid[a:b].sum()), 1) for a, b in bounds], dtype=lp.dtype, device=lp.device)
@@ -78,10 +82,12 @@ def policy_loss_reference(logits, labels, old_logprobs, advantages, ref_logprobs
     valid = _valid(labels, logits.shape[1], pad_idx)
     zero = torch.zeros_like(lp)
     adv = advantages.to(lp.dtype)
-    ratio = torch.exp(torch.where(valid, lp - old_logprobs.to(lp.dtype), zero))
+    delta = torch.where(valid, lp - old_logprobs.to(lp.dtype), zero)
+    ratio = torch.exp(delta.detach())
     held = ratio.clamp(1.0 - clip, 1.0 + (clip if clip_high is None else clip_high))
     clipped = valid & (ratio * adv > held * adv)
-    loss = torch.where(valid, -torch.where(clipped, held.detach(), ratio) * adv, zero)
+    # where a ratio is clipped, the exponential has no part in the gradient: 0 * inf otherwise
+    loss = torch.where(valid, -torch.where(clipped, held, torch.exp(torch.where(clipped, zero, delta))) * adv, zero)
     kl = zero
     if ref_logprobs is not None:
         d = torch.where(valid, ref_logprobs.to(lp.dtype) - (lp if kl_coef else lp.detach()), zero)

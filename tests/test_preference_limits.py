@@ -126,3 +126,39 @@ def test_offsets_of_sequence_scores(device):
     for words, cu in ((lp[None], good), (lp, good.float()), (lp, good[:0]), (lp, good[None])):
         with pytest.raises(ValueError):
             pref.sequence_logprobs(words, cu)
+
+
+@pytest.mark.parametrize("device,vocab,dtype", SIZES)
+def test_what_is_left_out_has_a_gradient_of_zero(device, vocab, dtype):
+    """NaN and infinities in rows of padding and outside every sequence, in their scores and advantages, too; a ratio beyond the type's range where it is clipped."""
+    x, y = _rows(device, 9, vocab, dtype, 3)
+    lp = torch.log_softmax(x.double(), 1).gather(1, y[:, None]).squeeze(1)
+    old, adv = lp.float(), torch.ones(9, device=device)
+    y[2], y[3], y[4] = 0, -1, vocab + 4
+    for r, v in ((2, math.nan), (3, math.inf), (4, -math.inf)):
+        x[r] = v
+        old[r] = adv[r] = v
+    old[7] = lp[7].float() - 2000.0                             # ratio e^2000, held at 1.2
+    out = torch.tensor([2, 3, 4], device=device)
+    keep = torch.tensor([0, 1, 5, 6, 8], device=device)
+    leaf = x.detach().requires_grad_(True)
+    grad = torch.autograd.grad(pref.token_logprobs(leaf, y).sum(), leaf)[0]
+    assert (grad[out] == 0).all()
+    _close(grad[keep], [1.0] * 5, x[keep], y[keep])
+    loss, n, _, _ = pref.policy_loss(leaf, y, old, adv)
+    # five ratios of 1, off by their log-probabilities' 2^-19 and the rounding of ``old``, below 2^-20 for 16; the held one
+    assert abs(loss.item() + 5 + 1.2) <= 5 * 2 ** -18 and n.item() == 1
+    grad = torch.autograd.grad(loss, leaf)[0]
+    assert (grad[out] == 0).all() and (grad[7] == 0).all()
+    _close(grad[keep], [-1.0] * 5, x[keep], y[keep], slack=2 ** -18)
+    y[2:5] = 1                                                  # words, but outside the sequences
+    x[4], x[2] = x[2].clone(), 0.0
+    for cu in ([5, 7, 9], [0, 1, 2]):
+        c = torch.tensor(cu, device=device)
+        z = x if cu[0] else x.flip(0)
+        labels = y if cu[0] else y.flip(0)
+        leaf = z.detach().requires_grad_(True)
+        grad = torch.autograd.grad(pref.preference_loss(leaf, labels, c, pad_idx=-1)[0], leaf)[0]
+        inside = torch.zeros(9, dtype=torch.bool, device=device)
+        inside[cu[0]:cu[-1]] = True
+        assert (grad[~inside] == 0).all() and torch.isfinite(grad[inside]).all() and (grad[inside] != 0).any()
