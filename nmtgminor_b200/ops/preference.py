@@ -59,7 +59,7 @@ def preference_loss_reference(logits, labels, cu, ref_logprobs=None, beta=0.1, k
     valid = _valid(labels, logits.shape[1], pad_idx)
     cu_l = ends.tolist()
     bounds = list(zip(cu_l[:-1], cu_l[1:]))
-    scores = torch.stack([lp[a:b].sum() for a, b in bounds]) if bounds else lp.new_zeros(0)
+    scores = torch.stack([lp[a:b].sum() for a, b in bounds]) if bounds else lp[:0]          # no pair: a loss of 0 with a gradient of 0
     count = torch.tensor([max(int(valid[a:b].sum()), 1) for a, b in bounds], dtype=lp.dtype, device=lp.device)
     each = 1.0 / count if average else torch.ones_like(scores)
     ratio = (scores if ref_logprobs is None else scores - ref_logprobs.to(lp.dtype)) * each

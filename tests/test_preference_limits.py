@@ -162,3 +162,13 @@ def test_what_is_left_out_has_a_gradient_of_zero(device, vocab, dtype):
         inside = torch.zeros(9, dtype=torch.bool, device=device)
         inside[cu[0]:cu[-1]] = True
         assert (grad[~inside] == 0).all() and torch.isfinite(grad[inside]).all() and (grad[inside] != 0).any()
+
+
+@pytest.mark.parametrize("device,vocab,dtype", SIZES)
+def test_no_pair_at_all(device, vocab, dtype):
+    """One offset: a loss of 0, and a gradient of 0 for every row."""
+    x, y = _rows(device, 4, vocab, dtype)
+    leaf = x.detach().requires_grad_(True)
+    loss, ranked, scores = pref.preference_loss(leaf, y, torch.tensor([2], device=device), pad_idx=-1)
+    assert loss.item() == 0 and ranked.item() == 0 and scores.shape == (0,)
+    assert (torch.autograd.grad(loss, leaf)[0] == 0).all()
