@@ -172,3 +172,17 @@ def test_no_pair_at_all(device, vocab, dtype):
     loss, ranked, scores = pref.preference_loss(leaf, y, torch.tensor([2], device=device), pad_idx=-1)
     assert loss.item() == 0 and ranked.item() == 0 and scores.shape == (0,)
     assert (torch.autograd.grad(loss, leaf)[0] == 0).all()
+
+
+@pytest.mark.parametrize("device,dtype", [("cpu", torch.float64), *(pytest.param("cuda", d, marks=pytest.mark.gpu) for d in (torch.float32, torch.bfloat16))])
+@pytest.mark.parametrize("size", [1e-1, 1e-3, 1e-5])
+def test_kl_terms_near_0(device, dtype, size):
+    """A single word: its log-probability is 0 exactly, and e^d - d - 1 as good as its rounding."""
+    x = torch.zeros(700, 1, dtype=dtype, device=device)
+    y = torch.zeros(700, dtype=torch.int64, device=device)
+    ref = ((torch.rand(700, generator=torch.Generator().manual_seed(5)) - 0.5) * size).to(device)
+    d = ref.double()
+    want = (d ** 2 / 2 + d ** 3 / 6 + d ** 4 / 24 + d ** 5 / 120 + d ** 6 / 720 + d ** 7 / 5040).sum().item()       # the next term: below 2^-36 of it
+    kl = pref.policy_loss(x, y, ref, ref, ref, kl_coef=0.1, pad_idx=-1)[2].item()
+    # the result is rounded to 32 bits; a double's expm1(d) - d is off by some 2^-52 d, of d^2 / 2
+    assert abs(kl - want) <= (2 ** -23 + 2 ** -49 / size) * want
