@@ -420,8 +420,7 @@ variable_list loss_backward(AutogradContext* ctx, const variable_list& g, size_t
   if (!g[0].defined()) return out;
   TORCH_CHECK(!ctx->saved_data["spent"].toBool(), "a second backward pass through a preference or policy loss: its gradient went to the first one");
   if (!ctx->saved_data["later"].toBool()) {
-    Tensor grad = ctx->saved_data["grad"].toTensor();
-    ctx->saved_data["grad"] = c10::IValue();
+    Tensor grad = ctx->get_saved_variables()[0].detach();
     if (!ctx->saved_data["prescaled"].toBool()) scale_rows(grad, g[0].to(at::kFloat).contiguous());
     out[0] = grad;
   } else {
@@ -449,9 +448,9 @@ void loss_forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labe
   ctx->saved_data["spent"] = false;
   ctx->saved_data["later"] = !grad.has_value();
   if (grad.has_value()) {
-    ctx->saved_data["grad"] = *grad;
     ctx->saved_data["prescaled"] = prescaled;
     if (inplace) logits.unsafeGetTensorImpl()->bump_version();    // what another node has saved of the logits is gone
+    ctx->save_for_backward({*grad});                              // as the logits' version is now: a change behind the call is refused
   } else {
     if (later.work.defined()) ctx->save_for_backward({logits, labels, later.work});
     else ctx->save_for_backward({logits, labels, later.stat, later.coef});

@@ -105,3 +105,42 @@ def test_one_backward_pass_of_a_loss(which, dtype):
     outside = x.detach().requires_grad_(True)                   # no pair at all: a gradient of zeros
     assert (torch.autograd.grad(pref.preference_loss(outside, y, torch.zeros(1, dtype=torch.int32, device=DEV))[0] * 3.0, outside)[0] == 0).all()
     assert ops.check_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["preference", "policy"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("scale", [None, 0.5])
+def test_what_a_loss_keeps_is_a_saved_tensor(which, dtype, scale):
+    """The gradient (or what it is made of) can be moved off the GPU by hooks, and is freed with the pass; logits consumed in place and changed behind
+    the call are refused."""
+    x, y, loss, coef, off = _case(20, 9001, dtype, which)
+    kw = {} if scale is None else {"grad_scale": scale}
+    leaf = x.detach().requires_grad_(True)
+    want = torch.autograd.grad(loss(leaf, **kw) * 2.0, leaf)[0]
+    moved = []
+
+    def pack(t):
+        moved.append(t.numel())
+        return t.cpu()
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t.to(DEV)):
+        value = loss(leaf, **kw)
+    assert max(moved) == x.numel()
+    assert torch.equal(torch.autograd.grad(value * 2.0, leaf)[0], want)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    value = loss(leaf, **kw)
+    grad = torch.autograd.grad(value * 2.0, leaf)[0]
+    assert torch.equal(grad, want)
+    del grad
+    assert torch.cuda.memory_allocated() - before <= 1024       # the loss itself
+    with pytest.raises(RuntimeError, match="second"):
+        torch.autograd.grad(value, leaf)
+    logits = x.detach().clone().requires_grad_(True) * 1.0
+    value = loss(logits, inplace=True, **kw)
+    with torch.no_grad():
+        logits.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        value.backward()
+    assert ops.check_status() == 0
