@@ -19,6 +19,7 @@
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <atomic>
 #include <climits>
 #include <stdint.h>
 #include "b200_ptx.cuh"
@@ -1129,14 +1130,13 @@ const char* launch_rows(const Args& from, cudaStream_t stream) {
   // the attribute belongs to a device's context: set at every call, which costs less than keeping account of the devices
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSlots * kVecs * kCompute * 16);
   if (e != cudaSuccess) return cudaGetErrorString(e);
-  static int blocks[kVecs + 1] = {};    // that an SM holds; all GPUs of a machine are alike
-  int& held = blocks[across / kCompute];
+  static std::atomic<int> blocks[kVecs + 1];      // that an SM holds, 0: not asked for yet; all GPUs of a machine are alike, and all threads find the same
+  int held = blocks[across / kCompute].load(std::memory_order_relaxed);
   if (held == 0) {
-    int n = 0;
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kCompute + 32, smem);
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kernel, kCompute + 32, smem);
     if (e != cudaSuccess) return cudaGetErrorString(e);
-    if (n < 1) return "preference: no block fits an SM";
-    held = n;
+    if (held < 1) return "preference: no block fits an SM";
+    blocks[across / kCompute].store(held, std::memory_order_relaxed);
   }
   const long items = static_cast<long>(a.rows) * a.pieces, most = static_cast<long>(held) * num_sms();
   if (4 * items + (1L << 20) >= 1L << 31) return "preference: too many rows";

@@ -144,3 +144,29 @@ def test_what_a_loss_keeps_is_a_saved_tensor(which, dtype, scale):
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         value.backward()
     assert ops.check_status() == 0
+
+
+@pytest.mark.gpu
+def test_losses_from_several_threads():
+    """Threads with a stream each, first calls among them, of rows of every length: the results of calls one after another."""
+    from concurrent.futures import ThreadPoolExecutor
+    cases = [_case(11, vocab, dtype, which, 7) for vocab in (2600, 5300, 12000, 17000, 33000, 66000) for dtype in (torch.bfloat16, torch.float32)
+             for which in ("preference", "policy")]
+    streams = [torch.cuda.Stream() for _ in range(6)]
+    torch.cuda.synchronize()
+
+    def run(i):
+        x, y, loss = cases[i % len(cases)][:3]
+        with torch.cuda.stream(streams[i % 6]):
+            leaf = x.detach().requires_grad_(True)
+            out = loss(leaf), pref.token_logprobs(leaf, y)
+            grads = [torch.autograd.grad(o.sum(), leaf)[0] for o in out]
+            streams[i % 6].synchronize()
+        return [o.detach() for o in out] + grads
+
+    with ThreadPoolExecutor(6) as pool:
+        together = list(pool.map(run, range(2 * len(cases))))
+    alone = [run(i) for i in range(len(cases))]
+    for i, got in enumerate(together):
+        assert all(torch.equal(a, b) for a, b in zip(got, alone[i % len(cases)]))
+    assert ops.check_status() == 0
