@@ -307,7 +307,7 @@ def _restore8(kept):
 
 
 def _long_sum_parts(rows, gw):
-    """Parts of a weight gradient's sum over ``rows``, about 2048 each: fewer of the accumulator's truncated additions in a row (8200 rows, 1024 x 4096:
+    """Parts of a kept layer's or block's weight gradient's sum over ``rows``, about 2048 each: fewer of the accumulator's truncated additions in a row (8200 rows, 1024 x 4096:
     2.1e-6 of the gradient off instead of 9.1e-6, 62.0 us instead of 60.5).  0, the product's own choice, where there are few rows, or
     few tiles, whose sums it cuts by itself."""
     tiles = -(-gw.shape[0] // 256) * -(-gw.shape[1] // 256)
@@ -422,6 +422,7 @@ class _MlpFn(torch.autograd.Function):
         act, p1, p2, seed, sid1, sid2, has_res = ctx.cfg
         gw1, gb1, gw2, gb2 = ctx.g
         dy = dy.contiguous()
+        parts = _long_sum_parts if kept_h is not None else lambda rows, gw: 0
         if kept_h is not None:
             from .kept import restore_activated
             x = _restore8(kept_x) if gw1 is not None else None
@@ -435,7 +436,7 @@ class _MlpFn(torch.autograd.Function):
         else:
             dz2 = ext().dropout_add(dy, None, p2, seed, sid2) if p2 > 0.0 else dy
         if gw2 is not None:
-            gemm(dz2, h, gw2, a_mn_major=True, b_mn_major=True, accumulate=True, allow_split_k=True)
+            gemm(dz2, h, gw2, a_mn_major=True, b_mn_major=True, accumulate=True, allow_split_k=True, split_k=parts(dz2.shape[0], gw2))
         if gb2 is not None and not fused_gb2:
             ext().colsum(dz2, gb2)
         dz1 = torch.empty_like(h)
@@ -449,7 +450,7 @@ class _MlpFn(torch.autograd.Function):
             gemm(dz2, w2, dz1, b_mn_major=True, aux=z, act=_ACT_BWD[act], dropout_p=p1, seed=seed, stream_id=sid1,
                  gather=ctx.gathers[1])
         if gw1 is not None:
-            gemm(dz1, x, gw1, a_mn_major=True, b_mn_major=True, accumulate=True, allow_split_k=True)
+            gemm(dz1, x, gw1, a_mn_major=True, b_mn_major=True, accumulate=True, allow_split_k=True, split_k=parts(dz1.shape[0], gw1))
         if gb1 is not None and not fused_gb1:
             ext().colsum(dz1, gb1)
         dx = torch.empty((dz1.shape[0], w1.shape[1]), dtype=torch.bfloat16, device=dz1.device)
