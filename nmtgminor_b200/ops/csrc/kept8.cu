@@ -7,8 +7,8 @@
 //
 //   quantise:   x -> codes                         restore:    codes -> x' and, where asked for, dropout(act(x'))
 //   forward:    z -> dropout(act(z)), codes        backward:   dy, codes -> dropout-mask(dy) act'(z')
-// One pass each, bound by memory.  A thread has one 16-byte vector, 4 (16-bit types) or 8 (fp32) lanes a block, whose largest magnitude
-// meets in shuffles.  For 16-bit types GELU takes one exponential and one division for the function and its slope together: with
+// One pass each, bound by memory.  A thread has 32 bytes of a 16-bit type where whole blocks follow one another (2 lanes to a block of 32), otherwise one
+// 16-byte vector (4 lanes; of fp32 8) or one element (32); a block's largest magnitude meets in shuffles.  For 16-bit types GELU takes one exponential and one division for the function and its slope together: with
 // t = 1 / (1 + p |z|) the tail Q(|z|) = exp(-z^2 / 2) (c1 t + ... + c7 t^7), fitted over the whole range to 1.1e-6 of itself (the
 // form of Hastings' approximation with coefficients of our own), against the 2^-9 and 2^-12 of the rounding that follows; erff and expf
 // would take longer than the bytes.  fp32 results use erfcf and expf.  Compiled without fast math: codes, restored

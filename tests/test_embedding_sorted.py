@@ -36,7 +36,8 @@ def test_refusals_on_the_cpu():
     _refusals("cpu")
 
 
-# rows: the counting kernel up to 8192, radix passes beyond; vocabularies of 1 to 3 digits
+# rows: one tile up to 2048, merged tiles up to 16384 (keys of up to 18 bits), radix passes beyond; vocabularies of 1 to 3 digits.  Where exactly the
+# kernels change: test_embedding_sorted_edges.py
 CASES = [(1, 1, 8), (7, 5, 1), (64, 3, 40), (65, 1000, 256), (1000, 7, 200), (4095, 32000, 64), (8192, 700, 16), (8193, 700, 16), (9000, 32000, 136),
          (20000, 250054, 24), (40000, 2, 8), (5000, 600000, 8), (12345, 1100000, 4)]
 
