@@ -284,7 +284,7 @@ __device__ __noinline__ void pair_loss(const Args& a, int p, double sw, double s
     const double z = q.beta * h - q.margin;
     if (q.kind == 1) {
       loss = z < 1.0 ? 1.0 - z : (z >= 1.0 ? 0.0 : z);             // the last: NaN
-      slope = z < 1.0 ? -static_cast<double>(q.beta) : 0.0;
+      slope = z < 1.0 ? -static_cast<double>(q.beta) : (z >= 1.0 ? 0.0 : z);      // so that NaN shows, as under the other kinds
     } else {
       const double less = exp(-fabs(z)), soft = log1p(less), eps = q.smoothing;
       const double up = z >= 0.0 ? 1.0 / (1.0 + less) : less / (1.0 + less);      // sigmoid(z)

@@ -68,7 +68,10 @@ def preference_loss_reference(logits, labels, cu, ref_logprobs=None, beta=0.1, k
         loss = (h - 0.5 / beta) ** 2
     else:
         z = beta * h - margin
-        loss = torch.relu(1.0 - z) if kind == "hinge" else -(1.0 - smoothing) * F.logsigmoid(z)
+        if kind == "hinge":
+            loss = torch.relu(1.0 - z) * torch.where(torch.isnan(z), z, torch.ones_like(z)).detach()      # NaN shows in the gradient, too
+        else:
+            loss = -(1.0 - smoothing) * F.logsigmoid(z)
         if smoothing:                                           # 0 * inf at z = inf otherwise
             loss = loss - smoothing * F.logsigmoid(-z)
     if nll_weight:

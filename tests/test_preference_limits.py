@@ -186,3 +186,18 @@ def test_kl_terms_near_0(device, dtype, size):
     kl = pref.policy_loss(x, y, ref, ref, ref, kl_coef=0.1, pad_idx=-1)[2].item()
     # the result is rounded to 32 bits; a double's expm1(d) - d is off by some 2^-52 d, of d^2 / 2
     assert abs(kl - want) <= (2 ** -23 + 2 ** -49 / size) * want
+
+
+@pytest.mark.parametrize("device,vocab,dtype", SIZES)
+@pytest.mark.parametrize("kind", list(pref.KINDS))
+def test_a_pair_without_a_value_shows_in_its_gradient(device, vocab, dtype, kind):
+    """inf - inf, or NaN in one of its rows: NaN in the gradient of every row of the pair, under each kind; the next pair is not touched."""
+    x, y = _rows(device, 12, vocab, dtype, 4)
+    cu = torch.tensor([0, 3, 8, 10, 12], device=device)
+    for damage in (lambda z: z[1].index_fill_(0, y[1], -math.inf) + z[6].index_fill_(0, y[6], -math.inf), lambda z: z[2].fill_(math.nan)):
+        leaf = x.clone()
+        damage(leaf)
+        leaf.requires_grad_(True)
+        loss = pref.preference_loss(leaf, y, cu, kind=kind, pad_idx=-1)[0]
+        grad = torch.autograd.grad(loss, leaf)[0]
+        assert math.isnan(loss.item()) and torch.isnan(grad[:8]).all() and torch.isfinite(grad[8:]).all()
