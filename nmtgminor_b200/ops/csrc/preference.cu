@@ -11,10 +11,12 @@
 // Bound by memory in 32 bits, in every gradient pass and where one pass does all.  The sums of 16-bit logits, two exponentials to a 32-bit word, keep the
 // memory at 0.8 of its rate and the exponentials (16 a cycle and SM) at 0.7 of theirs.
 // 8200 rows of 32000 in bf16: scores 96 us (floor 81), gradients 165 (163), paired loss 255 (163, of the two passes 244); policy loss of
-// 15360 rows 317 (305).
+// 15360 rows 317 (305).  Called without a pause for seconds the policy loss reaches the card's power limit (1014 W, 1620 MHz): 382 us then, the paired loss 260.
 //
 // All sums over rows are taken in one order in 64 bits: results do not depend on which block was first.
 // This file is compiled without fast math: expf and logf below are the accurate ones, ex2 where it is asked for.
+// Exponentials, ratios and a row's coefficient are in 32 bits, off by 2^-16 and less: for 16-bit results far below their rounding, for fp32 logits a choice,
+// since a row's sum has no more than 2^-19 itself.  Log-probabilities are held in two floats, what is summed of them (scores, losses, KL terms) in 64 bits.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
@@ -169,11 +171,12 @@ __device__ __forceinline__ float warp_max(float v) {
 __device__ __forceinline__ void copy16(uint4* to, const uint4* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
 }
-// Rows are gone through from the last to the first where they are read first: whatever has made the logits has left the last ones in L2.  The gradients behind
-// the sums go from the first to the last, and find in L2 what the sums read last, the first `stays` rows; the others pass through it first out.
+// Rows are gone through from the last to the first where they are read first.  The gradients behind the sums go from the first to the last, and find in L2
+// what the sums read last, the first `stays` rows; the others pass through it first out.
 // (Paired loss of 8200 rows of 32000 in bf16: 276 us with both in one order, 273 in opposite ones, 261 so; 8200 rows of 8000 in fp32 151, 144, 136.
-// 48 to 80 MB alike, 112 of the 126 that L2 has 2 % slower.  Behind a copy of the logits: scores of
-// the 8200 rows 102 us from the first row on, 94 from the last, paired loss 264 and 253.)
+// 48 to 80 MB alike, 112 of the 126 that L2 has 2 % slower.  From the last row rather than from the first, since what writes logits row by row leaves the last
+// rows in L2: behind a copy scores of the 8200 rows 94 us, from the first row 102.  The output layer's product leaves the last columns of all rows
+// there, and either order takes 98 behind it, the paired loss 258.)
 constexpr long kStaying = 48L << 20;
 __device__ __forceinline__ uint64_t policy_of(bool stay) {
   uint64_t first, normal;
