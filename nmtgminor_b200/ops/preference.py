@@ -166,8 +166,8 @@ def token_logprobs(logits, labels, pad_idx: int = 0, temperature: float = 1.0):
 def sequence_logprobs(logprobs, cu):
     """Sums of the words' log-probabilities over the sequences of ``cu``: what ``preference_loss`` takes from the frozen model.  fp32, summed in
     64 bits.  A sequence with a word of probability 0, or with NaN, is that and no other one.  Offsets are put in order as there."""
-    if logprobs.dim() != 1 or cu.dim() != 1 or cu.shape[0] < 1 or cu.dtype not in (torch.int32, torch.int64) or cu.device != logprobs.device:
-        raise ValueError("sequence_logprobs: log-probabilities [rows] and integer offsets [sequences + 1] on their device")
+    if logprobs.dim() != 1 or cu.dim() != 1 or cu.shape[0] < 1:
+        raise ValueError("sequence_logprobs: log-probabilities [rows] and offsets [sequences + 1], got %s and %s" % (tuple(logprobs.shape), tuple(cu.shape)))
     bounds = _bounds(cu, logprobs.shape[0])
     sums = lambda t: torch.diff(torch.cat([t.new_zeros(1), t.cumsum(0)])[bounds])
     lp = logprobs.double()

@@ -123,7 +123,8 @@ def test_offsets_of_sequence_scores(device):
     assert ((pref.sequence_logprobs(pref.token_logprobs(x, y, -1), bad) - scores).abs() <= 20 * 2 ** -23 * (scores.abs() + 1)).all()
     far = torch.tensor([0, 5, 2, 2 ** 32 + 3, 11], device=device)
     assert torch.equal(pref.preference_loss(x, y, far, pad_idx=-1)[2], scores)
-    for words, cu in ((lp[None], good), (lp, good.float()), (lp, good[:0]), (lp, good[None])):
+    assert torch.equal(pref.sequence_logprobs(lp, good.cpu()), want)
+    for words, cu in ((lp[None], good), (lp, good[:0]), (lp, good[None])):
         with pytest.raises(ValueError):
             pref.sequence_logprobs(words, cu)
 
