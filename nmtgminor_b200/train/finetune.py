@@ -200,7 +200,7 @@ def policy_step(model, batch, old_logprobs, advantages, ref_logprobs=None, grad_
     if advantages.dim() == 1 and advantages.shape[0] == cu.shape[0] - 1 and advantages.shape[0] != logits.shape[0]:
         rows = torch.arange(logits.shape[0], device=cu.device)
         of = torch.bucketize(rows, cu[1:].long(), right=True)                 # rows behind the last sentence are padding
-        advantages = advantages[of.clamp(max=advantages.shape[0] - 1)]
+        advantages = torch.cat([advantages, advantages.new_zeros(1)])[of]
     return preference.policy_loss(logits, labels, old_logprobs, advantages, ref_logprobs, pad_idx=getattr(model, "pad_idx", 0),
                                   grad_scale=grad_scale, inplace=True, **loss)
 
